@@ -256,8 +256,9 @@ def _handles(s, case):
     if case["op"] == "verify":
         s["verifier"] = DraftVerifier(case["batch"], case["drafts"], case["vocab"], device=DEV)
     elif case["op"] != "rope" or case["paged"]:
+        places = s["positions"] if case["op"] == "evict" else None
         s["cache"] = PagedKVCache.from_tensors(s["k_pages"], s["v_pages"], s["table"], s["lengths"], scores=s.get("scores"),
-                                               positions=s.get("positions"), next_pos=s.get("next_pos"))
+                                               positions=places, next_pos=s.get("next_pos"))
 
 
 # -- one pass ----------------------------------------------------------------
