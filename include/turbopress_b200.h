@@ -408,6 +408,158 @@ TP_API tp_status tp_step_status(const void* workspace, void* stream);
  * the call. */
 TP_API tp_status tp_step_set_wait(void* image_host, int64_t barrier_us, int extra_arrivals);
 
+/* ------------------------------------------------------------------------
+ * Serving from a paged key-value cache: rotary positions with the append,
+ * attention of new tokens, eviction by accumulated attention weight, and
+ * verification of drafted tokens.  They stand beside the decode step, whose
+ * caches are contiguous and whose step is one token: here a cache is a pool
+ * of pages shared by all sequences, a step may carry several tokens per
+ * sequence, and a cache can be held to a budget of slots.
+ * ---------------------------------------------------------------------- */
+
+/* One layer's cache.  Slot s of sequence b lies in page
+ * block_table[b][s / page_size] at offset s % page_size; element i of kv head
+ * h there is at page*page_stride + h*head_stride + offset*token_stride + i
+ * (elements, the same for k_pages and v_pages; int64, so a pool may pass 2^31
+ * elements).  A page id outside [0, num_pages) is a page the sequence does
+ * not have: nothing is read from or written to it.  lengths[b] counts the
+ * slots in use before the step's own tokens; a negative length marks an idle
+ * sequence.  Both are device data, checked where they are used. */
+typedef struct tp_paged_cache {
+  void* k_pages;
+  void* v_pages;
+  const int32_t* block_table;  /* [batch][table_stride], max_pages used           */
+  const int32_t* lengths;      /* [batch]                                         */
+  float* scores;               /* [batch][kv_heads][max_pages*page_size], or NULL:
+                                  each slot's accumulated attention weight        */
+  int32_t* positions;          /* the same shape, or NULL: each slot's position   */
+  int64_t num_pages, page_stride, head_stride, token_stride, table_stride;
+  int32_t batch, kv_heads, head_dim, page_size, max_pages;
+  int32_t dtype;               /* of the pages: TP_F16 or TP_BF16                 */
+} tp_paged_cache;
+
+typedef struct tp_rotary_args {
+  const void* q;            /* [tokens][q_heads][head_dim] by the strides below     */
+  const void* k;            /* [tokens][kv_heads][head_dim]                         */
+  const void* v;            /* likewise; read only when a cache is given            */
+  void* q_out;              /* contiguous; may be q itself                          */
+  void* k_out;              /* contiguous, may be k itself; unused with a cache     */
+  const int64_t* positions; /* [tokens], or NULL: base[b] + i                       */
+  const int32_t* base;      /* [tokens / seq] first position of each sequence       */
+  const uint64_t* freq;     /* [rot_dim/2] turns per position, in units of 2^-64    */
+  const void* q_norm;       /* [head_dim] RMS-norm weights of the heads, or NULL    */
+  const void* k_norm;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t tokens;           /* sequences * seq                                      */
+  int32_t seq;              /* tokens per sequence                                  */
+  int32_t q_heads, kv_heads, head_dim, rot_dim;
+  int32_t dtype;            /* of q, k, v, norms and outputs                        */
+  int32_t interleaved;      /* pairs (2p, 2p+1) instead of (p, p + rot_dim/2)       */
+  int32_t inverse;          /* rotate by the negative angle (also the gradient)     */
+  float scale;              /* factor on cos and sin                                */
+  float eps;                /* of the head norms                                    */
+} tp_rotary_args;
+
+/* Rotary positions of q and k: optional RMS norm of each head, then for every
+ * pair (i, j) of the first rot_dim elements
+ *   y_i = x_i c - x_j s,  y_j = x_j c + x_i s,  c, s = scale * cos, sin(angle)
+ * with the angle of position p and pair n being p * freq[n] turns (exact
+ * modulo one turn for any position), arithmetic in fp32 and one rounding.
+ * With a cache, k goes to the pages instead of k_out, at slots lengths[b] + i,
+ * v beside it, and (where the cache has them) positions are recorded and
+ * scores cleared; lengths do not change.  Tokens of idle sequences, past the
+ * capacity or without a page are not stored.  head_dim <= 256, both even. */
+TP_API tp_status tp_rotary(const tp_rotary_args* args, const tp_paged_cache* cache, void* stream);
+
+/* Attention of each sequence's last `tokens` tokens over its pages:
+ *   out[b][j][h] = sum_s p_s v_s,  p = softmax over s < lengths[b] + j + 1 of
+ *   softmax_scale * q[b][j][h] . k_s
+ * for query token j, head h reading kv head h / (q_heads / kv_heads): token j
+ * sees the cached slots and the step's own up to itself (append them first).
+ * Slots without a page are not seen.  A row that sees nothing (an idle
+ * sequence) gives zeros and lse -inf; what unseen slots hold, NaN included,
+ * has no effect.  Scores, softmax statistics and sums are fp32; products run
+ * on the tensor cores from the 16-bit operands, probabilities as two 16-bit
+ * terms.  Deterministic. */
+typedef struct tp_paged_attn_args {
+  const void* q;        /* contiguous [batch][tokens][q_heads][head_dim], 16-byte aligned */
+  void* out;            /* the same shape and dtype (the pages')                          */
+  float* lse;           /* [batch][tokens][q_heads] log-sum-exp of the scores, or NULL    */
+  int32_t tokens, q_heads;
+  float softmax_scale;
+  int32_t accumulate;   /* add each seen slot's probability, summed over the step's rows
+                           of its kv head, to cache->scores                               */
+} tp_paged_attn_args;
+
+/* Workspace of tp_paged_attn for a cache's sizes (batch, kv_heads, head_dim,
+ * page_size and max_pages of `cache` are read): zero-filled once, left fit
+ * for the next call of any such size that it can hold; one per stream.  Minus
+ * the status on bad arguments. */
+TP_API int64_t tp_paged_attn_workspace_bytes(const tp_paged_cache* cache, int tokens, int q_heads, int accumulate);
+TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_cache* cache, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
+/* Eviction: of each sequence's slots keep the `budget` that come first by
+ * (guarded, score, lower slot), per kv head, where a slot is guarded when its
+ * position is below `sinks` or at least next_pos[b] - recent.  Scores compare
+ * as numbers; a NaN ranks above all others and below a guarded slot.  The
+ * kept slots above the budget move, in order, into the freed ones below it
+ * (sources and destinations are disjoint: in place, and no more bytes than
+ * must move), so the caches need not be in order of position afterwards;
+ * attention does not depend on the order.  new_scores / new_positions receive
+ * the kept slots' entries (0 and -1 past them) and new_lengths the lengths;
+ * the cache's own lengths, scores and positions do not change, and may not
+ * overlap them.  Sequences within the budget (or idle) are copied as they are.
+ * The pages of a sequence over its budget must be its own. */
+typedef struct tp_evict_args {
+  const int32_t* next_pos;  /* [batch] position after the latest token              */
+  int32_t* new_lengths;     /* [batch]                                              */
+  float* new_scores;        /* [batch][kv_heads][max_pages*page_size]               */
+  int32_t* new_positions;   /* likewise                                             */
+  int32_t budget;           /* slots to keep, >= 1                                  */
+  int32_t recent, sinks;    /* >= 0, recent + sinks <= budget                       */
+} tp_evict_args;
+
+/* Workspace (no zero-fill needed; one per stream); minus the status on bad
+ * arguments, TP_ERR_UNSUPPORTED above 2^20 slots per sequence. */
+TP_API int64_t tp_cache_evict_workspace_bytes(const tp_paged_cache* cache, int budget);
+TP_API tp_status tp_cache_evict(const tp_evict_args* args, const tp_paged_cache* cache, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
+/* Verification of drafted tokens (speculative sampling), from given random
+ * numbers.  Row k of a sequence's logits is the target's distribution after k
+ * drafts.  With temperature t > 0, p_k = softmax(logits[k] / t); draft k is
+ * accepted while uniforms[k] * q_k(draft) < p_k(draft), q_k being
+ * draft_probs[k], or 1 at the draft without them (a greedy or looked-up
+ * draft).  At the first rejection the next token is drawn from
+ * max(p_k - q_k, 0) (from p_k should that be zero everywhere), after
+ * acceptance of all from p_K: the token i of largest r_i / noise[i] (noise:
+ * independent exponentials), lower i on equality.  With t = 0, drafts are
+ * accepted while they are the argmax of their row (lower index on equality, a
+ * NaN above all), and the next token is the argmax.  A draft outside the
+ * vocabulary is rejected; a next token of -1 says that the row had none with
+ * a positive probability. */
+typedef struct tp_verify_args {
+  const void* logits;         /* [batch][drafts + 1][vocab] by the strides           */
+  int64_t batch_stride, row_stride;  /* elements                                     */
+  const int64_t* draft_tokens;       /* [batch][drafts]                              */
+  const float* draft_probs;   /* [batch][drafts][vocab] or NULL                      */
+  const float* uniforms;      /* [batch][drafts] in [0, 1); NULL if all greedy       */
+  const float* noise;         /* [batch][vocab]; NULL if all greedy                  */
+  const float* temperature;   /* [batch], or NULL: all greedy                        */
+  const int32_t* counts;      /* [batch] drafts in use (0..drafts), or NULL: all     */
+  int32_t* accepted;          /* [batch]                                             */
+  int64_t* tokens;            /* [batch][drafts + 1]: accepted drafts, the next
+                                 token, then -1                                      */
+  int32_t batch, drafts, vocab;
+  int32_t dtype;              /* of the logits                                       */
+} tp_verify_args;
+
+/* Workspace: zero-filled once, left fit for the next call of any size that it
+ * can hold; one per stream.  Minus the status on bad arguments. */
+TP_API int64_t tp_verify_workspace_bytes(int batch, int drafts, int vocab);
+TP_API tp_status tp_verify_drafts(const tp_verify_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Reference-order GEMV straight from the format-v2 streams, any bits in 1..7:
  * y[B, n] = z[B, d] @ decode_rows^T (+ bias), z fp32 rotated activations.
  * Used for payloads the native stream does not cover (bits 5..7) and as an

@@ -1,0 +1,790 @@
+// Attention of new tokens over a paged key-value cache.
+//
+// Mathematics: with s = scale * q . k in log2 units, a pass over the slots
+// keeps m = max s, l = sum 2^(s - m) and o = sum 2^(s - m) v; two such states
+// join as m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m), o likewise, and
+// out = o / l.  m, l, o, s are fp32.  The products run on the tensor cores
+// with fp32 accumulation; q, k, v enter exactly (they are 16-bit) and the
+// probabilities as two 16-bit terms (p = hi + lo, 2^-16 relative or better),
+// so the output is rounded once.
+//
+// Bound: memory.  A cached token costs 4 * head_dim bytes per kv head and
+// 4 * head_dim * rows flops; with few rows (query heads of a kv head times
+// step tokens) warp-level MMAs at m = 16 rows keep far ahead of HBM, and
+// their operands come straight from the shared-memory tiles.
+//
+// Split: the 64-token tiles of all (sequence, row tile, kv head) items form
+// one index space, cut into equal runs, one per resident CTA; lengths are read
+// on the device, so ragged batches balance by themselves.  A run that ends
+// inside an item leaves (m, l, o) in the workspace and the item's last CTA to
+// arrive (a counter at the item's first CTA) joins them in run order, so the
+// result does not depend on timing.
+//
+// Tile: each of the four warps copies its own 16 tokens of K and V with
+// 16-byte asynchronous copies (page ids one tile ahead, unseen slots
+// zero-filled, so whatever they hold stays out) and, up to 16 rows, also
+// consumes only those: no CTA barrier in the loop.  With more rows the warps
+// share the tile: MT row tiles of 16, 4/MT warps each.
+#include <algorithm>
+
+#include "tp_decode.cuh"
+#include "tp_paged.cuh"
+
+using namespace tp;
+
+namespace {
+
+constexpr int kPaThreads = 128;
+constexpr int kPaWarps = 4;
+constexpr int kPaTile = 64;
+constexpr int kPaMaxCtas = 512;
+constexpr int kPaCounterBytes = kPaMaxCtas * 4;
+
+struct AttnParams {
+  const void* q;
+  void* out;
+  float* lse;
+  const void* k_pages;
+  const void* v_pages;
+  const int32_t* block_table;
+  const int32_t* lengths;
+  float* scores;
+  int64_t num_pages, page_stride, head_stride, token_stride, table_stride;
+  int batch, tokens, q_heads, kv_heads, group, head_dim;
+  int lg_page, capacity;
+  int rows;      // tokens * group: query rows of a kv head
+  int row_tiles;
+  float scale_log2;
+  unsigned* counters;
+  float* part_o;   // [ctas][2][16*MT][HD]
+  float2* part_ml; // [ctas][2][16*MT]
+  float* lse2;     // [batch][kv_heads][rows] log2 units (accumulate only)
+  float* sbuf;     // [tiles][16*MT][64] scores in log2 units (accumulate only)
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
+  const int bytes = on ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+
+template <class T>
+struct Mma;
+template <>
+struct Mma<__half> {
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+template <>
+struct Mma<__nv_bfloat16> {
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const float2 f = __bfloat1622float2(h);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+
+// 2^(a - b) for a <= b, 0 where a is -inf (also where both are).
+__device__ __forceinline__ float exp2_diff(float a, float b) { return a == -INFINITY ? 0.f : exp2f(a - b); }
+
+// ---------------------------------------------------------------------------
+// the index space of tiles
+// ---------------------------------------------------------------------------
+// Slots that query row `row` of sequence length `len` (before the step) sees.
+__device__ __forceinline__ int visible(const AttnParams& p, int len, int row) {
+  return len < 0 ? 0 : static_cast<int>(min((int64_t)len + row / p.group + 1, (int64_t)p.capacity));
+}
+// Tiles of an item: one at least, so that every output row is written.
+template <int RT>
+__device__ __forceinline__ int item_tiles(const AttnParams& p, int len, int rt) {
+  const int vis = visible(p, len, min(p.rows, (rt + 1) * RT) - 1);
+  return max(1, (vis + kPaTile - 1) / kPaTile);
+}
+template <int RT>
+__device__ __forceinline__ int seq_tiles(const AttnParams& p, int len) {
+  int n = 0;
+  for (int rt = 0; rt < p.row_tiles; ++rt) n += item_tiles<RT>(p, len, rt);
+  return n * p.kv_heads;
+}
+
+struct Cursor {  // one tile: sequence, row tile, kv head, tile of the item
+  int b, rt, h, tile, n, len;
+};
+
+template <int RT>
+__device__ __forceinline__ void step_cursor(const AttnParams& p, Cursor& c) {
+  if (++c.tile < c.n) return;
+  c.tile = 0;
+  if (++c.h < p.kv_heads) return;
+  c.h = 0;
+  if (++c.rt == p.row_tiles) {
+    c.rt = 0;
+    if (++c.b == p.batch) return;  // past the end: the caller does not use it
+    c.len = p.lengths[c.b];
+  }
+  c.n = item_tiles<RT>(p, c.len, c.rt);
+}
+
+// Sum over the block of one value per thread (all threads call it).
+__device__ __forceinline__ int block_sum(int v, int* s_tmp) {
+#pragma unroll
+  for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s_tmp[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int t = 0;
+#pragma unroll
+  for (int w = 0; w < kPaWarps; ++w) t += s_tmp[w];
+  return t;
+}
+
+// The sequence holding position `t0` of the concatenation of `count(len)`
+// positions per sequence, and the positions before it.
+template <class F>
+__device__ __forceinline__ void find_sequence(const AttnParams& p, int t0, F count, int* s_tmp, int& b_out, int& before) {
+  int run = 0;
+  for (int base = 0;; base += kPaThreads) {
+    const int b = base + threadIdx.x;
+    const int own = b < p.batch ? count(p.lengths[b]) : 0;
+    int inc = own;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inc, m);
+      if ((threadIdx.x & 31) >= m) inc += o;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 31) s_tmp[threadIdx.x >> 5] = inc;
+    if (threadIdx.x == 0) s_tmp[4] = -1;
+    __syncthreads();
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kPaWarps; ++w) {
+      if (w < (int)(threadIdx.x >> 5)) inc += s_tmp[w];
+      sum += s_tmp[w];
+    }
+    if (own > 0 && run + inc - own <= t0 && t0 < run + inc) {
+      s_tmp[4] = b;
+      s_tmp[5] = run + inc - own;
+    }
+    __syncthreads();
+    if (s_tmp[4] >= 0 || base + kPaThreads >= p.batch) {
+      b_out = s_tmp[4];
+      before = s_tmp[5];
+      return;
+    }
+    run += sum;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// the attention kernel
+// ---------------------------------------------------------------------------
+template <int HD, int MT>
+struct PaShape {
+  static constexpr int RT = 16 * MT;                      // rows of an item
+  static constexpr int WT = kPaWarps / MT;                // warps along the tokens
+  static constexpr int CH = HD / 8;                       // 16-byte chunks per token
+  static constexpr int kTokBytes = HD * 2;
+  static constexpr int kKV = kPaTile * kTokBytes;         // bytes of a K (or V) tile
+  static constexpr int kQ = RT * kTokBytes;
+  static constexpr int kStage = 2 * kKV + kQ;
+  // three tiles per CTA, two where three with the queries pass 227 KB
+  static constexpr int kStages = HD == 256 && MT > 1 ? 2 : 3;
+  static constexpr int kSmem = kStages * kStage;
+  static_assert(kSmem <= 227 * 1024 - 1024, "shared memory");
+  static_assert(kPaWarps * 16 * HD * 4 <= kStage, "the join buffer reuses a consumed stage");
+};
+
+template <class T, int HD, int MT, bool WEIGHTS>
+__global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_constant__ AttnParams p) {
+  using S = PaShape<HD, MT>;
+  constexpr int RT = S::RT, WT = S::WT, CH = S::CH, kStages = S::kStages;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int s_tmp[8];
+  __shared__ uint32_t s_valid[kStages][kPaWarps];
+  __shared__ float s_m[kPaWarps][16], s_l[kPaWarps][16];
+  __shared__ bool s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t sbase = smem_u32(smem);
+
+  // ---- this CTA's run of tiles ----
+  int cnt = 0;
+  for (int b = tid; b < p.batch; b += kPaThreads) cnt += seq_tiles<RT>(p, p.lengths[b]);
+  const int total = block_sum(cnt, s_tmp);
+  const int per = (total + gridDim.x - 1) / gridDim.x;
+  const int t0 = min((int)blockIdx.x * per, total), t1 = min(t0 + per, total);
+  if (WEIGHTS) pdl_trigger();
+  if (t0 >= t1) return;
+  Cursor c;
+  int before;
+  find_sequence(p, t0, [&](int len) { return seq_tiles<RT>(p, len); }, s_tmp, c.b, before);
+  c.len = p.lengths[c.b];
+  int rem = t0 - before;
+  for (c.rt = 0;; ++c.rt) {
+    c.n = item_tiles<RT>(p, c.len, c.rt);
+    if (rem < p.kv_heads * c.n) break;
+    rem -= p.kv_heads * c.n;
+  }
+  c.h = rem / c.n;
+  c.tile = rem - c.h * c.n;
+  Cursor ld = c;
+
+  // ---- loads ----
+  const int page_mask = (1 << p.lg_page) - 1;
+  const T* kp = static_cast<const T*>(p.k_pages);
+  const T* vp = static_cast<const T*>(p.v_pages);
+  auto page_of = [&](const Cursor& u) {  // of this lane's token (lanes 16.. repeat 0..)
+    const int tok = u.tile * kPaTile + warp * 16 + (lane & 15);
+    return tok < p.capacity ? p.block_table[u.b * p.table_stride + (tok >> p.lg_page)] : -1;
+  };
+  int pid = page_of(ld);
+  auto issue = [&](int t, bool first) {  // tile t of the index space, at cursor ld
+    const int stage = (t - t0) % kStages;
+    const uint32_t st = sbase + stage * S::kStage;
+    const int tok = ld.tile * kPaTile + warp * 16 + (lane & 15);
+    const int hi = visible(p, ld.len, min(p.rows, (ld.rt + 1) * RT) - 1);
+    const bool ok = tok < hi && pid >= 0 && pid < p.num_pages;
+    const int64_t off = ok ? pid * p.page_stride + ld.h * p.head_stride + (tok & page_mask) * p.token_stride : 0;
+    const uint32_t valid = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+    if (lane == 0) s_valid[stage][warp] = valid;
+#pragma unroll
+    for (int i = 0; i < 16 * CH / 32; ++i) {
+      const int r = i * (32 / CH) + lane / CH, chunk = lane % CH;
+      const int64_t o = __shfl_sync(0xffffffffu, off, r) + chunk * 8;
+      const bool on = ((valid >> r) & 1u) && chunk * 8 < p.head_dim;
+      const int row = warp * 16 + r;
+      const uint32_t d = st + row * S::kTokBytes + ((chunk ^ (row & 7)) << 4);
+      cp_async16_zfill(d, on ? kp + o : kp, on);
+      cp_async16_zfill(d + S::kKV, on ? vp + o : vp, on);
+    }
+    if (ld.tile == 0 || first) {
+      const T* q = static_cast<const T*>(p.q);
+      for (int i = tid; i < RT * CH; i += kPaThreads) {
+        const int r = i / CH, chunk = i % CH, row = ld.rt * RT + r;
+        const bool on = row < p.rows && chunk * 8 < p.head_dim;
+        const int j = on ? row / p.group : 0;
+        const int64_t o = on ? (((int64_t)ld.b * p.tokens + j) * p.q_heads + ld.h * p.group + row - j * p.group) *
+                                       p.head_dim + chunk * 8
+                             : 0;
+        cp_async16_zfill(st + 2 * S::kKV + r * S::kTokBytes + ((chunk ^ (r & 7)) << 4), q + o, on);
+      }
+    }
+    step_cursor<RT>(p, ld);
+    if (t + 1 < t1) pid = page_of(ld);
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (t0 + i < t1) issue(t0 + i, i == 0);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  // ---- state of this warp's 16 rows ----
+  const int mt = warp / WT, tw = warp % WT;
+  const int r0 = lane >> 2, cq = lane & 3;  // this thread: rows r0, r0 + 8, columns 2 cq + {0, 1} of each 8
+  float o[HD / 8][4];
+  uint32_t qf[HD / 16][4];
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  int vis[2] = {0, 0}, jr[2] = {0, 0};
+  int vis_lo = 0, j_lo = 0, j_hi = 0;
+  bool fresh = true;
+
+  for (int t = t0; t < t1; ++t) {
+    const int stage = (t - t0) % kStages;
+    const uint32_t st = sbase + stage * S::kStage;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    if (MT > 1 || fresh) __syncthreads();  // tiles (MT > 1) and queries are shared by the warps
+    else __syncwarp();
+    if (t + kStages - 1 < t1) issue(t + kStages - 1, false);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+
+    if (fresh) {
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        const int r = mt * 16 + (lane & 15), chunk = ks * 2 + (lane >> 4);
+        ldsm4(qf[ks], st + 2 * S::kKV + r * S::kTokBytes + ((chunk ^ (r & 7)) << 4));
+      }
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+      const int row0 = c.rt * RT + mt * 16;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = row0 + r0 + 8 * e;
+        jr[e] = row / p.group;
+        vis[e] = row < p.rows ? visible(p, c.len, row) : 0;
+      }
+      const int last = min(row0 + 16, p.rows) - 1;
+      j_lo = row0 / p.group;
+      j_hi = last / p.group;  // < j_lo where this row tile of 16 is empty
+      vis_lo = last >= row0 ? visible(p, c.len, row0) : 0;
+      fresh = false;
+      __syncthreads();  // every warp has its queries: their buffer may be filled again
+    }
+
+    // blocks of 16 tokens: one per warp at MT = 1, MT of them otherwise
+#pragma unroll 1
+    for (int blk = tw * MT; blk < (tw + 1) * MT; ++blk) {
+      const int tok0 = c.tile * kPaTile + blk * 16;
+      const uint32_t valid = s_valid[stage][blk];
+      const uint32_t kb = st + blk * 16 * S::kTokBytes;
+      float s[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        uint32_t kf[4];
+        const int r = (lane & 7) + ((lane >> 4) << 3), chunk = ks * 2 + ((lane >> 3) & 1);
+        ldsm4(kf, kb + r * S::kTokBytes + ((chunk ^ (r & 7)) << 4));
+        Mma<T>::run(s[0], qf[ks], kf[0], kf[1]);
+        Mma<T>::run(s[1], qf[ks], kf[2], kf[3]);
+      }
+      const bool whole = valid == 0xffffu && tok0 + 16 <= vis_lo;  // every slot seen by every row
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int col = n * 8 + cq * 2 + (e & 1);
+          const bool seen = whole || (((valid >> col) & 1u) && tok0 + col < vis[e >> 1]);
+          s[n][e] = seen ? s[n][e] * p.scale_log2 : -INFINITY;
+        }
+      if (WEIGHTS) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (c.rt * RT + mt * 16 + r0 + 8 * e < p.rows)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              *reinterpret_cast<float2*>(p.sbuf + ((size_t)t * RT + mt * 16 + r0 + 8 * e) * kPaTile + blk * 16 + n * 8 +
+                                         cq * 2) = make_float2(s[n][2 * e], s[n][2 * e + 1]);
+      }
+      // running maximum: the quad of four lanes shares a row
+      float mn[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        mn[e] = fmaxf(m[e], x);
+      }
+      if (__any_sync(0xffffffffu, mn[0] != m[0] || mn[1] != m[1])) {
+        const float a0 = exp2_diff(m[0], mn[0]), a1 = exp2_diff(m[1], mn[1]);
+        m[0] = mn[0];
+        m[1] = mn[1];
+        l[0] *= a0;
+        l[1] *= a1;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+          o[n][0] *= a0;
+          o[n][1] *= a0;
+          o[n][2] *= a1;
+          o[n][3] *= a1;
+        }
+      }
+      const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        s[n][0] = exp2f(s[n][0] - b0);
+        s[n][1] = exp2f(s[n][1] - b0);
+        s[n][2] = exp2f(s[n][2] - b1);
+        s[n][3] = exp2f(s[n][3] - b1);
+        l[0] += s[n][0] + s[n][1];
+        l[1] += s[n][2] + s[n][3];
+      }
+      uint32_t ph[4], pl[4];
+      Mma<T>::split(s[0][0], s[0][1], ph[0], pl[0]);
+      Mma<T>::split(s[0][2], s[0][3], ph[1], pl[1]);
+      Mma<T>::split(s[1][0], s[1][1], ph[2], pl[2]);
+      Mma<T>::split(s[1][2], s[1][3], ph[3], pl[3]);
+      const uint32_t vb = kb + S::kKV;
+      // Rows of several step tokens differ in the last slots they see.  There
+      // each token's product takes V with the slots it does not see zeroed
+      // (0 * inf would be NaN), and only its own rows of the result.  (With one
+      // token the slots past the last it sees were zero-filled.)
+      const bool mixed = p.tokens > 1 && tok0 + 16 > vis_lo;
+#pragma unroll
+      for (int nn = 0; nn < HD / 16; ++nn) {
+        uint32_t vf[4];
+        const int r = lane & 15, chunk = nn * 2 + (lane >> 4);
+        ldsm4t(vf, vb + r * S::kTokBytes + ((chunk ^ (r & 7)) << 4));
+        if (!mixed) {
+          Mma<T>::run(o[2 * nn], ph, vf[0], vf[1]);
+          Mma<T>::run(o[2 * nn], pl, vf[0], vf[1]);
+          Mma<T>::run(o[2 * nn + 1], ph, vf[2], vf[3]);
+          Mma<T>::run(o[2 * nn + 1], pl, vf[2], vf[3]);
+        } else {
+#pragma unroll 1
+          for (int j = j_lo; j <= j_hi; ++j) {
+            const int see = visible(p, c.len, j * p.group) - tok0;  // slots of this block
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int k = cq * 2 + 8 * (e & 1);
+              const uint32_t keep = (k < see ? 0x0000ffffu : 0u) | (k + 1 < see ? 0xffff0000u : 0u);
+              w[e] = vf[e] & keep;
+            }
+            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+            Mma<T>::run(x, ph, w[0], w[1]);
+            Mma<T>::run(x, pl, w[0], w[1]);
+            Mma<T>::run(y, ph, w[2], w[3]);
+            Mma<T>::run(y, pl, w[2], w[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (jr[e >> 1] == j) {
+                o[2 * nn][e] += x[e];
+                o[2 * nn + 1][e] += y[e];
+              }
+          }
+        }
+      }
+    }
+
+    // ---- the end of this CTA's part of the item ----
+    if (c.tile + 1 == c.n || t + 1 == t1) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+        if (cq == 0) {
+          s_m[warp][r0 + 8 * e] = m[e];
+          s_l[warp][r0 + 8 * e] = l[e];
+        }
+      }
+      __syncthreads();  // every warp is done with this tile: its stage becomes the join buffer
+      float* buf = reinterpret_cast<float*>(smem + stage * S::kStage);  // [warp][16][HD], 32-byte groups swizzled
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = r0 + 8 * e;
+          *reinterpret_cast<float2*>(buf + (warp * 16 + r) * HD + ((n * 8 + cq * 2) ^ ((r & 7) << 3))) =
+              make_float2(o[n][2 * e], o[n][2 * e + 1]);
+        }
+      __syncthreads();
+      const int begin = t - c.tile, end = begin + c.n;  // the item's tiles
+      const int c0 = begin / per, c1 = (end - 1) / per; // CTAs that share it
+      const bool alone = c0 == c1;
+      const int nrow = min(RT, p.rows - c.rt * RT);
+      const int slot = blockIdx.x == c0 ? 1 : 0;  // an item that began in an earlier CTA: slot 0
+      float* po = p.part_o + (size_t)(blockIdx.x * 2 + slot) * RT * HD;
+      float2* pml = p.part_ml + (blockIdx.x * 2 + slot) * RT;
+      const int64_t out0 = ((int64_t)c.b * p.tokens) * p.q_heads + c.h * p.group;
+      auto finish = [&](int r, int d, float4 v, float M, float L) {  // row r, elements d..d+3
+        const int row = c.rt * RT + r, j = row / p.group;
+        const int64_t at = out0 + (int64_t)j * p.q_heads + row - j * p.group;
+        const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+        if (d < p.head_dim) {
+          T w[4] = {Elem<T>::from(v.x * inv), Elem<T>::from(v.y * inv), Elem<T>::from(v.z * inv),
+                    Elem<T>::from(v.w * inv)};
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * p.head_dim + d) = *reinterpret_cast<uint2*>(w);
+        }
+        if (d == 0) {
+          const float lg = L > 0.f || L != L ? M + log2f(L) : -INFINITY;
+          if (p.lse) p.lse[at] = lg * 0.6931471805599453f;
+          if (WEIGHTS) p.lse2[((int64_t)c.b * p.kv_heads + c.h) * p.rows + row] = lg;
+        }
+      };
+      for (int i = tid; i < nrow * (HD / 4); i += kPaThreads) {
+        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+        const int w0 = (r / 16) * WT, rr = r % 16;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WT; ++w) M = fmaxf(M, s_m[w0 + w][rr]);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WT; ++w) {
+          const float f = exp2_diff(s_m[w0 + w][rr], M);
+          const float4 x = *reinterpret_cast<const float4*>(buf + ((w0 + w) * 16 + rr) * HD + (d ^ ((rr & 7) << 3)));
+          L = fmaf(s_l[w0 + w][rr], f, L);
+          v.x = fmaf(x.x, f, v.x);
+          v.y = fmaf(x.y, f, v.y);
+          v.z = fmaf(x.z, f, v.z);
+          v.w = fmaf(x.w, f, v.w);
+        }
+        if (alone) {
+          finish(r, d, v, M, L);
+        } else {
+          *reinterpret_cast<float4*>(po + r * HD + d) = v;
+          if (d == 0) pml[r] = make_float2(M, L);
+        }
+      }
+      if (!alone) {
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+          const unsigned n = static_cast<unsigned>(c1 - c0 + 1);
+          s_last = atomicAdd(&p.counters[c0], 1u) == n - 1;
+          if (s_last) p.counters[c0] = 0u;
+        }
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          for (int i = tid; i < nrow * (HD / 4); i += kPaThreads) {
+            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+            float M = -INFINITY, L = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int k = c0; k <= c1; ++k) {
+              const size_t part = static_cast<size_t>(k * 2 + (k == c0 ? 1 : 0)) * RT + r;
+              const float2 ml = __ldcg(p.part_ml + part);
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + part * HD + d));
+              const float mn = fmaxf(M, ml.x);
+              const float f = exp2_diff(M, mn), g = exp2_diff(ml.x, mn);
+              M = mn;
+              L = L * f + ml.y * g;
+              v.x = v.x * f + x.x * g;
+              v.y = v.y * f + x.y * g;
+              v.z = v.z * f + x.z * g;
+              v.w = v.w * f + x.w * g;
+            }
+            finish(r, d, v, M, L);
+          }
+        }
+      }
+      __syncthreads();  // the join buffer's stage may be filled again
+      fresh = true;
+    }
+    step_cursor<RT>(p, c);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------
+// accumulated weights: scores[b][h][s] += sum over the rows of 2^(s - lse)
+// from the scores that the attention kernel left in the workspace (16 bytes a
+// slot and four rows, against head_dim * 4 for reading K again)
+// ---------------------------------------------------------------------------
+template <int RT>
+__global__ void __launch_bounds__(kPaThreads) paged_weights_kernel(const __grid_constant__ AttnParams p) {
+  __shared__ int s_tmp[8];
+  pdl_wait();
+  const int last = p.row_tiles - 1;
+  auto count = [&](int len) { return p.kv_heads * item_tiles<RT>(p, len, last); };
+  int cnt = 0;
+  for (int b = threadIdx.x; b < p.batch; b += kPaThreads) cnt += count(p.lengths[b]);
+  const int total = block_sum(cnt, s_tmp);
+  const int per = (total + gridDim.x - 1) / gridDim.x;
+  const int t0 = min((int)blockIdx.x * per, total), t1 = min(t0 + per, total);
+  if (t0 >= t1) return;
+  int b, before;
+  find_sequence(p, t0, count, s_tmp, b, before);
+  // tiles of the attention kernel's index space before sequence b
+  int c1 = 0;
+  for (int i = threadIdx.x; i < b; i += kPaThreads) c1 += seq_tiles<RT>(p, p.lengths[i]);
+  int base = block_sum(c1, s_tmp);
+  int len = p.lengths[b], n = item_tiles<RT>(p, len, last);
+  const int half = threadIdx.x >> 6, tok = threadIdx.x & 63;  // two tiles at a time
+  for (int t = t0 + half; t < t1; t += 2) {
+    while (t - before >= p.kv_heads * n) {
+      before += p.kv_heads * n;
+      base += seq_tiles<RT>(p, len);
+      len = p.lengths[++b];
+      n = item_tiles<RT>(p, len, last);
+    }
+    const int h = (t - before) / n, tile = (t - before) - h * n;
+    const int slot = tile * kPaTile + tok;
+    if (slot >= visible(p, len, p.rows - 1)) continue;
+    float w = 0.f;
+    int off = base;
+    for (int rt = 0; rt <= last; ++rt) {
+      const int nt = item_tiles<RT>(p, len, rt);
+      if (tile < nt) {
+        const float* s = p.sbuf + (size_t)(off + h * nt + tile) * RT * kPaTile + tok;
+        const float* z = p.lse2 + ((int64_t)b * p.kv_heads + h) * p.rows + rt * RT;
+        const int rows = min(RT, p.rows - rt * RT);
+#pragma unroll 4
+        for (int r = 0; r < rows; ++r) w += exp2_diff(s[r * kPaTile], z[r]);
+      }
+      off += p.kv_heads * nt;
+    }
+    p.scores[((int64_t)b * p.kv_heads + h) * p.capacity + slot] += w;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct PaPlan {
+  int hd, mt;
+  int64_t max_tiles, ml_off, o_off, lse_off, s_off, bytes;
+};
+
+// Sizes of the call's index space and workspace (no device work).
+tp_status plan_attn(const tp_paged_cache* c, int tokens, int q_heads, int accumulate, PaPlan* out) {
+  if (tokens < 1 || q_heads < 1 || c->kv_heads < 1 || q_heads % c->kv_heads)
+    return fail(TP_ERR_ARG, "tp_paged_attn: need tokens >= 1 and q_heads a multiple of kv_heads");
+  PaPlan pl{};
+  pl.hd = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
+  const int64_t rows = (int64_t)tokens * (q_heads / c->kv_heads);
+  // rows of an item: as few 16-row tiles as hold them, four at most (each item
+  // reads the keys and values once)
+  pl.mt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int64_t rt = 16 * pl.mt, row_tiles = (rows + rt - 1) / rt;
+  const int64_t cap = (int64_t)c->max_pages * c->page_size;
+  const int64_t items = (int64_t)c->batch * c->kv_heads * row_tiles;
+  pl.max_tiles = items * std::max<int64_t>(1, (cap + kPaTile - 1) / kPaTile);
+  if (rows > (1 << 24) || items > (1 << 30) || pl.max_tiles > (int64_t(1) << 30))
+    return fail(TP_ERR_UNSUPPORTED, "tp_paged_attn: too many rows, sequences or slots");
+  int64_t at = kPaCounterBytes;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  pl.ml_off = take((int64_t)kPaMaxCtas * 2 * rt * 8);
+  pl.o_off = take((int64_t)kPaMaxCtas * 2 * rt * pl.hd * 4);
+  if (accumulate) {
+    pl.lse_off = take((int64_t)c->batch * c->kv_heads * rows * 4);
+    pl.s_off = take(pl.max_tiles * rt * kPaTile * 4);
+  }
+  pl.bytes = at;
+  *out = pl;
+  return TP_OK;
+}
+
+template <class T, int HD, int MT>
+tp_status launch_attn(const AttnParams& p, const PaPlan& pl, bool weights, cudaStream_t st) {
+  using S = PaShape<HD, MT>;
+  const auto kern = weights ? paged_attn_kernel<T, HD, MT, true> : paged_attn_kernel<T, HD, MT, false>;
+  static int smem_set[2][64];
+  static int ctas[2][64];  // resident CTAs per SM
+  tp_status s = ensure_smem(kern, S::kSmem, smem_set[weights], "paged_attn: shared memory attribute");
+  if (s != TP_OK) return s;
+  int sms = 0, dev = 0;
+  s = device_sms(&sms);
+  if (s != TP_OK) return s;
+  TP_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
+  int occ = __atomic_load_n(&ctas[weights][dev], __ATOMIC_RELAXED);
+  if (!occ) {
+    TP_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kPaThreads, S::kSmem), "paged_attn: occupancy");
+    if (occ < 1) return fail(TP_ERR_CUDA, "paged_attn: the kernel does not fit this device");
+    __atomic_store_n(&ctas[weights][dev], occ, __ATOMIC_RELAXED);
+  }
+  const int grid = static_cast<int>(std::min<int64_t>(std::min(kPaMaxCtas, sms * occ), pl.max_tiles));
+  kern<<<grid, kPaThreads, S::kSmem, st>>>(p);
+  s = check_launch("paged_attn launch");
+  if (s != TP_OK || !weights) return s;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(8 * sms, pl.max_tiles)));
+  cfg.blockDim = dim3(kPaThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_weights_kernel<S::RT>, p), "paged_weights launch");
+  return clear_ok();
+}
+
+template <class T, int HD>
+tp_status dispatch_rows(const AttnParams& p, const PaPlan& pl, bool weights, cudaStream_t st) {
+  if (pl.mt == 1) return launch_attn<T, HD, 1>(p, pl, weights, st);
+  if (pl.mt == 2) return launch_attn<T, HD, 2>(p, pl, weights, st);
+  return launch_attn<T, HD, 4>(p, pl, weights, st);
+}
+
+template <class T>
+tp_status dispatch_dim(const AttnParams& p, const PaPlan& pl, bool weights, cudaStream_t st) {
+  if (pl.hd == 64) return dispatch_rows<T, 64>(p, pl, weights, st);
+  if (pl.hd == 128) return dispatch_rows<T, 128>(p, pl, weights, st);
+  return dispatch_rows<T, 256>(p, pl, weights, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+TP_API int64_t tp_paged_attn_workspace_bytes(const tp_paged_cache* cache, int tokens, int q_heads, int accumulate) {
+  PaPlan pl;
+  tp_status s = check_cache(cache, "tp_paged_attn_workspace_bytes");
+  if (s == TP_OK) s = plan_attn(cache, tokens, q_heads, accumulate, &pl);
+  return s == TP_OK ? pl.bytes : -static_cast<int64_t>(s);
+}
+
+TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_cache* cache, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+  if (!args || !args->q || !args->out) return fail(TP_ERR_ARG, "tp_paged_attn: null pointer");
+  const tp_paged_attn_args& a = *args;
+  tp_status s = check_cache(cache, "tp_paged_attn");
+  if (s != TP_OK) return s;
+  PaPlan pl;
+  s = plan_attn(cache, a.tokens, a.q_heads, a.accumulate, &pl);
+  if (s != TP_OK) return s;
+  if (a.accumulate && !cache->scores) return fail(TP_ERR_ARG, "tp_paged_attn: the cache has no scores to accumulate in");
+  if (!aligned(a.q, 16) || !aligned(a.out, 16))
+    return fail(TP_ERR_ALIGN, "tp_paged_attn: q and out must be 16-byte aligned");
+  if (!workspace || workspace_bytes < pl.bytes || !aligned(workspace, 256))
+    return fail(TP_ERR_WORKSPACE, "tp_paged_attn: workspace missing, not 256-byte aligned or smaller than %lld bytes",
+                (long long)pl.bytes);
+  AttnParams p{};
+  p.q = a.q;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.k_pages = cache->k_pages;
+  p.v_pages = cache->v_pages;
+  p.block_table = cache->block_table;
+  p.lengths = cache->lengths;
+  p.scores = cache->scores;
+  p.num_pages = cache->num_pages;
+  p.page_stride = cache->page_stride;
+  p.head_stride = cache->head_stride;
+  p.token_stride = cache->token_stride;
+  p.table_stride = cache->table_stride;
+  p.batch = cache->batch;
+  p.tokens = a.tokens;
+  p.q_heads = a.q_heads;
+  p.kv_heads = cache->kv_heads;
+  p.group = a.q_heads / cache->kv_heads;
+  p.head_dim = cache->head_dim;
+  p.lg_page = log2_int(cache->page_size);
+  p.capacity = cache->max_pages * cache->page_size;
+  p.rows = a.tokens * p.group;
+  p.row_tiles = (p.rows + 16 * pl.mt - 1) / (16 * pl.mt);
+  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  auto* ws = static_cast<unsigned char*>(workspace);
+  p.counters = reinterpret_cast<unsigned*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_off);
+  p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
+  p.lse2 = reinterpret_cast<float*>(ws + pl.lse_off);
+  p.sbuf = reinterpret_cast<float*>(ws + pl.s_off);
+  cudaStream_t st = as_stream(stream);
+  const bool weights = a.accumulate != 0;
+  return cache->dtype == TP_F16 ? dispatch_dim<__half>(p, pl, weights, st)
+                                : dispatch_dim<__nv_bfloat16>(p, pl, weights, st);
+}
+
+}  // extern "C"

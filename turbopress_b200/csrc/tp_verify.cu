@@ -1,0 +1,405 @@
+// Verification of drafted tokens against the target's logits.
+//
+// Mathematics: with p = softmax(x / t) and u uniform, accepting a draft d ~ q
+// while u q(d) < p(d) and drawing a replacement from max(p - q, 0) at the first
+// rejection leaves the tokens distributed as the target's own.  The draw is an
+// exponential race: with independent exponentials e, argmax r_i / e_i is i with
+// probability r_i / sum r, needs no normaliser and no prefix sums, and a
+// maximum does not depend on the order it is taken in.
+//
+// Bound: memory.  One pass over the logits (running maximum m and sum of
+// 2^((x - m) c), or the argmax for a greedy sequence), one pass over the one
+// row that decides (in L2 for small batches), its draft row and its noise.
+//
+// Split: rows are cut into slices of equal length over the GPU; the last CTA
+// of a sequence joins its rows' slices, walks the drafts and leaves the row to
+// draw from; a second launch races over it, its last CTA writing the token.
+// Counters and keys in the workspace return to zero.
+#include <algorithm>
+
+#include "tp_decode.cuh"
+#include "tp_paged.cuh"
+
+using namespace tp;
+
+namespace {
+
+constexpr int kVfThreads = 256;
+constexpr int kVfWarps = kVfThreads / 32;
+constexpr int kVfMaxRows = 64;    // drafts + 1
+constexpr int kVfMaxSplits = 128;
+
+struct Part {  // one slice of a row
+  float m, l;               // sampled: maximum and sum of 2^((x - m) c)
+  unsigned long long key;   // greedy: argmax key
+};
+
+struct Choice {  // what a sequence draws from
+  float m, c, inv_l;  // p_i = 2^((x_i - m) c) * inv_l
+  int row;            // of its logits; -1: nothing to draw
+  int residual;       // 1: from max(p - q, 0)
+};
+
+struct VerifyParams {
+  tp_verify_args a;
+  int splits, race_splits;
+  Part* part;                 // [batch][rows][splits]
+  Choice* choice;             // [batch]
+  unsigned long long* key;    // [batch][2]: race over the residual, over p
+  unsigned* done;             // [batch][2]: CTAs that have arrived
+};
+
+__device__ __forceinline__ unsigned long long argmax_key(float v, unsigned idx) {
+  unsigned u;
+  if (v != v) {
+    u = 0xFFFFFFFFu;
+  } else {
+    if (v == 0.f) v = 0.f;
+    u = __float_as_uint(v);
+    u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  }
+  return (static_cast<unsigned long long>(u) << 32) | (0xFFFFFFFFu - idx);
+}
+__device__ __forceinline__ unsigned key_index(unsigned long long k) { return 0xFFFFFFFFu - static_cast<unsigned>(k); }
+
+__device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
+#pragma unroll
+  for (int m = 16; m; m >>= 1) {
+    const unsigned long long o = __shfl_xor_sync(0xffffffffu, k, m);
+    k = o > k ? o : k;
+  }
+  return k;
+}
+
+// f(i, x_i) for the elements [lo, hi) of a row that fall to this thread, in
+// ascending order: 16-byte vectors of the aligned middle, single elements at
+// ragged ends.
+template <class T, class F, class G>
+__device__ __forceinline__ void for_slice(const T* row, int lo, int hi, F each, G vec) {
+  constexpr int V = 16 / sizeof(T);
+  const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
+  const int head = min(hi, lo + (mis ? V - mis : 0));
+  if (lo + (int)threadIdx.x < head) each(lo + threadIdx.x, Elem<T>::to(row[lo + threadIdx.x]));
+  const int nvec = (hi - head) / V;
+  const uint4* mid = reinterpret_cast<const uint4*>(row + head);
+  int i = threadIdx.x;
+  for (; i + 3 * kVfThreads < nvec; i += 4 * kVfThreads) {
+    uint4 w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w[u] = __ldg(mid + i + u * kVfThreads);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float x[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = Elem<T>::to(reinterpret_cast<const T*>(&w[u])[e]);
+      vec(head + (i + u * kVfThreads) * V, x);
+    }
+  }
+  for (; i < nvec; i += kVfThreads) {
+    const uint4 w = __ldg(mid + i);
+    float x[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = Elem<T>::to(reinterpret_cast<const T*>(&w)[e]);
+    vec(head + i * V, x);
+  }
+  const int tail = head + nvec * V + threadIdx.x;
+  if (tail < hi) each(tail, Elem<T>::to(row[tail]));
+}
+
+// Joins two (m, l) with 2^((x - m) c) terms.
+__device__ __forceinline__ void join(float& m, float& l, float m2, float l2, float c) {
+  const float top = fmaxf(m, m2);
+  const float f = m == top ? 1.f : exp2f((m - top) * c), g = m2 == top ? 1.f : exp2f((m2 - top) * c);
+  l = (l == 0.f ? 0.f : l * f) + (l2 == 0.f ? 0.f : l2 * g);
+  m = top;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const __grid_constant__ VerifyParams p) {
+  __shared__ float s_m[kVfWarps], s_l[kVfWarps];
+  __shared__ unsigned long long s_k[kVfWarps];
+  __shared__ bool s_last;
+  __shared__ bool s_ok[kVfMaxRows];
+  __shared__ float s_rm[kVfMaxRows], s_rl[kVfMaxRows];
+  __shared__ unsigned s_arg[kVfMaxRows];
+  pdl_trigger();
+  const int rows = p.a.drafts + 1;
+  const int b = blockIdx.y / rows, k = blockIdx.y - b * rows;
+  const int used = p.a.counts ? max(0, min(p.a.counts[b], p.a.drafts)) : p.a.drafts;
+  if (k > used) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float heat = p.a.temperature ? p.a.temperature[b] : 0.f;
+  const bool greedy = !(heat > 0.f);
+  const float c = greedy ? 0.f : 1.4426950408889634f / heat;
+  const T* row = static_cast<const T*>(p.a.logits) + (int64_t)b * p.a.batch_stride + (int64_t)k * p.a.row_stride;
+  const int per = (p.a.vocab + p.splits - 1) / p.splits;
+  const int lo = min((int)blockIdx.x * per, p.a.vocab), hi = min(lo + per, p.a.vocab);
+
+  float m = -INFINITY, l = 0.f;
+  unsigned long long best = 0ull;
+  if (greedy) {
+    float top = -INFINITY;
+    int at = -1;
+    auto one = [&](int i, float x) {
+      if (at < 0 || (!(x <= top) && top == top)) {  // a larger value, or the first NaN
+        top = x;
+        at = i;
+      }
+    };
+    constexpr int V = 16 / sizeof(T);
+    for_slice<T>(row, lo, hi, one, [&](int i, const float (&x)[V]) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) one(i + e, x[e]);
+    });
+    if (at >= 0) best = argmax_key(top, at);
+  } else {
+    auto one = [&](int, float x) {
+      if (x == -INFINITY) return;
+      if (x > m) {
+        l *= m == -INFINITY ? 0.f : exp2f((m - x) * c);
+        m = x;
+      }
+      l += exp2f((x - m) * c);
+    };
+    constexpr int V = 16 / sizeof(T);
+    for_slice<T>(row, lo, hi, one, [&](int, const float (&x)[V]) {
+      float t = x[0];
+#pragma unroll
+      for (int e = 1; e < V; ++e) t = fmaxf(t, x[e]);
+      if (t > m) {
+        l *= m == -INFINITY ? 0.f : exp2f((m - t) * c);
+        m = t;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int e = 0; e < V; ++e) l += exp2f((x[e] - base) * c);
+    });
+  }
+  if (greedy) {
+    best = warp_max(best);
+    if (lane == 0) s_k[warp] = best;
+  } else {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+      join(m, l, m2, l2, c);
+    }
+    if (lane == 0) {
+      s_m[warp] = m;
+      s_l[warp] = l;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    Part out{-INFINITY, 0.f, 0ull};
+    for (int w = 0; w < kVfWarps; ++w) {
+      if (greedy) out.key = s_k[w] > out.key ? s_k[w] : out.key;
+      else join(out.m, out.l, s_m[w], s_l[w], c);
+    }
+    p.part[((int64_t)b * rows + k) * p.splits + blockIdx.x] = out;
+    __threadfence();
+    s_last = atomicAdd(&p.done[2 * b], 1u) == static_cast<unsigned>((used + 1) * p.splits - 1);
+    if (s_last) p.done[2 * b] = 0u;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+
+  // ---- the sequence's rows, a warp each: statistics, and whether the draft stands ----
+  const int64_t* drafts = p.a.draft_tokens + (int64_t)b * p.a.drafts;
+  for (int r = warp; r <= used; r += kVfWarps) {
+    const Part* q = p.part + ((int64_t)b * rows + r) * p.splits;
+    float rm = -INFINITY, rl = 0.f;
+    unsigned long long rk = 0ull;
+    for (int i = lane; i < p.splits; i += 32) {
+      const float qm = __ldcg(&q[i].m), ql = __ldcg(&q[i].l);
+      const unsigned long long qk = __ldcg(&q[i].key);
+      rk = qk > rk ? qk : rk;
+      if (!greedy) join(rm, rl, qm, ql, c);
+    }
+    rk = warp_max(rk);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, rm, o), l2 = __shfl_xor_sync(0xffffffffu, rl, o);
+      join(rm, rl, m2, l2, c);
+    }
+    if (lane == 0) {
+      s_rm[r] = rm;
+      s_rl[r] = rl;
+      s_arg[r] = key_index(rk);
+      if (r < used) {
+        const int64_t d = drafts[r];
+        bool ok = d >= 0 && d < p.a.vocab;
+        if (ok && greedy) ok = d == (int64_t)key_index(rk);
+        if (ok && !greedy) {
+          const T* x = static_cast<const T*>(p.a.logits) + (int64_t)b * p.a.batch_stride + (int64_t)r * p.a.row_stride;
+          const float pd = exp2f((Elem<T>::to(x[d]) - rm) * c) / rl;
+          const float qd = p.a.draft_probs ? p.a.draft_probs[((int64_t)b * p.a.drafts + r) * p.a.vocab + d] : 1.f;
+          ok = p.a.uniforms[(int64_t)b * p.a.drafts + r] * qd < pd;
+        }
+        s_ok[r] = ok;
+      }
+    }
+  }
+  __syncthreads();
+  int n = 0;
+  while (n < used && s_ok[n]) ++n;
+  if (tid < rows) {
+    const int64_t at = (int64_t)b * rows + tid;
+    if (tid < n) p.a.tokens[at] = drafts[tid];
+    else p.a.tokens[at] = tid == n && greedy ? (int64_t)s_arg[n] : -1;
+  }
+  if (tid == 0) {
+    p.a.accepted[b] = n;
+    p.choice[b] = Choice{s_rm[n], c, 1.f / s_rl[n], greedy ? -1 : n, n < used};
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kVfThreads) verify_race_kernel(const __grid_constant__ VerifyParams p) {
+  __shared__ unsigned long long s_k[2][kVfWarps];
+  __shared__ bool s_last;
+  pdl_wait();
+  const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Choice ch = p.choice[b];
+  if (ch.row < 0) return;
+  const T* row = static_cast<const T*>(p.a.logits) + (int64_t)b * p.a.batch_stride + (int64_t)ch.row * p.a.row_stride;
+  const float* noise = p.a.noise + (int64_t)b * p.a.vocab;
+  const float* q = ch.residual && p.a.draft_probs
+                       ? p.a.draft_probs + ((int64_t)b * p.a.drafts + ch.row) * p.a.vocab
+                       : nullptr;
+  const int64_t hot = ch.residual && !q ? p.a.draft_tokens[(int64_t)b * p.a.drafts + ch.row] : -1;
+  const int per = (p.a.vocab + p.race_splits - 1) / p.race_splits;
+  const int lo = min((int)blockIdx.x * per, p.a.vocab), hi = min(lo + per, p.a.vocab);
+  float bt[2] = {0.f, 0.f};  // largest r / e and p / e, and where
+  int at[2] = {-1, -1};
+  auto one = [&](int i, float x) {
+    const float pi = exp2f((x - ch.m) * ch.c) * ch.inv_l, e = noise[i];
+    const float qi = q ? q[i] : i == hot ? 1.f : 0.f;
+    const float r = fmaxf(pi - qi, 0.f) / e, f = pi / e;
+    if (r > bt[0]) {
+      bt[0] = r;
+      at[0] = i;
+    }
+    if (f > bt[1]) {
+      bt[1] = f;
+      at[1] = i;
+    }
+  };
+  constexpr int V = 16 / sizeof(T);
+  for_slice<T>(row, lo, hi, one, [&](int i, const float (&x)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) one(i + e, x[e]);
+  });
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const unsigned long long k = warp_max(at[w] >= 0 ? argmax_key(bt[w], at[w]) : 0ull);
+    if (lane == 0) s_k[w][warp] = k;
+  }
+  __syncthreads();
+  if (tid < 2) {
+    unsigned long long k = 0ull;
+    for (int w = 0; w < kVfWarps; ++w) k = s_k[tid][w] > k ? s_k[tid][w] : k;
+    if (k) atomicMax(&p.key[2 * b + tid], k);
+    __threadfence();
+  }
+  __syncthreads();
+  if (tid == 0) {
+    s_last = atomicAdd(&p.done[2 * b + 1], 1u) == gridDim.x - 1;
+    if (s_last) {
+      __threadfence();
+      const unsigned long long r = atomicExch(&p.key[2 * b], 0ull), f = atomicExch(&p.key[2 * b + 1], 0ull);
+      const unsigned long long k = r ? r : f;
+      p.a.tokens[(int64_t)b * (p.a.drafts + 1) + ch.row] = k ? (int64_t)key_index(k) : -1;
+      p.done[2 * b + 1] = 0u;
+    }
+  }
+}
+
+int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+
+struct VfPlan {
+  int64_t choice_off, part_off, bytes;
+};
+
+tp_status plan_verify(int64_t batch, int64_t drafts, int64_t vocab, VfPlan* pl) {
+  if (batch < 1 || drafts < 0 || vocab < 1) return fail(TP_ERR_ARG, "tp_verify_drafts: bad sizes");
+  if (drafts + 1 > kVfMaxRows) return fail(TP_ERR_UNSUPPORTED, "tp_verify_drafts: more than %d drafts", kVfMaxRows - 1);
+  if (batch * (drafts + 1) > 65535) return fail(TP_ERR_UNSUPPORTED, "tp_verify_drafts: more than 65535 rows");
+  if (vocab > 0x7FFFFFF0) return fail(TP_ERR_UNSUPPORTED, "tp_verify_drafts: vocabulary too large");
+  // counters and keys of up to 65535 sequences at a fixed place, so that calls
+  // of other sizes find them zero
+  pl->choice_off = round256(65536 * (2 * 4 + 2 * 8));
+  pl->part_off = pl->choice_off + round256(batch * (int64_t)sizeof(Choice));
+  pl->bytes = pl->part_off + round256(batch * (drafts + 1) * kVfMaxSplits * (int64_t)sizeof(Part));
+  return TP_OK;
+}
+
+template <class T>
+tp_status launch_verify(VerifyParams& p, cudaStream_t st) {
+  int sms = 0;
+  tp_status s = device_sms(&sms);
+  if (s != TP_OK) return s;
+  const int rows = p.a.batch * (p.a.drafts + 1);
+  // slices: about eight CTAs per SM in all, at least 1024 elements each
+  auto slices = [&](int n) {
+    const int64_t most = (p.a.vocab + 1023) / 1024;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(8 * sms + n - 1) / n, most, kVfMaxSplits})));
+  };
+  p.splits = slices(rows);
+  p.race_splits = slices(p.a.batch);
+  verify_rows_kernel<T><<<dim3(p.splits, rows), kVfThreads, 0, st>>>(p);
+  s = check_launch("verify_rows launch");
+  if (s != TP_OK || !p.a.temperature) return s;  // all greedy: the tokens are written
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.race_splits, p.a.batch);
+  cfg.blockDim = dim3(kVfThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, verify_race_kernel<T>, p), "verify_race launch");
+  return clear_ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+TP_API int64_t tp_verify_workspace_bytes(int batch, int drafts, int vocab) {
+  VfPlan pl;
+  const tp_status s = plan_verify(batch, drafts, vocab, &pl);
+  return s == TP_OK ? pl.bytes : -static_cast<int64_t>(s);
+}
+
+TP_API tp_status tp_verify_drafts(const tp_verify_args* args, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (!args) return fail(TP_ERR_ARG, "tp_verify_drafts: null arguments");
+  const tp_verify_args& a = *args;
+  VfPlan pl;
+  const tp_status s = plan_verify(a.batch, a.drafts, a.vocab, &pl);
+  if (s != TP_OK) return s;
+  if (!a.logits || !a.accepted || !a.tokens || (a.drafts && !a.draft_tokens) ||
+      (a.temperature && (!a.noise || (a.drafts && !a.uniforms))))
+    return fail(TP_ERR_ARG, "tp_verify_drafts: null pointer");
+  if (!valid_dtype(a.dtype)) return fail(TP_ERR_ARG, "tp_verify_drafts: bad dtype %d", a.dtype);
+  if (!aligned(a.logits, a.dtype == TP_F32 ? 4 : 2))
+    return fail(TP_ERR_ALIGN, "tp_verify_drafts: logits are not aligned to their elements");
+  if (!workspace || workspace_bytes < pl.bytes || !aligned(workspace, 256))
+    return fail(TP_ERR_WORKSPACE, "tp_verify_drafts: workspace missing, not 256-byte aligned or smaller than %lld bytes",
+                (long long)pl.bytes);
+  VerifyParams p{};
+  p.a = a;
+  auto* ws = static_cast<unsigned char*>(workspace);
+  p.key = reinterpret_cast<unsigned long long*>(ws);
+  p.done = reinterpret_cast<unsigned*>(ws + 65536 * 16);
+  p.choice = reinterpret_cast<Choice*>(ws + pl.choice_off);
+  p.part = reinterpret_cast<Part*>(ws + pl.part_off);
+  cudaStream_t st = as_stream(stream);
+  if (a.dtype == TP_F16) return launch_verify<__half>(p, st);
+  if (a.dtype == TP_BF16) return launch_verify<__nv_bfloat16>(p, st);
+  return launch_verify<float>(p, st);
+}
+
+}  // extern "C"

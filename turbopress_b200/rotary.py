@@ -1,0 +1,174 @@
+"""Rotary positions: ``tp_rotary`` behind a small class.
+
+The decode step's rotary embedding is the plain one (half layout, the whole
+head, unscaled frequencies).  ``Rotary`` covers the layouts and scalings that
+other checkpoints and long contexts need -- half or interleaved pairs, part of
+the head, linear / llama3 / yarn scaled frequencies -- for any number of
+tokens, with the per-head RMS norm that Qwen3 applies before it.
+
+    rotary = Rotary.from_config(model.config)            # a Hugging Face config
+    q, k = rotary(q, k, positions)                        # [..., heads, head_dim], int64 [...]
+    q = cache.append(rotary, q, k, v)                     # the same, k and v into a PagedKVCache
+
+Angles are exact modulo one turn for every position (a 64-bit phase, not a
+32-bit product); arithmetic is fp32 with one rounding to the tensors' dtype.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from fractions import Fraction
+
+import torch
+from torch import Tensor
+
+from . import _abi
+
+# 2^64 / (2 pi), from 60 digits of pi
+_TURNS = 2 ** 63 / Fraction("3.14159265358979323846264338327950288419716939937510582097494")
+SCALINGS = ("default", "linear", "llama3", "yarn")
+
+
+class _RotaryArgs(ctypes.Structure):
+    """Mirror of ``tp_rotary_args``."""
+
+    _fields_ = [(nm, ctypes.c_void_p) for nm in ("q", "k", "v", "q_out", "k_out", "positions", "base", "freq", "q_norm",
+                                                 "k_norm")] + [
+        (nm, ctypes.c_int64) for nm in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                                        "v_token_stride", "v_head_stride", "tokens")] + [
+        (nm, ctypes.c_int32) for nm in ("seq", "q_heads", "kv_heads", "head_dim", "rot_dim", "dtype", "interleaved",
+                                        "inverse")] + [("scale", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: dict | None = None) -> tuple[Tensor, float]:
+    """(inverse frequencies fp32 [rot_dim/2], factor on cos and sin).
+
+    ``scaling`` holds a Hugging Face config's rope parameters: ``rope_type``
+    one of ``SCALINGS``, ``factor`` and what the type needs beside it
+    (``original_max_position_embeddings``; ``low_freq_factor`` /
+    ``high_freq_factor`` for llama3; ``beta_fast`` / ``beta_slow`` /
+    ``attention_factor`` for yarn)."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be a positive even number, got {rot_dim}")
+    inv = 1.0 / (theta ** (torch.arange(0, rot_dim, 2, dtype=torch.int64).to(dtype=torch.float) / rot_dim))
+    p = scaling or {}
+    kind = p.get("rope_type", p.get("type", "default"))
+    if kind not in SCALINGS:
+        raise ValueError(f"unsupported rope type {kind!r} (one of {SCALINGS})")
+    if kind == "default":
+        return inv, 1.0
+    factor = float(p["factor"])
+    if kind == "linear":  # every position divided by the factor
+        return inv / factor, 1.0
+    # llama3 and yarn: waves that turn often within the original context stay
+    # as they are, those that do not complete a few turns are stretched by the
+    # factor, and a linear ramp joins the two
+    original = float(p["original_max_position_embeddings"])
+    if kind == "llama3":
+        low, high = float(p["low_freq_factor"]), float(p["high_freq_factor"])
+        turns = original * inv / (2 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        return inv * keep + inv / factor * (1 - keep), 1.0
+
+    # yarn: the ramp is over the pair's index, between the pairs that make
+    # beta_fast and beta_slow turns in the original context
+    def pair_of(turns: float) -> float:
+        return rot_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+    first, last = pair_of(float(p.get("beta_fast") or 32)), pair_of(float(p.get("beta_slow") or 1))
+    if p.get("truncate", True):
+        first, last = math.floor(first), math.ceil(last)
+    first, last = max(first, 0), min(last, rot_dim - 1)
+    ramp = ((torch.arange(rot_dim // 2, dtype=torch.float) - first) / max(last - first, 0.001)).clamp(0, 1)
+
+    def temperature(scale: float, m: float = 1.0) -> float:
+        return 0.1 * m * math.log(scale) + 1.0 if scale > 1 else 1.0
+
+    attention = p.get("attention_factor")
+    if attention is None:
+        m, m_all = p.get("mscale"), p.get("mscale_all_dim")
+        attention = temperature(factor, m) / temperature(factor, m_all) if m and m_all else temperature(factor)
+    return inv * (1 - ramp) + inv / factor * ramp, float(attention)
+
+
+class Rotary:
+    """Rotary positions of one model: its frequencies, laid out once."""
+
+    def __init__(self, head_dim: int, inv_freq: Tensor | None = None, *, theta: float = 10000.0,
+                 scaling: dict | None = None, rot_dim: int | None = None, interleaved: bool = False,
+                 scale: float | None = None, device="cuda") -> None:
+        if inv_freq is None:
+            inv_freq, factor = rope_frequencies(head_dim if rot_dim is None else rot_dim, theta, scaling)
+            scale = factor if scale is None else scale
+        if inv_freq.dim() != 1 or (rot_dim is not None and 2 * inv_freq.numel() != rot_dim):
+            raise ValueError("inv_freq must be 1-D with rot_dim / 2 entries")
+        self.head_dim, self.rot_dim = int(head_dim), 2 * inv_freq.numel()
+        if not 2 <= self.rot_dim <= self.head_dim <= 256 or self.head_dim % 2:
+            raise ValueError(f"need an even head_dim <= 256 and rot_dim <= head_dim, got {head_dim} and {self.rot_dim}")
+        self.interleaved, self.scale = bool(interleaved), 1.0 if scale is None else float(scale)
+        self.inv_freq = inv_freq.detach().to(device="cpu", dtype=torch.float32)
+        if not torch.isfinite(self.inv_freq).all():
+            raise ValueError("inv_freq must be finite")
+        # turns per position as 64-bit fractions of a turn; whole turns drop out
+        words = [round(Fraction(f) * _TURNS) % 2 ** 64 for f in self.inv_freq.tolist()]
+        self.freq = torch.tensor([w - 2 ** 64 if w >= 2 ** 63 else w for w in words], dtype=torch.int64).to(device)
+        self.device = self.freq.device
+
+    @classmethod
+    def from_config(cls, config, device="cuda", interleaved: bool = False) -> "Rotary":
+        """From a Hugging Face decoder config (its theta, scaling and partial factor)."""
+        head_dim = getattr(config, "head_dim", None) or config.hidden_size // config.num_attention_heads
+        p = getattr(config, "rope_parameters", None) or getattr(config, "rope_scaling", None) or {}
+        theta = float(p.get("rope_theta") or getattr(config, "rope_theta", None) or 10000.0)
+        part = float(p.get("partial_rotary_factor") or getattr(config, "partial_rotary_factor", None) or 1.0)
+        if p and "original_max_position_embeddings" not in p and getattr(config, "max_position_embeddings", None):
+            p = {**p, "original_max_position_embeddings": config.max_position_embeddings}
+        return cls(head_dim, theta=theta, scaling=p, rot_dim=int(head_dim * part), interleaved=interleaved, device=device)
+
+    # -- arguments shared with PagedKVCache.append ------------------------------
+    def _args(self, q: Tensor, k: Tensor, positions: Tensor | None, q_norm: Tensor | None, k_norm: Tensor | None,
+              eps: float, inverse: bool) -> tuple[_RotaryArgs, Tensor, list[Tensor]]:
+        """The call's arguments without k's destination, the queries' output and
+        the tensors to keep until the launch."""
+        hd = self.head_dim
+        if q.dim() < 2 or k.dim() != q.dim() or q.shape[-1] != hd or k.shape[-1] != hd or q.shape[:-2] != k.shape[:-2]:
+            raise ValueError(f"q and k must be [..., heads, {hd}] over the same tokens, got {tuple(q.shape)} and {tuple(k.shape)}")
+        if k.dtype != q.dtype or q.device != self.device or k.device != self.device:
+            raise ValueError("q and k must share one dtype and be on the frequencies' CUDA device")
+        q3, k3 = q.reshape(-1, q.shape[-2], hd), k.reshape(-1, k.shape[-2], hd)
+        if q3.stride(2) != 1:
+            q3 = q3.contiguous()
+        if k3.stride(2) != 1:
+            k3 = k3.contiguous()
+        keep = [q3, k3]
+        if positions is not None:
+            if positions.shape != q.shape[:-2] or positions.device != self.device:
+                raise ValueError(f"positions must be {tuple(q.shape[:-2])} on {self.device}, got {tuple(positions.shape)}")
+            positions = positions.to(torch.int64).contiguous()
+            keep.append(positions)
+        for w in (q_norm, k_norm):
+            if w is not None and (w.shape != (hd,) or w.dtype != q.dtype or w.device != self.device or not w.is_contiguous()):
+                raise ValueError(f"norm weights must be contiguous [{hd}] tensors of the queries' dtype and device")
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        a = _RotaryArgs(q3.data_ptr(), k3.data_ptr(), None, out.data_ptr(), None, _abi.ptr(positions), None,
+                        self.freq.data_ptr(), _abi.ptr(q_norm), _abi.ptr(k_norm), q3.stride(0), q3.stride(1), k3.stride(0),
+                        k3.stride(1), 0, 0, q3.shape[0], 1, q3.shape[1], k3.shape[1], hd, self.rot_dim,
+                        _abi.dtype_code(q.dtype), self.interleaved, inverse, self.scale, eps)
+        return a, out, keep
+
+    def __call__(self, q: Tensor, k: Tensor, positions: Tensor, *, q_norm: Tensor | None = None,
+                 k_norm: Tensor | None = None, eps: float = 1e-6, inverse: bool = False) -> tuple[Tensor, Tensor]:
+        """q [..., q_heads, head_dim] and k [..., kv_heads, head_dim] at integer
+        ``positions`` [...] -> the rotated pair (new contiguous tensors), on the
+        current stream.  ``q_norm`` / ``k_norm`` [head_dim]: RMS norm of each
+        head before it.  ``inverse`` turns back, which is also the gradient of
+        the rotation."""
+        if positions is None:
+            raise ValueError("positions are needed")
+        a, q_out, keep = self._args(q, k, positions, q_norm, k_norm, eps, inverse)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        a.k_out = k_out.data_ptr()
+        with torch.cuda.device(self.device):
+            _abi.check(_abi.lib().tp_rotary(ctypes.addressof(a), None, _abi.stream_of(q)), "rotary")
+        return q_out, k_out
