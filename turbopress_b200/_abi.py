@@ -144,3 +144,27 @@ def require_cuda(*tensors: torch.Tensor | None) -> torch.device:
     if dev is None:
         raise ValueError("no tensor given")
     return dev
+
+
+# -- short host paths ----------------------------------------------------------
+# A decode-step call takes a few microseconds on the GPU, so its wrapper looks
+# its argument checks up by what they depend on (shapes, strides, dtypes and
+# devices, never addresses) instead of repeating them.
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def meta(t: torch.Tensor | None) -> tuple | None:
+    """What the checks of a tensor argument depend on."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def launch(fn, what: str, index: int, *args) -> None:
+    """``fn(*args, stream)`` on device ``index`` and its current stream."""
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return launch(fn, what, index, *args)
+    st = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+    status = fn(*args, st)
+    if status != TP_OK:
+        check(status, what)

@@ -117,23 +117,10 @@ class PagedKVCache:
             None if scores is None else scores[i].data_ptr(), None if positions is None else positions[i].data_ptr(),
             self.num_pages, k_pages.stride(1), k_pages.stride(2), k_pages.stride(3), block_table.stride(0), self.batch,
             self.kv_heads, self.head_dim, self.page_size, self.max_pages, _abi.dtype_code(self.dtype)) for i in range(L)]
-
         self._ws: Tensor | None = None
-        self._ws_bytes: dict[tuple[int, int, bool], int] = {}
         self._evict_ws: Tensor | None = None
-
-    def _workspace(self, tokens: int, q_heads: int, accumulate: bool) -> Tensor:
-        """The attention workspace, grown (and zero-filled) to the call's sizes."""
-        key = (tokens, q_heads, accumulate)
-        need = self._ws_bytes.get(key)
-        if need is None:
-            need = _abi.lib().tp_paged_attn_workspace_bytes(ctypes.addressof(self._structs[0]), tokens, q_heads, accumulate)
-            if need < 0:
-                _abi.check(-need, "attend")
-            self._ws_bytes[key] = need
-        if self._ws is None or self._ws.numel() < need:
-            self._ws = torch.zeros(need, dtype=torch.uint8, device=self.device)
-        return self._ws
+        self._outgrown: list[Tensor] = []  # workspaces that a captured graph may still use
+        self._plans: dict[tuple, _AttnArgs] = {}
 
     def _layer(self, layer: int) -> int:
         """Address of the layer's ``tp_paged_cache``."""
@@ -151,23 +138,27 @@ class PagedKVCache:
         tokens], by default ``next_pos`` onwards.  ``lengths`` stays: call
         ``advance`` once all layers have the step's tokens.  Tokens of idle
         sequences, past the capacity or without a page are not stored."""
-        if q.dim() != 4 or q.shape[0] != self.batch or k.shape[-2] != self.kv_heads or v.shape != k.shape:
-            raise ValueError(f"expected q [{self.batch}, tokens, heads, {self.head_dim}] and k, v with {self.kv_heads} heads")
-        if q.dtype != self.dtype or v.dtype != self.dtype or v.device != self.device or rotary.device != self.device:
-            raise ValueError("q, k, v and the pages must share one dtype and device")
-        a, out, keep = rotary._args(q, k, positions, q_norm, k_norm, eps, inverse)
-        v3 = v.reshape(-1, self.kv_heads, self.head_dim)
-        if v3.stride(2) != 1:
-            v3 = v3.contiguous()
-        a.v, a.v_token_stride, a.v_head_stride = v3.data_ptr(), v3.stride(0), v3.stride(1)
-        a.seq = max(1, q.shape[1])
+        if q.dim() != 4 or q.shape[0] != self.batch or k.shape[-2] != self.kv_heads or q.dtype != self.dtype:
+            raise ValueError(f"expected q [{self.batch}, tokens, heads, {self.head_dim}] and k, v with {self.kv_heads} heads, "
+                             f"all {self.dtype}")
+        if rotary.device != self.device or rotary.head_dim != self.head_dim:
+            raise ValueError("the rotary's device and head_dim differ from the cache's")
+        a, out, keep = rotary._args(q, k, v, positions, q_norm, k_norm, eps, inverse)
+        a.seq = q.shape[1]
         if positions is None:
             a.base = self.next_pos.data_ptr()
-        if q.shape[1] == 0:
-            return out
-        with torch.cuda.device(self.device):
-            _abi.check(_abi.lib().tp_rotary(ctypes.addressof(a), self._layer(layer), _abi.stream_of(q)), "append")
+        addr = self._layer(layer)
+        if a.seq:
+            _abi.launch(_abi.lib().tp_rotary, "append", self.device.index, ctypes.addressof(a), addr)
         return out
+
+    def advance(self, tokens: int | Tensor) -> None:
+        """Count ``tokens`` (a number, or int32 [batch]) as cached: after the
+        last layer's ``append``.  Idle sequences stay idle.  Fewer than were
+        appended drops the last ones (rejected drafts)."""
+        live = (self.lengths >= 0).int() * tokens
+        self.lengths.add_(live)
+        self.next_pos.add_(live)
 
     def attend(self, q: Tensor, *, layer: int = 0, scale: float | None = None, accumulate: bool = False,
                return_lse: bool = False):
@@ -177,6 +168,29 @@ class PagedKVCache:
         ``accumulate`` adds each slot's attention weight to ``scores``.  A row
         that sees nothing (an idle sequence) gives zeros.  Returns out in q's
         shape, with the fp32 log-sum-exp [batch, tokens, q_heads] on request."""
+        key = (_abi.meta(q), scale, accumulate)
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._checked(q, scale, accumulate)
+            if len(self._plans) >= 256:
+                self._plans.clear()
+            self._plans[key] = plan
+        addr = self._layer(layer)
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
+        if plan.tokens:
+            q = q.contiguous()
+            a = _AttnArgs.from_buffer_copy(plan)
+            a.q, a.out = q.data_ptr(), out.data_ptr()
+            if lse is not None:
+                a.lse = lse.data_ptr()
+            _abi.launch(_abi.lib().tp_paged_attn, "attend", self.device.index, ctypes.addressof(a), addr, self._ws.data_ptr(),
+                        self._ws.numel())
+        return (out, lse) if return_lse else out
+
+    def _checked(self, q: Tensor, scale: float | None, accumulate: bool) -> _AttnArgs:
+        """Checks an ``attend`` call by what its key holds; grows the workspace
+        (zero-filled) to its sizes."""
         if q.dim() != 4 or q.shape[0] != self.batch or q.shape[3] != self.head_dim:
             raise ValueError(f"expected q [{self.batch}, tokens, heads, {self.head_dim}], got {tuple(q.shape)}")
         if q.dtype != self.dtype or q.device != self.device:
@@ -184,25 +198,25 @@ class PagedKVCache:
         if accumulate and self.scores is None:
             raise ValueError("the cache keeps no scores to accumulate in")
         tokens, heads = q.shape[1], q.shape[2]
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
-        if tokens:
-            q = q.contiguous()
-            ws = self._workspace(tokens, heads, accumulate)
-            a = _AttnArgs(q.data_ptr(), out.data_ptr(), _abi.ptr(lse), tokens, heads,
-                          self.head_dim ** -0.5 if scale is None else scale, accumulate)
-            with torch.cuda.device(self.device):
-                _abi.check(_abi.lib().tp_paged_attn(ctypes.addressof(a), self._layer(layer), ws.data_ptr(), ws.numel(),
-                                                    _abi.stream_of(q)), "attend")
-        return (out, lse) if return_lse else out
+        template = _AttnArgs(tokens=tokens, q_heads=heads, softmax_scale=self.head_dim ** -0.5 if scale is None else scale,
+                             accumulate=accumulate)
+        if tokens == 0:
+            return template
+        need = _abi.lib().tp_paged_attn_workspace_bytes(ctypes.addressof(self._structs[0]), tokens, heads, accumulate)
+        if need < 0:
+            _abi.check(-need, "attend")
+        self._ws = self._grown(self._ws, need)
+        return template
 
-    def advance(self, tokens: int | Tensor) -> None:
-        """Count ``tokens`` (a number, or int32 [batch]) as cached: after the
-        last layer's ``append``.  Idle sequences stay idle.  Fewer than were
-        appended drops the last ones (rejected drafts)."""
-        live = (self.lengths >= 0).int() * tokens
-        self.lengths.add_(live)
-        self.next_pos.add_(live)
+    def _grown(self, ws: Tensor | None, need: int) -> Tensor:
+        """``ws`` if it holds ``need`` bytes, else a zero-filled one that does."""
+        if ws is not None and ws.numel() >= need:
+            return ws
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the workspace has to grow: run this call once before capturing it")
+        if ws is not None:
+            self._outgrown.append(ws)
+        return torch.zeros(need, dtype=torch.uint8, device=self.device)
 
     # -- a bounded cache --------------------------------------------------------
     def evict_slots(self, budget: int, *, recent: int = 0, sinks: int = 0, layer: int = 0) -> tuple[Tensor, Tensor, Tensor]:
@@ -215,19 +229,15 @@ class PagedKVCache:
         ``evict`` does all layers and takes them over."""
         if self.scores is None or self.positions is None:
             raise ValueError("eviction needs a cache with scores and positions")
-        addr = self._layer(layer)
+        addr, lib = self._layer(layer), _abi.lib()
         new = (torch.empty_like(self.lengths), torch.empty_like(self.scores[layer]), torch.empty_like(self.positions[layer]))
-        with torch.cuda.device(self.device):
-            lib = _abi.lib()
-            need = lib.tp_cache_evict_workspace_bytes(addr, budget)
-            if need < 0:
-                _abi.check(-need, "evict")
-            if self._evict_ws is None or self._evict_ws.numel() < need:
-                self._evict_ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-            a = _EvictArgs(self.next_pos.data_ptr(), new[0].data_ptr(), new[1].data_ptr(), new[2].data_ptr(), budget, recent,
-                           sinks)
-            _abi.check(lib.tp_cache_evict(ctypes.addressof(a), addr, self._evict_ws.data_ptr(), self._evict_ws.numel(),
-                                          _abi.stream_of(self.lengths)), "evict")
+        need = lib.tp_cache_evict_workspace_bytes(addr, budget)
+        if need < 0:
+            _abi.check(-need, "evict")
+        self._evict_ws = self._grown(self._evict_ws, need)
+        a = _EvictArgs(self.next_pos.data_ptr(), new[0].data_ptr(), new[1].data_ptr(), new[2].data_ptr(), budget, recent, sinks)
+        _abi.launch(lib.tp_cache_evict, "evict", self.device.index, ctypes.addressof(a), addr, self._evict_ws.data_ptr(),
+                    self._evict_ws.numel())
         return new
 
     def evict(self, budget: int, *, recent: int = 0, sinks: int = 0) -> None:

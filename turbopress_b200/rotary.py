@@ -114,6 +114,7 @@ class Rotary:
         words = [round(Fraction(f) * _TURNS) % 2 ** 64 for f in self.inv_freq.tolist()]
         self.freq = torch.tensor([w - 2 ** 64 if w >= 2 ** 63 else w for w in words], dtype=torch.int64).to(device)
         self.device = self.freq.device
+        self._plans: dict[tuple, _RotaryArgs] = {}
 
     @classmethod
     def from_config(cls, config, device="cuda", interleaved: bool = False) -> "Rotary":
@@ -127,35 +128,67 @@ class Rotary:
         return cls(head_dim, theta=theta, scaling=p, rot_dim=int(head_dim * part), interleaved=interleaved, device=device)
 
     # -- arguments shared with PagedKVCache.append ------------------------------
-    def _args(self, q: Tensor, k: Tensor, positions: Tensor | None, q_norm: Tensor | None, k_norm: Tensor | None,
-              eps: float, inverse: bool) -> tuple[_RotaryArgs, Tensor, list[Tensor]]:
+    def _args(self, q: Tensor, k: Tensor, v: Tensor | None, positions: Tensor | None, q_norm: Tensor | None,
+              k_norm: Tensor | None, eps: float, inverse: bool) -> tuple[_RotaryArgs, Tensor, tuple]:
         """The call's arguments without k's destination, the queries' output and
         the tensors to keep until the launch."""
+        key = (_abi.meta(q), _abi.meta(k), _abi.meta(v), _abi.meta(positions), _abi.meta(q_norm), _abi.meta(k_norm))
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._checked(q, k, v, positions, q_norm, k_norm)
+            if plan is None:  # not views of [tokens, heads, head_dim]
+                return self._args(q.contiguous(), k.contiguous(), None if v is None else v.contiguous(), positions, q_norm,
+                                  k_norm, eps, inverse)
+            if len(self._plans) >= 256:
+                self._plans.clear()
+            self._plans[key] = plan
+        if positions is not None:
+            positions = positions.to(torch.int64).contiguous()
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        a = _RotaryArgs.from_buffer_copy(plan)
+        a.q, a.k, a.q_out, a.inverse, a.eps = q.data_ptr(), k.data_ptr(), out.data_ptr(), inverse, eps
+        if v is not None:
+            a.v = v.data_ptr()
+        if positions is not None:
+            a.positions = positions.data_ptr()
+        if q_norm is not None:
+            a.q_norm = q_norm.data_ptr()
+        if k_norm is not None:
+            a.k_norm = k_norm.data_ptr()
+        return a, out, (q, k, v, positions)
+
+    def _checked(self, q: Tensor, k: Tensor, v: Tensor | None, positions: Tensor | None, q_norm: Tensor | None,
+                 k_norm: Tensor | None) -> _RotaryArgs | None:
+        """The part of the arguments that shapes, strides and dtypes decide;
+        None where q, k or v is not a view of [tokens, heads, head_dim]."""
         hd = self.head_dim
         if q.dim() < 2 or k.dim() != q.dim() or q.shape[-1] != hd or k.shape[-1] != hd or q.shape[:-2] != k.shape[:-2]:
             raise ValueError(f"q and k must be [..., heads, {hd}] over the same tokens, got {tuple(q.shape)} and {tuple(k.shape)}")
-        if k.dtype != q.dtype or q.device != self.device or k.device != self.device:
-            raise ValueError("q and k must share one dtype and be on the frequencies' CUDA device")
-        q3, k3 = q.reshape(-1, q.shape[-2], hd), k.reshape(-1, k.shape[-2], hd)
-        if q3.stride(2) != 1:
-            q3 = q3.contiguous()
-        if k3.stride(2) != 1:
-            k3 = k3.contiguous()
-        keep = [q3, k3]
-        if positions is not None:
-            if positions.shape != q.shape[:-2] or positions.device != self.device:
-                raise ValueError(f"positions must be {tuple(q.shape[:-2])} on {self.device}, got {tuple(positions.shape)}")
-            positions = positions.to(torch.int64).contiguous()
-            keep.append(positions)
+        for t in (q, k, v):
+            if t is not None and (t.dtype != q.dtype or t.device != self.device):
+                raise ValueError("q, k and v must share one dtype and be on the frequencies' CUDA device")
+        if v is not None and v.shape != k.shape:
+            raise ValueError(f"v must have k's shape {tuple(k.shape)}, got {tuple(v.shape)}")
+        if positions is not None and (positions.shape != q.shape[:-2] or positions.device != self.device):
+            raise ValueError(f"positions must be {tuple(q.shape[:-2])} on {self.device}, got {tuple(positions.shape)}")
         for w in (q_norm, k_norm):
             if w is not None and (w.shape != (hd,) or w.dtype != q.dtype or w.device != self.device or not w.is_contiguous()):
                 raise ValueError(f"norm weights must be contiguous [{hd}] tensors of the queries' dtype and device")
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        a = _RotaryArgs(q3.data_ptr(), k3.data_ptr(), None, out.data_ptr(), None, _abi.ptr(positions), None,
-                        self.freq.data_ptr(), _abi.ptr(q_norm), _abi.ptr(k_norm), q3.stride(0), q3.stride(1), k3.stride(0),
-                        k3.stride(1), 0, 0, q3.shape[0], 1, q3.shape[1], k3.shape[1], hd, self.rot_dim,
-                        _abi.dtype_code(q.dtype), self.interleaved, inverse, self.scale, eps)
-        return a, out, keep
+        a = _RotaryArgs(freq=self.freq.data_ptr(), seq=1, q_heads=q.shape[-2], kv_heads=k.shape[-2], head_dim=hd,
+                        rot_dim=self.rot_dim, dtype=_abi.dtype_code(q.dtype), interleaved=self.interleaved, scale=self.scale)
+        for nm, t in (("q", q), ("k", k), ("v", v)):
+            if t is None:
+                continue
+            try:
+                flat = t.view(-1, t.shape[-2], hd) if t.numel() else t.reshape(0, t.shape[-2], hd)
+            except RuntimeError:
+                return None
+            if flat.stride(2) != 1:
+                return None
+            setattr(a, nm + "_token_stride", flat.stride(0))
+            setattr(a, nm + "_head_stride", flat.stride(1))
+        a.tokens = math.prod(q.shape[:-2])
+        return a
 
     def __call__(self, q: Tensor, k: Tensor, positions: Tensor, *, q_norm: Tensor | None = None,
                  k_norm: Tensor | None = None, eps: float = 1e-6, inverse: bool = False) -> tuple[Tensor, Tensor]:
@@ -166,9 +199,8 @@ class Rotary:
         the rotation."""
         if positions is None:
             raise ValueError("positions are needed")
-        a, q_out, keep = self._args(q, k, positions, q_norm, k_norm, eps, inverse)
+        a, q_out, keep = self._args(q, k, None, positions, q_norm, k_norm, eps, inverse)
         k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         a.k_out = k_out.data_ptr()
-        with torch.cuda.device(self.device):
-            _abi.check(_abi.lib().tp_rotary(ctypes.addressof(a), None, _abi.stream_of(q)), "rotary")
+        _abi.launch(_abi.lib().tp_rotary, "rotary", self.device.index, ctypes.addressof(a), None)
         return q_out, k_out

@@ -50,6 +50,7 @@ class DraftVerifier:
         self.workspace = torch.zeros(need, dtype=torch.uint8, device=device)
         self.device = self.workspace.device
         _abi.require_cuda(self.workspace)
+        self._plans: dict[tuple, _VerifyArgs] = {}
 
     def __call__(self, logits: Tensor, draft_tokens: Tensor, *, uniforms: Tensor | None = None, noise: Tensor | None = None,
                  draft_probs: Tensor | None = None, temperature: Tensor | None = None,
@@ -61,6 +62,36 @@ class DraftVerifier:
         [batch] (0: greedy; None: all greedy), n_drafts int32 [batch] (drafts
         in use; None: all).  Returns accepted int32 [batch] and tokens int64
         [batch, drafts + 1]: the accepted drafts, the next token, then -1."""
+        key = (_abi.meta(logits), _abi.meta(draft_tokens), _abi.meta(uniforms), _abi.meta(noise), _abi.meta(draft_probs),
+               _abi.meta(temperature), _abi.meta(n_drafts))
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._checked(logits, draft_tokens, uniforms, noise, draft_probs, temperature, n_drafts)
+            if len(self._plans) >= 256:
+                self._plans.clear()
+            self._plans[key] = plan
+        B, rows = plan.batch, plan.drafts + 1
+        accepted = torch.empty(B, dtype=torch.int32, device=self.device)
+        tokens = torch.empty(B, rows, dtype=torch.int64, device=self.device)
+        a = _VerifyArgs.from_buffer_copy(plan)
+        a.logits, a.draft_tokens, a.accepted, a.tokens = (logits.data_ptr(), draft_tokens.data_ptr(), accepted.data_ptr(),
+                                                          tokens.data_ptr())
+        if temperature is not None:
+            a.temperature, a.noise = temperature.data_ptr(), noise.data_ptr()
+            if uniforms is not None:
+                a.uniforms = uniforms.data_ptr()
+            if draft_probs is not None:
+                a.draft_probs = draft_probs.data_ptr()
+        if n_drafts is not None:
+            a.counts = n_drafts.data_ptr()
+        _abi.launch(_abi.lib().tp_verify_drafts, "verify_drafts", self.device.index, ctypes.addressof(a),
+                    self.workspace.data_ptr(), self.workspace.numel())
+        return accepted, tokens
+
+    def _checked(self, logits: Tensor, draft_tokens: Tensor, uniforms: Tensor | None, noise: Tensor | None,
+                 draft_probs: Tensor | None, temperature: Tensor | None, n_drafts: Tensor | None) -> _VerifyArgs:
+        """Checks a call by what its key holds; the sizes and strides of its
+        arguments."""
         if logits.dim() != 3:
             raise ValueError(f"logits must be [batch, drafts + 1, vocab], got {tuple(logits.shape)}")
         B, rows, V = logits.shape
@@ -79,12 +110,5 @@ class DraftVerifier:
                 raise ValueError(f"{nm} must be a contiguous {dt} tensor {shape} on {self.device}")
         if logits.device != self.device:
             raise ValueError(f"logits must be on {self.device}")
-        accepted = torch.empty(B, dtype=torch.int32, device=self.device)
-        tokens = torch.empty(B, rows, dtype=torch.int64, device=self.device)
-        a = _VerifyArgs(logits.data_ptr(), logits.stride(0), logits.stride(1), draft_tokens.data_ptr(), _abi.ptr(draft_probs),
-                        _abi.ptr(uniforms), _abi.ptr(noise), _abi.ptr(temperature), _abi.ptr(n_drafts), accepted.data_ptr(),
-                        tokens.data_ptr(), B, K, V, _abi.dtype_code(logits.dtype))
-        with torch.cuda.device(self.device):
-            _abi.check(_abi.lib().tp_verify_drafts(ctypes.addressof(a), self.workspace.data_ptr(), self.workspace.numel(),
-                                                   _abi.stream_of(logits)), "verify_drafts")
-        return accepted, tokens
+        return _VerifyArgs(batch_stride=logits.stride(0), row_stride=logits.stride(1), batch=B, drafts=K, vocab=V,
+                           dtype=_abi.dtype_code(logits.dtype))
