@@ -499,6 +499,11 @@ TP_API int64_t tp_paged_attn_workspace_bytes(const tp_paged_cache* cache, int to
 TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_cache* cache, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* Reads (synchronizing `stream`) and clears the status word of a workspace of
+ * tp_paged_attn: TP_OK, or TP_ERR_DEVICE when a wait for a copy gave up (the
+ * outputs of that call are NaN; the workspace is fit for the next). */
+TP_API tp_status tp_paged_attn_status(void* workspace, void* stream);
+
 /* Eviction: of each sequence's slots keep the `budget` that come first by
  * (guarded, score, lower slot), per kv head, where a slot is guarded when its
  * position is below `sinks` or at least next_pos[b] - recent.  Scores compare

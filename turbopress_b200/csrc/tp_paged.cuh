@@ -50,6 +50,12 @@ inline tp_status device_sms(int* sms) {
   return TP_OK;
 }
 
+// N neighbouring elements, accessed 16 bytes at a time at most.
+template <class T, int VEC>
+struct alignas(VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16) Pack {
+  T v[VEC];
+};
+
 // Element types of the kernels.
 template <class T>
 struct Elem;

@@ -20,11 +20,16 @@
 // arrive (a counter at the item's first CTA) joins them in run order, so the
 // result does not depend on timing.
 //
-// Tile: each of the four warps copies its own 16 tokens of K and V with
-// 16-byte asynchronous copies (page ids one tile ahead, unseen slots
-// zero-filled, so whatever they hold stays out) and, up to 16 rows, also
-// consumes only those: no CTA barrier in the loop.  With more rows the warps
-// share the tile: MT row tiles of 16, 4/MT warps each.
+// Tile: each of the four warps fetches its own 16 tokens of K and V as tensor
+// (TMA) boxes of up to 16 tokens x 128 bytes, one page id per box fetched one
+// tile ahead, two tiles in flight behind the one in use; the hardware's
+// 128-byte swizzle makes the fragment loads conflict-free.  Up to 16 rows a
+// warp consumes only what it fetched: no CTA barrier in the loop.  With more
+// rows the warps share the tile: MT row tiles of 16, 4/MT warps each.  Slots
+// that a row does not see may hold anything: their scores are replaced and
+// their V zeroed in registers, in the blocks where that can happen.
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "tp_decode.cuh"
@@ -38,35 +43,42 @@ constexpr int kPaThreads = 128;
 constexpr int kPaWarps = 4;
 constexpr int kPaTile = 64;
 constexpr int kPaMaxCtas = 512;
-constexpr int kPaCounterBytes = kPaMaxCtas * 4;
+constexpr int kPaStatusOff = kPaMaxCtas * 4;      // status word after the counters
+constexpr int kPaCounterBytes = kPaStatusOff + 256;
 
 struct AttnParams {
+  CUtensorMap k_map, v_map;  // {head_dim, token | head, head | token, page}
   const void* q;
   void* out;
   float* lse;
-  const void* k_pages;
-  const void* v_pages;
   const int32_t* block_table;
   const int32_t* lengths;
   float* scores;
-  int64_t num_pages, page_stride, head_stride, token_stride, table_stride;
+  int64_t num_pages, table_stride;
+  int token_major;  // the maps' second dimension is the head
+  int lg_box;       // log2 of the tokens per box: min(16, page_size)
   int batch, tokens, q_heads, kv_heads, group, head_dim;
   int lg_page, capacity;
   int rows;      // tokens * group: query rows of a kv head
   int row_tiles;
   float scale_log2;
   unsigned* counters;
+  unsigned* status;
   float* part_o;   // [ctas][2][16*MT][HD]
   float2* part_ml; // [ctas][2][16*MT]
   float* lse2;     // [batch][kv_heads][rows] log2 units (accumulate only)
   float* sbuf;     // [tiles][16*MT][64] scores in log2 units (accumulate only)
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
   const int bytes = on ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
@@ -140,9 +152,15 @@ __device__ __forceinline__ int seq_tiles(const AttnParams& p, int len) {
   return n * p.kv_heads;
 }
 
-struct Cursor {  // one tile: sequence, row tile, kv head, tile of the item
-  int b, rt, h, tile, n, len;
+struct Cursor {  // one tile: sequence, row tile, kv head, tile of the item, the item's tiles and last seen slot + 1
+  int b, rt, h, tile, n, hi, len;
 };
+
+template <int RT>
+__device__ __forceinline__ void set_item(const AttnParams& p, Cursor& c) {
+  c.hi = visible(p, c.len, min(p.rows, (c.rt + 1) * RT) - 1);
+  c.n = max(1, (c.hi + kPaTile - 1) / kPaTile);
+}
 
 template <int RT>
 __device__ __forceinline__ void step_cursor(const AttnParams& p, Cursor& c) {
@@ -155,7 +173,7 @@ __device__ __forceinline__ void step_cursor(const AttnParams& p, Cursor& c) {
     if (++c.b == p.batch) return;  // past the end: the caller does not use it
     c.len = p.lengths[c.b];
   }
-  c.n = item_tiles<RT>(p, c.len, c.rt);
+  set_item<RT>(p, c);
 }
 
 // Sum over the block of one value per thread (all threads call it).
@@ -214,36 +232,43 @@ __device__ __forceinline__ void find_sequence(const AttnParams& p, int t0, F cou
 // ---------------------------------------------------------------------------
 template <int HD, int MT>
 struct PaShape {
-  static constexpr int RT = 16 * MT;                      // rows of an item
-  static constexpr int WT = kPaWarps / MT;                // warps along the tokens
-  static constexpr int CH = HD / 8;                       // 16-byte chunks per token
-  static constexpr int kTokBytes = HD * 2;
-  static constexpr int kKV = kPaTile * kTokBytes;         // bytes of a K (or V) tile
-  static constexpr int kQ = RT * kTokBytes;
+  static constexpr int RT = 16 * MT;                 // rows of an item
+  static constexpr int WT = kPaWarps / MT;           // warps along the tokens
+  static constexpr int CH = HD / 8;                  // 16-byte chunks per token
+  static constexpr int kPanels = HD / 64;            // 128-byte columns of a 16-token block
+  static constexpr int kBlock = 16 * HD * 2;         // K (or V) of a block: [panel][16][128 bytes], swizzled
+  static constexpr int kKV = (kPaTile / 16) * kBlock;
+  static constexpr int kQ = RT * HD * 2;
   static constexpr int kStage = 2 * kKV + kQ;
   // three tiles per CTA, two where three with the queries pass 227 KB
   static constexpr int kStages = HD == 256 && MT > 1 ? 2 : 3;
   static constexpr int kSmem = kStages * kStage;
   static_assert(kSmem <= 227 * 1024 - 1024, "shared memory");
-  static_assert(kPaWarps * 16 * HD * 4 <= kStage, "the join buffer reuses a consumed stage");
+  static_assert(kStage % 1024 == 0, "the swizzle repeats every 1024 bytes");
+  static_assert(kPaWarps * 16 * HD * 4 <= 2 * kKV, "the join buffer reuses a consumed stage");
 };
 
 template <class T, int HD, int MT, bool WEIGHTS>
 __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_constant__ AttnParams p) {
   using S = PaShape<HD, MT>;
   constexpr int RT = S::RT, WT = S::WT, CH = S::CH, kStages = S::kStages;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ int s_tmp[8];
-  __shared__ uint32_t s_valid[kStages][kPaWarps];
+  __shared__ __align__(8) uint64_t s_full[kStages][kPaWarps];  // one per block of 16 tokens
+  __shared__ uint32_t s_valid[kStages][kPaWarps];              // its tokens that have a page
   __shared__ float s_m[kPaWarps][16], s_l[kPaWarps][16];
   __shared__ bool s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sbase = smem_u32(smem);
+  if (tid == 0) {
+    for (int i = 0; i < kStages * kPaWarps; ++i) mbar_init(&s_full[0][0] + i, 1);
+    fence_mbar_init();
+  }
 
   // ---- this CTA's run of tiles ----
   int cnt = 0;
   for (int b = tid; b < p.batch; b += kPaThreads) cnt += seq_tiles<RT>(p, p.lengths[b]);
-  const int total = block_sum(cnt, s_tmp);
+  const int total = block_sum(cnt, s_tmp);  // (its barriers also publish the mbarriers)
   const int per = (total + gridDim.x - 1) / gridDim.x;
   const int t0 = min((int)blockIdx.x * per, total), t1 = min(t0 + per, total);
   if (WEIGHTS) pdl_trigger();
@@ -254,7 +279,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   c.len = p.lengths[c.b];
   int rem = t0 - before;
   for (c.rt = 0;; ++c.rt) {
-    c.n = item_tiles<RT>(p, c.len, c.rt);
+    set_item<RT>(p, c);
     if (rem < p.kv_heads * c.n) break;
     rem -= p.kv_heads * c.n;
   }
@@ -262,33 +287,38 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   c.tile = rem - c.h * c.n;
   Cursor ld = c;
 
-  // ---- loads ----
+  // ---- loads: lane i < boxes of a warp fetches box i of the warp's block ----
+  const int boxes = 16 >> p.lg_box;
   const int page_mask = (1 << p.lg_page) - 1;
-  const T* kp = static_cast<const T*>(p.k_pages);
-  const T* vp = static_cast<const T*>(p.v_pages);
-  auto page_of = [&](const Cursor& u) {  // of this lane's token (lanes 16.. repeat 0..)
-    const int tok = u.tile * kPaTile + warp * 16 + (lane & 15);
-    return tok < p.capacity ? p.block_table[u.b * p.table_stride + (tok >> p.lg_page)] : -1;
+  auto page_of = [&](const Cursor& u) {  // of this lane's box
+    const int tok = u.tile * kPaTile + warp * 16 + (lane << p.lg_box);
+    return lane < boxes && tok < p.capacity ? p.block_table[u.b * p.table_stride + (tok >> p.lg_page)] : -1;
   };
   int pid = page_of(ld);
-  auto issue = [&](int t, bool first) {  // tile t of the index space, at cursor ld
-    const int stage = (t - t0) % kStages;
-    const uint32_t st = sbase + stage * S::kStage;
-    const int tok = ld.tile * kPaTile + warp * 16 + (lane & 15);
-    const int hi = visible(p, ld.len, min(p.rows, (ld.rt + 1) * RT) - 1);
-    const bool ok = tok < hi && pid >= 0 && pid < p.num_pages;
-    const int64_t off = ok ? pid * p.page_stride + ld.h * p.head_stride + (tok & page_mask) * p.token_stride : 0;
-    const uint32_t valid = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-    if (lane == 0) s_valid[stage][warp] = valid;
+  int ld_stage = 0;
+  auto issue = [&](bool first, bool more) {  // the tile at cursor ld, into stage ld_stage
+    const uint32_t st = sbase + ld_stage * S::kStage;
+    const int tok = ld.tile * kPaTile + warp * 16 + (lane << p.lg_box);
+    const bool ok = lane < boxes && tok < ld.hi && pid >= 0 && pid < p.num_pages;
+    const uint32_t got = __ballot_sync(0xffffffffu, ok);
+    const uint32_t bar = smem_u32(&s_full[ld_stage][warp]);
+    if (lane == 0) {
+      uint32_t valid = 0;
+      for (int i = 0; i < boxes; ++i)
+        if ((got >> i) & 1u) valid |= ((1u << (1 << p.lg_box)) - 1u) << (i << p.lg_box);
+      s_valid[ld_stage][warp] = valid;
+      const uint32_t bytes = __popc(got) * (S::kPanels * 2 * 128 << p.lg_box);
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+    }
+    __syncwarp();
+    if (ok) {
+      const int y = p.token_major ? ld.h : tok & page_mask, z = p.token_major ? tok & page_mask : ld.h;
+      const uint32_t d = st + warp * S::kBlock + ((lane << p.lg_box) << 7);
 #pragma unroll
-    for (int i = 0; i < 16 * CH / 32; ++i) {
-      const int r = i * (32 / CH) + lane / CH, chunk = lane % CH;
-      const int64_t o = __shfl_sync(0xffffffffu, off, r) + chunk * 8;
-      const bool on = ((valid >> r) & 1u) && chunk * 8 < p.head_dim;
-      const int row = warp * 16 + r;
-      const uint32_t d = st + row * S::kTokBytes + ((chunk ^ (row & 7)) << 4);
-      cp_async16_zfill(d, on ? kp + o : kp, on);
-      cp_async16_zfill(d + S::kKV, on ? vp + o : vp, on);
+      for (int i = 0; i < S::kPanels; ++i) {
+        tma_box(d + i * 2048, &p.k_map, i * 64, y, z, pid, bar);
+        tma_box(d + S::kKV + i * 2048, &p.v_map, i * 64, y, z, pid, bar);
+      }
     }
     if (ld.tile == 0 || first) {
       const T* q = static_cast<const T*>(p.q);
@@ -299,287 +329,350 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
         const int64_t o = on ? (((int64_t)ld.b * p.tokens + j) * p.q_heads + ld.h * p.group + row - j * p.group) *
                                        p.head_dim + chunk * 8
                              : 0;
-        cp_async16_zfill(st + 2 * S::kKV + r * S::kTokBytes + ((chunk ^ (r & 7)) << 4), q + o, on);
+        cp_async16_zfill(st + 2 * S::kKV + r * (HD * 2) + ((chunk ^ (r & 7)) << 4), q + o, on);
       }
     }
+    ld_stage = ld_stage + 1 == kStages ? 0 : ld_stage + 1;
     step_cursor<RT>(p, ld);
-    if (t + 1 < t1) pid = page_of(ld);
+    if (more) pid = page_of(ld);
   };
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    if (t0 + i < t1) issue(t0 + i, i == 0);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
+  for (int i = 0; i < kStages - 1; ++i)
+    if (t0 + i < t1) issue(i == 0, t0 + i + 1 < t1);
 
   // ---- state of this warp's 16 rows ----
   const int mt = warp / WT, tw = warp % WT;
   const int r0 = lane >> 2, cq = lane & 3;  // this thread: rows r0, r0 + 8, columns 2 cq + {0, 1} of each 8
-  float o[HD / 8][4];
-  uint32_t qf[HD / 16][4];
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  int vis[2] = {0, 0}, jr[2] = {0, 0};
-  int vis_lo = 0, j_lo = 0, j_hi = 0;
-  bool fresh = true;
+  bool dead = false;
+  int stage = 0, t = t0;
+  unsigned phase = 0;
 
-  for (int t = t0; t < t1; ++t) {
-    const int stage = (t - t0) % kStages;
-    const uint32_t st = sbase + stage * S::kStage;
-    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    if (MT > 1 || fresh) __syncthreads();  // tiles (MT > 1) and queries are shared by the warps
-    else __syncwarp();
-    if (t + kStages - 1 < t1) issue(t + kStages - 1, false);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-
-    if (fresh) {
+  while (t < t1) {  // an item, or this run's part of it
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the queries are here
+    uint32_t qf[HD / 16][4];
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
-        const int r = mt * 16 + (lane & 15), chunk = ks * 2 + (lane >> 4);
-        ldsm4(qf[ks], st + 2 * S::kKV + r * S::kTokBytes + ((chunk ^ (r & 7)) << 4));
-      }
-#pragma unroll
-      for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
-      const int row0 = c.rt * RT + mt * 16;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int row = row0 + r0 + 8 * e;
-        jr[e] = row / p.group;
-        vis[e] = row < p.rows ? visible(p, c.len, row) : 0;
-      }
-      const int last = min(row0 + 16, p.rows) - 1;
-      j_lo = row0 / p.group;
-      j_hi = last / p.group;  // < j_lo where this row tile of 16 is empty
-      vis_lo = last >= row0 ? visible(p, c.len, row0) : 0;
-      fresh = false;
-      __syncthreads();  // every warp has its queries: their buffer may be filled again
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      const int r = mt * 16 + (lane & 15), chunk = ks * 2 + (lane >> 4);
+      ldsm4(qf[ks], sbase + stage * S::kStage + 2 * S::kKV + r * (HD * 2) + ((chunk ^ (r & 7)) << 4));
     }
+    float o[HD / 8][4];
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const int row0 = c.rt * RT + mt * 16, last_row = min(row0 + 16, p.rows) - 1;
+    int jr[2], vis[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = row0 + r0 + 8 * e;
+      jr[e] = row / p.group;
+      vis[e] = row < p.rows ? visible(p, c.len, row) : 0;
+    }
+    const int j_lo = row0 / p.group, j_hi = last_row / p.group;  // j_hi < j_lo where these 16 rows are empty
+    const int vis_lo = last_row >= row0 ? visible(p, c.len, row0) : 0;
+    const int t_end = min(t1, t + c.n - c.tile);
 
-    // blocks of 16 tokens: one per warp at MT = 1, MT of them otherwise
+    for (bool head = true;; head = false) {
+      // Every warp has its queries, and is done with the stage that is filled
+      // next (last read in the round before; at MT = 1 by this warp alone).
+      if (MT > 1 || head) __syncthreads();
+      else __syncwarp();
+      if (t + kStages - 1 < t1) issue(false, t + kStages < t1);
+      const uint32_t st = sbase + stage * S::kStage;
+
+      // blocks of 16 tokens: one per warp at MT = 1, MT of them otherwise
 #pragma unroll 1
-    for (int blk = tw * MT; blk < (tw + 1) * MT; ++blk) {
-      const int tok0 = c.tile * kPaTile + blk * 16;
-      const uint32_t valid = s_valid[stage][blk];
-      const uint32_t kb = st + blk * 16 * S::kTokBytes;
-      float s[2][4];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
-        uint32_t kf[4];
-        const int r = (lane & 7) + ((lane >> 4) << 3), chunk = ks * 2 + ((lane >> 3) & 1);
-        ldsm4(kf, kb + r * S::kTokBytes + ((chunk ^ (r & 7)) << 4));
-        Mma<T>::run(s[0], qf[ks], kf[0], kf[1]);
-        Mma<T>::run(s[1], qf[ks], kf[2], kf[3]);
-      }
-      const bool whole = valid == 0xffffu && tok0 + 16 <= vis_lo;  // every slot seen by every row
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int col = n * 8 + cq * 2 + (e & 1);
-          const bool seen = whole || (((valid >> col) & 1u) && tok0 + col < vis[e >> 1]);
-          s[n][e] = seen ? s[n][e] * p.scale_log2 : -INFINITY;
+      for (int blk = tw * MT; blk < (tw + 1) * MT; ++blk) {
+        const int tok0 = c.tile * kPaTile + blk * 16;
+        if (!dead && !mbar_wait(&s_full[stage][blk], phase)) {
+          dead = true;  // reported through the status word; the outputs become NaN
+          atomicOr(p.status, 1u);
         }
-      if (WEIGHTS) {
+        const uint32_t valid = s_valid[stage][blk];
+        const uint32_t kb = st + blk * S::kBlock;
+        float s[2][4], s2[2][4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (c.rt * RT + mt * 16 + r0 + 8 * e < p.rows)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-              *reinterpret_cast<float2*>(p.sbuf + ((size_t)t * RT + mt * 16 + r0 + 8 * e) * kPaTile + blk * 16 + n * 8 +
-                                         cq * 2) = make_float2(s[n][2 * e], s[n][2 * e + 1]);
-      }
-      // running maximum: the quad of four lanes shares a row
-      float mn[2];
+          for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float x = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-        mn[e] = fmaxf(m[e], x);
-      }
-      if (__any_sync(0xffffffffu, mn[0] != m[0] || mn[1] != m[1])) {
-        const float a0 = exp2_diff(m[0], mn[0]), a1 = exp2_diff(m[1], mn[1]);
-        m[0] = mn[0];
-        m[1] = mn[1];
-        l[0] *= a0;
-        l[1] *= a1;
-#pragma unroll
-        for (int n = 0; n < HD / 8; ++n) {
-          o[n][0] *= a0;
-          o[n][1] *= a0;
-          o[n][2] *= a1;
-          o[n][3] *= a1;
+        for (int ks = 0; ks < HD / 16; ++ks) {  // two chains of products per score
+          uint32_t kf[4];
+          const int r = (lane & 7) + ((lane >> 4) << 3), chunk = ks * 2 + ((lane >> 3) & 1);
+          ldsm4(kf, kb + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
+          Mma<T>::run(ks & 1 ? s2[0] : s[0], qf[ks], kf[0], kf[1]);
+          Mma<T>::run(ks & 1 ? s2[1] : s[1], qf[ks], kf[2], kf[3]);
         }
-      }
-      const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        s[n][0] = exp2f(s[n][0] - b0);
-        s[n][1] = exp2f(s[n][1] - b0);
-        s[n][2] = exp2f(s[n][2] - b1);
-        s[n][3] = exp2f(s[n][3] - b1);
-        l[0] += s[n][0] + s[n][1];
-        l[1] += s[n][2] + s[n][3];
-      }
-      uint32_t ph[4], pl[4];
-      Mma<T>::split(s[0][0], s[0][1], ph[0], pl[0]);
-      Mma<T>::split(s[0][2], s[0][3], ph[1], pl[1]);
-      Mma<T>::split(s[1][0], s[1][1], ph[2], pl[2]);
-      Mma<T>::split(s[1][2], s[1][3], ph[3], pl[3]);
-      const uint32_t vb = kb + S::kKV;
-      // Rows of several step tokens differ in the last slots they see.  There
-      // each token's product takes V with the slots it does not see zeroed
-      // (0 * inf would be NaN), and only its own rows of the result.  (With one
-      // token the slots past the last it sees were zero-filled.)
-      const bool mixed = p.tokens > 1 && tok0 + 16 > vis_lo;
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int nn = 0; nn < HD / 16; ++nn) {
-        uint32_t vf[4];
-        const int r = lane & 15, chunk = nn * 2 + (lane >> 4);
-        ldsm4t(vf, vb + r * S::kTokBytes + ((chunk ^ (r & 7)) << 4));
-        if (!mixed) {
-          Mma<T>::run(o[2 * nn], ph, vf[0], vf[1]);
-          Mma<T>::run(o[2 * nn], pl, vf[0], vf[1]);
-          Mma<T>::run(o[2 * nn + 1], ph, vf[2], vf[3]);
-          Mma<T>::run(o[2 * nn + 1], pl, vf[2], vf[3]);
-        } else {
-#pragma unroll 1
-          for (int j = j_lo; j <= j_hi; ++j) {
-            const int see = visible(p, c.len, j * p.group) - tok0;  // slots of this block
-            uint32_t w[4];
+          for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + s2[n][e]) * p.scale_log2;
+        const bool whole = valid == 0xffffu && tok0 + 16 <= vis_lo;  // every slot seen by every row
+        if (!whole) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int k = cq * 2 + 8 * (e & 1);
-              const uint32_t keep = (k < see ? 0x0000ffffu : 0u) | (k + 1 < see ? 0xffff0000u : 0u);
-              w[e] = vf[e] & keep;
+              const int col = n * 8 + cq * 2 + (e & 1);
+              if (!((valid >> col) & 1u) || tok0 + col >= vis[e >> 1]) s[n][e] = -INFINITY;
             }
-            float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-            Mma<T>::run(x, ph, w[0], w[1]);
-            Mma<T>::run(x, pl, w[0], w[1]);
-            Mma<T>::run(y, ph, w[2], w[3]);
-            Mma<T>::run(y, pl, w[2], w[3]);
+        }
+        if (WEIGHTS) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (jr[e >> 1] == j) {
-                o[2 * nn][e] += x[e];
-                o[2 * nn + 1][e] += y[e];
-              }
+          for (int e = 0; e < 2; ++e)
+            if (c.rt * RT + mt * 16 + r0 + 8 * e < p.rows)
+#pragma unroll
+              for (int n = 0; n < 2; ++n)
+                *reinterpret_cast<float2*>(p.sbuf + ((size_t)t * RT + mt * 16 + r0 + 8 * e) * kPaTile + blk * 16 + n * 8 +
+                                           cq * 2) = make_float2(s[n][2 * e], s[n][2 * e + 1]);
+        }
+        // running maximum: the quad of four lanes shares a row
+        float mn[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          mn[e] = fmaxf(m[e], x);
+        }
+        if (__any_sync(0xffffffffu, mn[0] != m[0] || mn[1] != m[1])) {
+          const float a0 = exp2_diff(m[0], mn[0]), a1 = exp2_diff(m[1], mn[1]);
+          m[0] = mn[0];
+          m[1] = mn[1];
+          l[0] *= a0;
+          l[1] *= a1;
+#pragma unroll
+          for (int n = 0; n < HD / 8; ++n) {
+            o[n][0] *= a0;
+            o[n][1] *= a0;
+            o[n][2] *= a1;
+            o[n][3] *= a1;
           }
         }
+        const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          s[n][0] = exp2f(s[n][0] - b0);
+          s[n][1] = exp2f(s[n][1] - b0);
+          s[n][2] = exp2f(s[n][2] - b1);
+          s[n][3] = exp2f(s[n][3] - b1);
+          l[0] += s[n][0] + s[n][1];
+          l[1] += s[n][2] + s[n][3];
+        }
+        uint32_t ph[4], pl[4];
+        Mma<T>::split(s[0][0], s[0][1], ph[0], pl[0]);
+        Mma<T>::split(s[0][2], s[0][3], ph[1], pl[1]);
+        Mma<T>::split(s[1][0], s[1][1], ph[2], pl[2]);
+        Mma<T>::split(s[1][2], s[1][3], ph[3], pl[3]);
+        const uint32_t vb = kb + S::kKV;
+        if (whole) {
+#pragma unroll
+          for (int nn = 0; nn < HD / 16; ++nn) {
+            uint32_t vf[4];
+            const int r = lane & 15, chunk = nn * 2 + (lane >> 4);
+            ldsm4t(vf, vb + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
+            Mma<T>::run(o[2 * nn], ph, vf[0], vf[1]);
+            Mma<T>::run(o[2 * nn + 1], ph, vf[2], vf[3]);
+            Mma<T>::run(o[2 * nn], pl, vf[0], vf[1]);
+            Mma<T>::run(o[2 * nn + 1], pl, vf[2], vf[3]);
+          }
+        } else {
+          // Some slots are not seen by some rows, and 0 * (what they hold) may be
+          // NaN: each step token's product takes V with the slots it does not see
+          // zeroed, and only its own rows of the result.
+#pragma unroll
+          for (int nn = 0; nn < HD / 16; ++nn) {
+            uint32_t vf[4];
+            const int r = lane & 15, chunk = nn * 2 + (lane >> 4);
+            ldsm4t(vf, vb + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
+#pragma unroll 1
+            for (int j = j_lo; j <= j_hi; ++j) {
+              const int see = visible(p, c.len, j * p.group) - tok0;  // slots of this block
+              const uint32_t seen = see >= 16 ? valid : see <= 0 ? 0u : valid & ((1u << see) - 1u);
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int k = cq * 2 + 8 * (e & 1);
+                w[e] = vf[e] & (((seen >> k) & 1u ? 0x0000ffffu : 0u) | ((seen >> (k + 1)) & 1u ? 0xffff0000u : 0u));
+              }
+              float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+              Mma<T>::run(x, ph, w[0], w[1]);
+              Mma<T>::run(y, ph, w[2], w[3]);
+              Mma<T>::run(x, pl, w[0], w[1]);
+              Mma<T>::run(y, pl, w[2], w[3]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (jr[e >> 1] == j) {
+                  o[2 * nn][e] += x[e];
+                  o[2 * nn + 1][e] += y[e];
+                }
+            }
+          }
+        }
+      }
+      if (t + 1 == t_end) break;
+      ++t;
+      ++c.tile;
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1u;
       }
     }
 
     // ---- the end of this CTA's part of the item ----
-    if (c.tile + 1 == c.n || t + 1 == t1) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (dead) l[e] = __int_as_float(0x7fc00000);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
+      if (cq == 0) {
+        s_m[warp][r0 + 8 * e] = m[e];
+        s_l[warp][r0 + 8 * e] = l[e];
+      }
+    }
+    __syncthreads();  // every warp is done with this tile: its stage becomes the join buffer
+    float* buf = reinterpret_cast<float*>(smem + stage * S::kStage);  // [warp][16][HD], 32-byte groups swizzled
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-        if (cq == 0) {
-          s_m[warp][r0 + 8 * e] = m[e];
-          s_l[warp][r0 + 8 * e] = l[e];
-        }
+        const int r = r0 + 8 * e;
+        *reinterpret_cast<float2*>(buf + (warp * 16 + r) * HD + ((n * 8 + cq * 2) ^ ((r & 7) << 3))) =
+            make_float2(o[n][2 * e], o[n][2 * e + 1]);
       }
-      __syncthreads();  // every warp is done with this tile: its stage becomes the join buffer
-      float* buf = reinterpret_cast<float*>(smem + stage * S::kStage);  // [warp][16][HD], 32-byte groups swizzled
+    __syncthreads();
+    const int begin = t - c.tile, end = begin + c.n;  // the item's tiles
+    const int c0 = begin / per, c1 = (end - 1) / per; // CTAs that share it
+    const bool alone = c0 == c1;
+    const int nrow = min(RT, p.rows - c.rt * RT);
+    const int slot = blockIdx.x == c0 ? 1 : 0;  // an item that began in an earlier CTA: slot 0
+    float* po = p.part_o + (size_t)(blockIdx.x * 2 + slot) * RT * HD;
+    float2* pml = p.part_ml + (blockIdx.x * 2 + slot) * RT;
+    const int64_t out0 = ((int64_t)c.b * p.tokens) * p.q_heads + c.h * p.group;
+    auto finish = [&](int r, int d, const auto& v, float M, float L) {  // row r, elements d..
+      constexpr int N = sizeof(v) / sizeof(float);
+      const int row = c.rt * RT + r, j = row / p.group;
+      const int64_t at = out0 + (int64_t)j * p.q_heads + row - j * p.group;
+      const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+      if (d < p.head_dim) {
+        Pack<T, N> w;
 #pragma unroll
-      for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = r0 + 8 * e;
-          *reinterpret_cast<float2*>(buf + (warp * 16 + r) * HD + ((n * 8 + cq * 2) ^ ((r & 7) << 3))) =
-              make_float2(o[n][2 * e], o[n][2 * e + 1]);
-        }
-      __syncthreads();
-      const int begin = t - c.tile, end = begin + c.n;  // the item's tiles
-      const int c0 = begin / per, c1 = (end - 1) / per; // CTAs that share it
-      const bool alone = c0 == c1;
-      const int nrow = min(RT, p.rows - c.rt * RT);
-      const int slot = blockIdx.x == c0 ? 1 : 0;  // an item that began in an earlier CTA: slot 0
-      float* po = p.part_o + (size_t)(blockIdx.x * 2 + slot) * RT * HD;
-      float2* pml = p.part_ml + (blockIdx.x * 2 + slot) * RT;
-      const int64_t out0 = ((int64_t)c.b * p.tokens) * p.q_heads + c.h * p.group;
-      auto finish = [&](int r, int d, float4 v, float M, float L) {  // row r, elements d..d+3
-        const int row = c.rt * RT + r, j = row / p.group;
-        const int64_t at = out0 + (int64_t)j * p.q_heads + row - j * p.group;
-        const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-        if (d < p.head_dim) {
-          T w[4] = {Elem<T>::from(v.x * inv), Elem<T>::from(v.y * inv), Elem<T>::from(v.z * inv),
-                    Elem<T>::from(v.w * inv)};
-          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * p.head_dim + d) = *reinterpret_cast<uint2*>(w);
-        }
-        if (d == 0) {
-          const float lg = L > 0.f || L != L ? M + log2f(L) : -INFINITY;
-          if (p.lse) p.lse[at] = lg * 0.6931471805599453f;
-          if (WEIGHTS) p.lse2[((int64_t)c.b * p.kv_heads + c.h) * p.rows + row] = lg;
-        }
-      };
-      for (int i = tid; i < nrow * (HD / 4); i += kPaThreads) {
-        const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-        const int w0 = (r / 16) * WT, rr = r % 16;
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < WT; ++w) M = fmaxf(M, s_m[w0 + w][rr]);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        float L = 0.f;
-#pragma unroll
-        for (int w = 0; w < WT; ++w) {
-          const float f = exp2_diff(s_m[w0 + w][rr], M);
-          const float4 x = *reinterpret_cast<const float4*>(buf + ((w0 + w) * 16 + rr) * HD + (d ^ ((rr & 7) << 3)));
-          L = fmaf(s_l[w0 + w][rr], f, L);
-          v.x = fmaf(x.x, f, v.x);
-          v.y = fmaf(x.y, f, v.y);
-          v.z = fmaf(x.z, f, v.z);
-          v.w = fmaf(x.w, f, v.w);
-        }
-        if (alone) {
-          finish(r, d, v, M, L);
-        } else {
-          *reinterpret_cast<float4*>(po + r * HD + d) = v;
-          if (d == 0) pml[r] = make_float2(M, L);
-        }
+        for (int e = 0; e < N; ++e) w.v[e] = Elem<T>::from(v[e] * inv);
+        *reinterpret_cast<Pack<T, N>*>(static_cast<T*>(p.out) + at * p.head_dim + d) = w;
       }
-      if (!alone) {
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-          const unsigned n = static_cast<unsigned>(c1 - c0 + 1);
-          s_last = atomicAdd(&p.counters[c0], 1u) == n - 1;
-          if (s_last) p.counters[c0] = 0u;
-        }
-        __syncthreads();
-        if (s_last) {
-          __threadfence();
-          for (int i = tid; i < nrow * (HD / 4); i += kPaThreads) {
-            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-            float M = -INFINITY, L = 0.f;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int k = c0; k <= c1; ++k) {
-              const size_t part = static_cast<size_t>(k * 2 + (k == c0 ? 1 : 0)) * RT + r;
-              const float2 ml = __ldcg(p.part_ml + part);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + part * HD + d));
-              const float mn = fmaxf(M, ml.x);
-              const float f = exp2_diff(M, mn), g = exp2_diff(ml.x, mn);
-              M = mn;
-              L = L * f + ml.y * g;
-              v.x = v.x * f + x.x * g;
-              v.y = v.y * f + x.y * g;
-              v.z = v.z * f + x.z * g;
-              v.w = v.w * f + x.w * g;
-            }
-            finish(r, d, v, M, L);
-          }
-        }
+      if (d == 0) {
+        const float lg = L > 0.f || L != L ? M + log2f(L) : -INFINITY;
+        if (p.lse) p.lse[at] = lg * 0.6931471805599453f;
+        if (WEIGHTS) p.lse2[((int64_t)c.b * p.kv_heads + c.h) * p.rows + row] = lg;
       }
-      __syncthreads();  // the join buffer's stage may be filled again
-      fresh = true;
+    };
+    for (int i = tid; i < nrow * (HD / 4); i += kPaThreads) {
+      const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+      const int w0 = (r / 16) * WT, rr = r % 16;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WT; ++w) M = fmaxf(M, s_m[w0 + w][rr]);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float L = 0.f;
+#pragma unroll
+      for (int w = 0; w < WT; ++w) {
+        const float f = exp2_diff(s_m[w0 + w][rr], M);
+        const float4 x = *reinterpret_cast<const float4*>(buf + ((w0 + w) * 16 + rr) * HD + (d ^ ((rr & 7) << 3)));
+        L = fmaf(s_l[w0 + w][rr], f, L);
+        v.x = fmaf(x.x, f, v.x);
+        v.y = fmaf(x.y, f, v.y);
+        v.z = fmaf(x.z, f, v.z);
+        v.w = fmaf(x.w, f, v.w);
+      }
+      if (alone) {
+        const float vv[4] = {v.x, v.y, v.z, v.w};
+        finish(r, d, vv, M, L);
+      } else {
+        *reinterpret_cast<float4*>(po + r * HD + d) = v;
+        if (d == 0) pml[r] = make_float2(M, L);
+      }
     }
+    if (!alone) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned n = static_cast<unsigned>(c1 - c0 + 1);
+        s_last = atomicAdd(&p.counters[c0], 1u) == n - 1;
+        if (s_last) p.counters[c0] = 0u;
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        // a warp per row, each lane HD / 32 neighbouring elements; 32 parts'
+        // loads in flight at a time
+        constexpr int E = HD / 32;
+        for (int r = warp; r < nrow; r += kPaWarps) {
+          float M = -INFINITY, L = 0.f, v[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[e] = 0.f;
+          for (int k0 = c0; k0 <= c1; k0 += 32) {
+            const int k = k0 + lane;
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if (k <= c1) ml = __ldcg(p.part_ml + static_cast<size_t>(k * 2 + (k == c0 ? 1 : 0)) * RT + r);
+            constexpr int U = HD == 256 ? 16 : 32;
+            float x[U][E];
+            auto fetch = [&](int i0) {
+#pragma unroll
+              for (int i = 0; i < U; ++i) {
+                const int kk = k0 + i0 + i;
+                const float* src = p.part_o + (static_cast<size_t>(min(kk, c1) * 2 + (kk == c0 ? 1 : 0)) * RT + r) * HD + lane * E;
+                if (E == 2) {
+                  const float2 t2 = kk <= c1 ? __ldcg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
+                  x[i][0] = t2.x;
+                  x[i][1 % E] = t2.y;
+                } else {
+#pragma unroll
+                  for (int e = 0; e < E / 4; ++e) {
+                    const float4 t4 = kk <= c1 ? __ldcg(reinterpret_cast<const float4*>(src) + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[i][(4 * e) % E] = t4.x;
+                    x[i][(4 * e + 1) % E] = t4.y;
+                    x[i][(4 * e + 2) % E] = t4.z;
+                    x[i][(4 * e + 3) % E] = t4.w;
+                  }
+                }
+              }
+            };
+            fetch(0);
+            float mx = ml.x;
+#pragma unroll
+            for (int o2 = 16; o2; o2 >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o2));
+            const float top = fmaxf(M, mx), f = exp2_diff(M, top), g = exp2_diff(ml.x, top);
+            float lg = ml.y == 0.f ? 0.f : ml.y * g;
+#pragma unroll
+            for (int o2 = 16; o2; o2 >>= 1) lg += __shfl_xor_sync(0xffffffffu, lg, o2);
+            M = top;
+            L = L * f + lg;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] *= f;
+#pragma unroll
+            for (int i0 = 0; i0 < 32; i0 += U) {
+              if (i0) fetch(i0);
+#pragma unroll
+              for (int i = 0; i < U; ++i) {
+                const float w = __shfl_sync(0xffffffffu, g, i0 + i);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = fmaf(x[i][e], w, v[e]);
+              }
+            }
+          }
+          finish(r, lane * E, v, M, L);
+        }
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();  // the join buffer's stage may be filled again
+    ++t;
     step_cursor<RT>(p, c);
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1u;
+    }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -675,6 +768,48 @@ tp_status plan_attn(const tp_paged_cache* c, int tokens, int q_heads, int accumu
   return TP_OK;
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder, looked up once.
+tp_status encoder(EncodeTiled* out) {
+  static void* cached;
+  void* fn = __atomic_load_n(&cached, __ATOMIC_ACQUIRE);
+  if (!fn) {
+    cudaDriverEntryPointQueryResult found;
+    TP_CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found),
+                "cuTensorMapEncodeTiled");
+    if (found != cudaDriverEntryPointSuccess || !fn) return fail(TP_ERR_CUDA, "cuTensorMapEncodeTiled: not in this driver");
+    __atomic_store_n(&cached, fn, __ATOMIC_RELEASE);
+  }
+  *out = reinterpret_cast<EncodeTiled>(fn);
+  return TP_OK;
+}
+
+// The pages as a 4-D tensor of boxes of 64 elements x min(16, page_size)
+// tokens; the smaller of the token and head strides comes first.
+tp_status page_map(const tp_paged_cache* c, void* base, bool token_major, int box, CUtensorMap* map) {
+  EncodeTiled encode;
+  const tp_status s = encoder(&encode);
+  if (s != TP_OK) return s;
+  const auto u64 = [](int64_t v) { return static_cast<cuuint64_t>(v); };
+  const cuuint64_t tok_bytes = u64(c->token_stride * 2), head_bytes = u64(c->head_stride * 2);
+  const cuuint64_t dims[4] = {u64(c->head_dim), u64(token_major ? c->kv_heads : c->page_size),
+                              u64(token_major ? c->page_size : c->kv_heads), u64(std::max<int64_t>(1, c->num_pages))};
+  const cuuint64_t strides[3] = {token_major ? head_bytes : tok_bytes, token_major ? tok_bytes : head_bytes,
+                                 u64(c->page_stride * 2)};
+  const cuuint32_t boxes[4] = {64u, token_major ? 1u : static_cast<cuuint32_t>(box),
+                               token_major ? static_cast<cuuint32_t>(box) : 1u, 1u};
+  const cuuint32_t ones[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = encode(map, c->dtype == TP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                            base, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(TP_ERR_UNSUPPORTED, "tp_paged_attn: the pages' sizes and strides make no tensor map (error %d)", (int)r);
+  return TP_OK;
+}
+
 template <class T, int HD, int MT>
 tp_status launch_attn(const AttnParams& p, const PaPlan& pl, bool weights, cudaStream_t st) {
   using S = PaShape<HD, MT>;
@@ -751,18 +886,19 @@ TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_ca
     return fail(TP_ERR_WORKSPACE, "tp_paged_attn: workspace missing, not 256-byte aligned or smaller than %lld bytes",
                 (long long)pl.bytes);
   AttnParams p{};
+  p.token_major = cache->head_stride < cache->token_stride;
+  const int box = std::min(16, cache->page_size);
+  p.lg_box = log2_int(box);
+  s = page_map(cache, cache->k_pages, p.token_major, box, &p.k_map);
+  if (s == TP_OK) s = page_map(cache, cache->v_pages, p.token_major, box, &p.v_map);
+  if (s != TP_OK) return s;
   p.q = a.q;
   p.out = a.out;
   p.lse = a.lse;
-  p.k_pages = cache->k_pages;
-  p.v_pages = cache->v_pages;
   p.block_table = cache->block_table;
   p.lengths = cache->lengths;
   p.scores = cache->scores;
   p.num_pages = cache->num_pages;
-  p.page_stride = cache->page_stride;
-  p.head_stride = cache->head_stride;
-  p.token_stride = cache->token_stride;
   p.table_stride = cache->table_stride;
   p.batch = cache->batch;
   p.tokens = a.tokens;
@@ -777,6 +913,7 @@ TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_ca
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   auto* ws = static_cast<unsigned char*>(workspace);
   p.counters = reinterpret_cast<unsigned*>(ws);
+  p.status = reinterpret_cast<unsigned*>(ws + kPaStatusOff);
   p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_off);
   p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
   p.lse2 = reinterpret_cast<float*>(ws + pl.lse_off);
@@ -785,6 +922,18 @@ TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_ca
   const bool weights = a.accumulate != 0;
   return cache->dtype == TP_F16 ? dispatch_dim<__half>(p, pl, weights, st)
                                 : dispatch_dim<__nv_bfloat16>(p, pl, weights, st);
+}
+
+TP_API tp_status tp_paged_attn_status(void* workspace, void* stream) {
+  if (!workspace) return fail(TP_ERR_ARG, "tp_paged_attn_status: null workspace");
+  auto* word = reinterpret_cast<unsigned*>(static_cast<unsigned char*>(workspace) + kPaStatusOff);
+  cudaStream_t st = as_stream(stream);
+  unsigned v = 0;
+  TP_CUDA_TRY(cudaMemcpyAsync(&v, word, 4, cudaMemcpyDeviceToHost, st), "status copy");
+  TP_CUDA_TRY(cudaStreamSynchronize(st), "status sync");
+  if (!v) return clear_ok();
+  TP_CUDA_TRY(cudaMemsetAsync(word, 0, 4, st), "status clear");
+  return fail(TP_ERR_DEVICE, "tp_paged_attn: a bounded device wait ran out, outputs are NaN (status %u)", v);
 }
 
 }  // extern "C"

@@ -45,11 +45,6 @@ struct RotaryParams {
   int lg_group;    // log2 G
 };
 
-template <class T, int VEC>
-struct alignas(VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16) Pack {
-  T v[VEC];
-};
-
 // Positions the unit's two vectors start at.
 template <int VEC>
 __device__ __forceinline__ void unit_at(const RotaryParams& p, int u, int& lo, int& hi) {

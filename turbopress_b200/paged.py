@@ -218,6 +218,11 @@ class PagedKVCache:
             self._outgrown.append(ws)
         return torch.zeros(need, dtype=torch.uint8, device=self.device)
 
+    def status(self) -> None:
+        """Raise if a device-side wait of an ``attend`` gave up (synchronizes)."""
+        if self._ws is not None:
+            _abi.launch(_abi.lib().tp_paged_attn_status, "attend", self.device.index, self._ws.data_ptr())
+
     # -- a bounded cache --------------------------------------------------------
     def evict_slots(self, budget: int, *, recent: int = 0, sinks: int = 0, layer: int = 0) -> tuple[Tensor, Tensor, Tensor]:
         """Keep ``budget`` slots of each sequence that has more, per kv head:
