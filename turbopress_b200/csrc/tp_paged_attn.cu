@@ -14,7 +14,8 @@
 // their operands come straight from the shared-memory tiles.
 //
 // Split: the 64-token tiles of all (sequence, row tile, kv head) items form
-// one index space, cut into equal runs, one per resident CTA; lengths are read
+// one index space (an item's tiles follow kItemCost positions that stand for
+// its fixed cost), cut into equal runs, one per resident CTA; lengths are read
 // on the device, so ragged batches balance by themselves.  A run that ends
 // inside an item leaves (m, l, o) in the workspace and the item's last CTA to
 // arrive (a counter at the item's first CTA) joins them in run order, so the
@@ -42,6 +43,10 @@ namespace {
 constexpr int kPaThreads = 128;
 constexpr int kPaWarps = 4;
 constexpr int kPaTile = 64;
+// An item costs about two tiles beside its own (its queries, the join of the
+// warps), so the split counts it as that many tiles more: sequences of many
+// lengths 119 -> KRAG us (64 of 100 to 8000 tokens), against equal tile counts.
+constexpr int kItemCost = 2;
 constexpr int kPaMaxCtas = 512;
 constexpr int kPaStatusOff = kPaMaxCtas * 4;      // status word after the counters
 constexpr int kPaCounterBytes = kPaStatusOff + 256;
@@ -67,7 +72,7 @@ struct AttnParams {
   float* part_o;   // [ctas][2][16*MT][HD]
   float2* part_ml; // [ctas][2][16*MT]
   float* lse2;     // [batch][kv_heads][rows] log2 units (accumulate only)
-  float* sbuf;     // [tiles][16*MT][64] scores in log2 units (accumulate only)
+  float* sbuf;     // [index space][16*MT][64] scores in log2 units (accumulate only)
 };
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
@@ -145,10 +150,11 @@ __device__ __forceinline__ int item_tiles(const AttnParams& p, int len, int rt) 
   const int vis = visible(p, len, min(p.rows, (rt + 1) * RT) - 1);
   return max(1, (vis + kPaTile - 1) / kPaTile);
 }
+// Positions of a sequence's items.
 template <int RT>
-__device__ __forceinline__ int seq_tiles(const AttnParams& p, int len) {
+__device__ __forceinline__ int seq_size(const AttnParams& p, int len) {
   int n = 0;
-  for (int rt = 0; rt < p.row_tiles; ++rt) n += item_tiles<RT>(p, len, rt);
+  for (int rt = 0; rt < p.row_tiles; ++rt) n += kItemCost + item_tiles<RT>(p, len, rt);
   return n * p.kv_heads;
 }
 
@@ -170,8 +176,7 @@ __device__ __forceinline__ void step_cursor(const AttnParams& p, Cursor& c) {
   c.h = 0;
   if (++c.rt == p.row_tiles) {
     c.rt = 0;
-    if (++c.b == p.batch) return;  // past the end: the caller does not use it
-    c.len = p.lengths[c.b];
+    c.len = p.lengths[++c.b];
   }
   set_item<RT>(p, c);
 }
@@ -189,42 +194,59 @@ __device__ __forceinline__ int block_sum(int v, int* s_tmp) {
   return t;
 }
 
-// The sequence holding position `t0` of the concatenation of `count(len)`
-// positions per sequence, and the positions before it.
+// This CTA's equal share [t0, t1) of the concatenation of `count(len)`
+// positions per sequence, `per` positions each; the sequence holding t0, its
+// length and the positions before it.  False (in every thread) where the share
+// is empty.
 template <class F>
-__device__ __forceinline__ void find_sequence(const AttnParams& p, int t0, F count, int* s_tmp, int& b_out, int& before) {
+__device__ __forceinline__ bool find_share(const AttnParams& p, F count, int* s_tmp, int& per, int& t0, int& t1, int& b_out,
+                                           int& len_out, int& before) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int len = threadIdx.x < p.batch ? p.lengths[threadIdx.x] : 0;
+  int own = threadIdx.x < p.batch ? count(len) : 0;
+  int sum = own;
+  for (int b = threadIdx.x + kPaThreads; b < p.batch; b += kPaThreads) sum += count(p.lengths[b]);
+  const int total = block_sum(sum, s_tmp);
+  per = (total + gridDim.x - 1) / gridDim.x;
+  t0 = min((int)blockIdx.x * per, total);
+  t1 = min(t0 + per, total);
+  if (t0 >= t1) return false;
   int run = 0;
   for (int base = 0;; base += kPaThreads) {
-    const int b = base + threadIdx.x;
-    const int own = b < p.batch ? count(p.lengths[b]) : 0;
+    if (base) {
+      const int b = base + threadIdx.x;
+      len = b < p.batch ? p.lengths[b] : 0;
+      own = b < p.batch ? count(len) : 0;
+    }
     int inc = own;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
       const int o = __shfl_up_sync(0xffffffffu, inc, m);
-      if ((threadIdx.x & 31) >= m) inc += o;
+      if (lane >= m) inc += o;
     }
     __syncthreads();
-    if ((threadIdx.x & 31) == 31) s_tmp[threadIdx.x >> 5] = inc;
+    if (lane == 31) s_tmp[warp] = inc;
     if (threadIdx.x == 0) s_tmp[4] = -1;
     __syncthreads();
-    int sum = 0;
+    int part = 0;
 #pragma unroll
     for (int w = 0; w < kPaWarps; ++w) {
-      if (w < (int)(threadIdx.x >> 5)) inc += s_tmp[w];
-      sum += s_tmp[w];
+      if (w < warp) inc += s_tmp[w];
+      part += s_tmp[w];
     }
     if (own > 0 && run + inc - own <= t0 && t0 < run + inc) {
-      s_tmp[4] = b;
+      s_tmp[4] = base + threadIdx.x;
       s_tmp[5] = run + inc - own;
+      s_tmp[6] = len;
     }
     __syncthreads();
-    if (s_tmp[4] >= 0 || base + kPaThreads >= p.batch) {
-      b_out = s_tmp[4];
-      before = s_tmp[5];
-      return;
-    }
-    run += sum;
+    if (s_tmp[4] >= 0 || base + kPaThreads >= p.batch) break;
+    run += part;
   }
+  b_out = s_tmp[4];
+  before = s_tmp[5];
+  len_out = s_tmp[6];
+  return true;
 }
 
 // ---------------------------------------------------------------------------
@@ -239,13 +261,14 @@ struct PaShape {
   static constexpr int kBlock = 16 * HD * 2;         // K (or V) of a block: [panel][16][128 bytes], swizzled
   static constexpr int kKV = (kPaTile / 16) * kBlock;
   static constexpr int kQ = RT * HD * 2;
-  static constexpr int kStage = 2 * kKV + kQ;
-  // three tiles per CTA, two where three with the queries pass 227 KB
-  static constexpr int kStages = HD == 256 && MT > 1 ? 2 : 3;
-  static constexpr int kSmem = kStages * kStage;
+  static constexpr int kStage = 2 * kKV;
+  // three tiles per CTA; two where three would leave one CTA per SM at
+  // head_dim 128, or none at 256
+  static constexpr int kStages = (HD == 128 && MT == 4) || (HD == 256 && MT > 1) ? 2 : 3;
+  static constexpr int kSmem = kStages * kStage + 2 * kQ;  // queries of the next two items
   static_assert(kSmem <= 227 * 1024 - 1024, "shared memory");
   static_assert(kStage % 1024 == 0, "the swizzle repeats every 1024 bytes");
-  static_assert(kPaWarps * 16 * HD * 4 <= 2 * kKV, "the join buffer reuses a consumed stage");
+  static_assert(kPaWarps * 16 * HD * 4 == kStage, "the join buffer reuses a consumed stage");
 };
 
 template <class T, int HD, int MT, bool WEIGHTS>
@@ -265,26 +288,25 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     fence_mbar_init();
   }
 
-  // ---- this CTA's run of tiles ----
-  int cnt = 0;
-  for (int b = tid; b < p.batch; b += kPaThreads) cnt += seq_tiles<RT>(p, p.lengths[b]);
-  const int total = block_sum(cnt, s_tmp);  // (its barriers also publish the mbarriers)
-  const int per = (total + gridDim.x - 1) / gridDim.x;
-  const int t0 = min((int)blockIdx.x * per, total), t1 = min(t0 + per, total);
-  if (WEIGHTS) pdl_trigger();
-  if (t0 >= t1) return;
+  // ---- this CTA's run [t0, t1) of the index space ----
+  int per, t0, t1, before;
   Cursor c;
-  int before;
-  find_sequence(p, t0, [&](int len) { return seq_tiles<RT>(p, len); }, s_tmp, c.b, before);
-  c.len = p.lengths[c.b];
+  if (WEIGHTS) pdl_trigger();
+  // (its barriers also publish the mbarriers)
+  if (!find_share(p, [&](int len) { return seq_size<RT>(p, len); }, s_tmp, per, t0, t1, c.b, c.len, before)) return;
   int rem = t0 - before;
   for (c.rt = 0;; ++c.rt) {
     set_item<RT>(p, c);
-    if (rem < p.kv_heads * c.n) break;
-    rem -= p.kv_heads * c.n;
+    if (rem < p.kv_heads * (kItemCost + c.n)) break;
+    rem -= p.kv_heads * (kItemCost + c.n);
   }
-  c.h = rem / c.n;
-  c.tile = rem - c.h * c.n;
+  c.h = rem / (kItemCost + c.n);
+  c.tile = rem - c.h * (kItemCost + c.n) - kItemCost;
+  if (c.tile < 0) {  // the run begins in the item's fixed part
+    t0 -= c.tile;
+    c.tile = 0;
+  }
+  if (t0 >= t1) return;
   Cursor ld = c;
 
   // ---- loads: lane i < boxes of a warp fetches box i of the warp's block ----
@@ -295,8 +317,9 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     return lane < boxes && tok < p.capacity ? p.block_table[u.b * p.table_stride + (tok >> p.lg_page)] : -1;
   };
   int pid = page_of(ld);
-  int ld_stage = 0;
-  auto issue = [&](bool first, bool more) {  // the tile at cursor ld, into stage ld_stage
+  int ld_stage = 0, ld_item = 0, t_ld = t0;
+  auto issue = [&](bool first) {  // the tile at cursor ld (position t_ld), into stage ld_stage
+    if (t_ld >= t1) return;
     const uint32_t st = sbase + ld_stage * S::kStage;
     const int tok = ld.tile * kPaTile + warp * 16 + (lane << p.lg_box);
     const bool ok = lane < boxes && tok < ld.hi && pid >= 0 && pid < p.num_pages;
@@ -329,22 +352,25 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
         const int64_t o = on ? (((int64_t)ld.b * p.tokens + j) * p.q_heads + ld.h * p.group + row - j * p.group) *
                                        p.head_dim + chunk * 8
                              : 0;
-        cp_async16_zfill(st + 2 * S::kKV + r * (HD * 2) + ((chunk ^ (r & 7)) << 4), q + o, on);
+        cp_async16_zfill(sbase + kStages * S::kStage + ld_item * S::kQ + r * (HD * 2) + ((chunk ^ (r & 7)) << 4), q + o, on);
       }
+      ld_item ^= 1;
     }
     ld_stage = ld_stage + 1 == kStages ? 0 : ld_stage + 1;
-    step_cursor<RT>(p, ld);
-    if (more) pid = page_of(ld);
+    t_ld += ld.tile + 1 == ld.n ? 1 + kItemCost : 1;
+    if (t_ld < t1) {
+      step_cursor<RT>(p, ld);
+      pid = page_of(ld);
+    }
   };
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i)
-    if (t0 + i < t1) issue(i == 0, t0 + i + 1 < t1);
+  for (int i = 0; i < kStages - 1; ++i) issue(i == 0);
 
   // ---- state of this warp's 16 rows ----
   const int mt = warp / WT, tw = warp % WT;
   const int r0 = lane >> 2, cq = lane & 3;  // this thread: rows r0, r0 + 8, columns 2 cq + {0, 1} of each 8
   bool dead = false;
-  int stage = 0, t = t0;
+  int stage = 0, item = 0, t = t0;
   unsigned phase = 0;
 
   while (t < t1) {  // an item, or this run's part of it
@@ -354,8 +380,9 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) {
       const int r = mt * 16 + (lane & 15), chunk = ks * 2 + (lane >> 4);
-      ldsm4(qf[ks], sbase + stage * S::kStage + 2 * S::kKV + r * (HD * 2) + ((chunk ^ (r & 7)) << 4));
+      ldsm4(qf[ks], sbase + kStages * S::kStage + item * S::kQ + r * (HD * 2) + ((chunk ^ (r & 7)) << 4));
     }
+    item ^= 1;
     float o[HD / 8][4];
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -369,21 +396,36 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       vis[e] = row < p.rows ? visible(p, c.len, row) : 0;
     }
     const int j_lo = row0 / p.group, j_hi = last_row / p.group;  // j_hi < j_lo where these 16 rows are empty
-    const int vis_lo = last_row >= row0 ? visible(p, c.len, row0) : 0;
+    const int vis_lo = last_row >= row0 ? visible(p, c.len, row0) : 0;  // slots seen by every row,
+    const int vis_hi = last_row >= row0 ? visible(p, c.len, last_row) : 0;  // and by any
     const int t_end = min(t1, t + c.n - c.tile);
+    // the rows' scores of a block, in log2 units, for the accumulated weights
+    auto store_scores = [&](int blk, const float (*s)[4]) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (row0 + r0 + 8 * e < p.rows)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            *reinterpret_cast<float2*>(p.sbuf + ((size_t)t * RT + mt * 16 + r0 + 8 * e) * kPaTile + blk * 16 + n * 8 + cq * 2) =
+                s ? make_float2(s[n][2 * e], s[n][2 * e + 1]) : make_float2(-INFINITY, -INFINITY);
+    };
 
     for (bool head = true;; head = false) {
       // Every warp has its queries, and is done with the stage that is filled
       // next (last read in the round before; at MT = 1 by this warp alone).
       if (MT > 1 || head) __syncthreads();
       else __syncwarp();
-      if (t + kStages - 1 < t1) issue(false, t + kStages < t1);
+      issue(false);
       const uint32_t st = sbase + stage * S::kStage;
 
       // blocks of 16 tokens: one per warp at MT = 1, MT of them otherwise
 #pragma unroll 1
       for (int blk = tw * MT; blk < (tw + 1) * MT; ++blk) {
         const int tok0 = c.tile * kPaTile + blk * 16;
+        if (tok0 >= vis_hi) {  // nothing here for these rows (what was fetched is waited for by the rows that see it)
+          if (WEIGHTS) store_scores(blk, nullptr);
+          continue;
+        }
         if (!dead && !mbar_wait(&s_full[stage][blk], phase)) {
           dead = true;  // reported through the status word; the outputs become NaN
           atomicOr(p.status, 1u);
@@ -417,15 +459,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
               if (!((valid >> col) & 1u) || tok0 + col >= vis[e >> 1]) s[n][e] = -INFINITY;
             }
         }
-        if (WEIGHTS) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (c.rt * RT + mt * 16 + r0 + 8 * e < p.rows)
-#pragma unroll
-              for (int n = 0; n < 2; ++n)
-                *reinterpret_cast<float2*>(p.sbuf + ((size_t)t * RT + mt * 16 + r0 + 8 * e) * kPaTile + blk * 16 + n * 8 +
-                                           cq * 2) = make_float2(s[n][2 * e], s[n][2 * e + 1]);
-        }
+        if (WEIGHTS) store_scores(blk, s);
         // running maximum: the quad of four lanes shares a row
         float mn[2];
 #pragma unroll
@@ -480,26 +514,22 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
           // Some slots are not seen by some rows, and 0 * (what they hold) may be
           // NaN: each step token's product takes V with the slots it does not see
           // zeroed, and only its own rows of the result.
-#pragma unroll
-          for (int nn = 0; nn < HD / 16; ++nn) {
-            uint32_t vf[4];
-            const int r = lane & 15, chunk = nn * 2 + (lane >> 4);
-            ldsm4t(vf, vb + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
 #pragma unroll 1
-            for (int j = j_lo; j <= j_hi; ++j) {
-              const int see = visible(p, c.len, j * p.group) - tok0;  // slots of this block
-              const uint32_t seen = see >= 16 ? valid : see <= 0 ? 0u : valid & ((1u << see) - 1u);
-              uint32_t w[4];
+          for (int j = j_lo; j <= j_hi; ++j) {
+            const int see = visible(p, c.len, j * p.group) - tok0;  // slots of this block
+            const uint32_t seen = (see >= 16 ? valid : see <= 0 ? 0u : valid & ((1u << see) - 1u)) >> (cq * 2);
+            const uint32_t k0 = (seen & 1u ? 0x0000ffffu : 0u) | (seen & 2u ? 0xffff0000u : 0u);
+            const uint32_t k1 = (seen & 0x100u ? 0x0000ffffu : 0u) | (seen & 0x200u ? 0xffff0000u : 0u);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int k = cq * 2 + 8 * (e & 1);
-                w[e] = vf[e] & (((seen >> k) & 1u ? 0x0000ffffu : 0u) | ((seen >> (k + 1)) & 1u ? 0xffff0000u : 0u));
-              }
+            for (int nn = 0; nn < HD / 16; ++nn) {
+              uint32_t vf[4];
+              const int r = lane & 15, chunk = nn * 2 + (lane >> 4);
+              ldsm4t(vf, vb + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
               float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-              Mma<T>::run(x, ph, w[0], w[1]);
-              Mma<T>::run(y, ph, w[2], w[3]);
-              Mma<T>::run(x, pl, w[0], w[1]);
-              Mma<T>::run(y, pl, w[2], w[3]);
+              Mma<T>::run(x, ph, vf[0] & k0, vf[1] & k1);
+              Mma<T>::run(y, ph, vf[2] & k0, vf[3] & k1);
+              Mma<T>::run(x, pl, vf[0] & k0, vf[1] & k1);
+              Mma<T>::run(y, pl, vf[2] & k0, vf[3] & k1);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (jr[e >> 1] == j) {
@@ -593,71 +623,70 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       }
     }
     if (!alone) {
-      __threadfence();
       __syncthreads();
-      if (tid == 0) {
-        const unsigned n = static_cast<unsigned>(c1 - c0 + 1);
-        s_last = atomicAdd(&p.counters[c0], 1u) == n - 1;
+      if (tid == 0) {  // one acq_rel add publishes this part and orders the last arriver's reads
+        unsigned n;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(p.counters + c0) : "memory");
+        s_last = n == static_cast<unsigned>(c1 - c0);
         if (s_last) p.counters[c0] = 0u;
       }
       __syncthreads();
       if (s_last) {
-        __threadfence();
-        // a warp per row, each lane HD / 32 neighbouring elements; 32 parts'
-        // loads in flight at a time
+        // a warp per row, each lane HD / 32 neighbouring elements
         constexpr int E = HD / 32;
         for (int r = warp; r < nrow; r += kPaWarps) {
           float M = -INFINITY, L = 0.f, v[E];
 #pragma unroll
           for (int e = 0; e < E; ++e) v[e] = 0.f;
-          for (int k0 = c0; k0 <= c1; k0 += 32) {
-            const int k = k0 + lane;
-            float2 ml = make_float2(-INFINITY, 0.f);
-            if (k <= c1) ml = __ldcg(p.part_ml + static_cast<size_t>(k * 2 + (k == c0 ? 1 : 0)) * RT + r);
-            constexpr int U = HD == 256 ? 16 : 32;
+          constexpr int U = HD == 256 ? 16 : 40;  // parts whose loads are in flight together
+          for (int k0 = c0; k0 <= c1; k0 += U) {
+            auto part = [&](int k) { return static_cast<size_t>(min(k, c1) * 2 + (k == c0 ? 1 : 0)) * RT + r; };
+            float2 ml[2];
             float x[U][E];
-            auto fetch = [&](int i0) {
 #pragma unroll
-              for (int i = 0; i < U; ++i) {
-                const int kk = k0 + i0 + i;
-                const float* src = p.part_o + (static_cast<size_t>(min(kk, c1) * 2 + (kk == c0 ? 1 : 0)) * RT + r) * HD + lane * E;
-                if (E == 2) {
-                  const float2 t2 = kk <= c1 ? __ldcg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
-                  x[i][0] = t2.x;
-                  x[i][1 % E] = t2.y;
+            for (int w = 0; w < 2; ++w) {
+              const int i = 32 * w + lane;
+              ml[w] = i < U && k0 + i <= c1 ? __ldcg(p.part_ml + part(k0 + i)) : make_float2(-INFINITY, 0.f);
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+#pragma unroll
+              for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+              if (k0 + i <= c1) {
+                const float* src = p.part_o + part(k0 + i) * HD + lane * E;
+                if constexpr (E == 2) {
+                  const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+                  x[i][0] = y.x;
+                  x[i][1] = y.y;
                 } else {
 #pragma unroll
-                  for (int e = 0; e < E / 4; ++e) {
-                    const float4 t4 = kk <= c1 ? __ldcg(reinterpret_cast<const float4*>(src) + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    x[i][(4 * e) % E] = t4.x;
-                    x[i][(4 * e + 1) % E] = t4.y;
-                    x[i][(4 * e + 2) % E] = t4.z;
-                    x[i][(4 * e + 3) % E] = t4.w;
+                  for (int e = 0; e < E; e += 4) {
+                    const float4 y = __ldcg(reinterpret_cast<const float4*>(src + e));
+                    x[i][e] = y.x;
+                    x[i][e + 1] = y.y;
+                    x[i][e + 2] = y.z;
+                    x[i][e + 3] = y.w;
                   }
                 }
               }
-            };
-            fetch(0);
-            float mx = ml.x;
+            }
+            float top = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
-            for (int o2 = 16; o2; o2 >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o2));
-            const float top = fmaxf(M, mx), f = exp2_diff(M, top), g = exp2_diff(ml.x, top);
-            float lg = ml.y == 0.f ? 0.f : ml.y * g;
+            for (int q = 16; q; q >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, q));
+            top = fmaxf(top, M);
+            const float f = exp2_diff(M, top), g[2] = {exp2_diff(ml[0].x, top), exp2_diff(ml[1].x, top)};
+            float lg = (ml[0].y == 0.f ? 0.f : ml[0].y * g[0]) + (ml[1].y == 0.f ? 0.f : ml[1].y * g[1]);
 #pragma unroll
-            for (int o2 = 16; o2; o2 >>= 1) lg += __shfl_xor_sync(0xffffffffu, lg, o2);
+            for (int q = 16; q; q >>= 1) lg += __shfl_xor_sync(0xffffffffu, lg, q);
             M = top;
             L = L * f + lg;
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] *= f;
 #pragma unroll
-            for (int i0 = 0; i0 < 32; i0 += U) {
-              if (i0) fetch(i0);
+            for (int i = 0; i < U; ++i) {
+              const float w = __shfl_sync(0xffffffffu, g[i / 32], i % 32);
 #pragma unroll
-              for (int i = 0; i < U; ++i) {
-                const float w = __shfl_sync(0xffffffffu, g, i0 + i);
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = fmaf(x[i][e], w, v[e]);
-              }
+              for (int e = 0; e < E; ++e) v[e] = fmaf(x[i][e], w, v[e]);
             }
           }
           finish(r, lane * E, v, M, L);
@@ -666,8 +695,8 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();  // the join buffer's stage may be filled again
-    ++t;
-    step_cursor<RT>(p, c);
+    t += c.tile + 1 == c.n ? 1 + kItemCost : 1;
+    if (t < t1) step_cursor<RT>(p, c);
     if (++stage == kStages) {
       stage = 0;
       phase ^= 1u;
@@ -686,24 +715,18 @@ __global__ void __launch_bounds__(kPaThreads) paged_weights_kernel(const __grid_
   pdl_wait();
   const int last = p.row_tiles - 1;
   auto count = [&](int len) { return p.kv_heads * item_tiles<RT>(p, len, last); };
-  int cnt = 0;
-  for (int b = threadIdx.x; b < p.batch; b += kPaThreads) cnt += count(p.lengths[b]);
-  const int total = block_sum(cnt, s_tmp);
-  const int per = (total + gridDim.x - 1) / gridDim.x;
-  const int t0 = min((int)blockIdx.x * per, total), t1 = min(t0 + per, total);
-  if (t0 >= t1) return;
-  int b, before;
-  find_sequence(p, t0, count, s_tmp, b, before);
-  // tiles of the attention kernel's index space before sequence b
+  int per, t0, t1, b, len, before;
+  if (!find_share(p, count, s_tmp, per, t0, t1, b, len, before)) return;
+  // positions of the attention kernel's index space before sequence b
   int c1 = 0;
-  for (int i = threadIdx.x; i < b; i += kPaThreads) c1 += seq_tiles<RT>(p, p.lengths[i]);
+  for (int i = threadIdx.x; i < b; i += kPaThreads) c1 += seq_size<RT>(p, p.lengths[i]);
   int base = block_sum(c1, s_tmp);
-  int len = p.lengths[b], n = item_tiles<RT>(p, len, last);
+  int n = item_tiles<RT>(p, len, last);
   const int half = threadIdx.x >> 6, tok = threadIdx.x & 63;  // two tiles at a time
   for (int t = t0 + half; t < t1; t += 2) {
     while (t - before >= p.kv_heads * n) {
       before += p.kv_heads * n;
-      base += seq_tiles<RT>(p, len);
+      base += seq_size<RT>(p, len);
       len = p.lengths[++b];
       n = item_tiles<RT>(p, len, last);
     }
@@ -715,13 +738,13 @@ __global__ void __launch_bounds__(kPaThreads) paged_weights_kernel(const __grid_
     for (int rt = 0; rt <= last; ++rt) {
       const int nt = item_tiles<RT>(p, len, rt);
       if (tile < nt) {
-        const float* s = p.sbuf + (size_t)(off + h * nt + tile) * RT * kPaTile + tok;
+        const float* s = p.sbuf + (size_t)(off + h * (kItemCost + nt) + kItemCost + tile) * RT * kPaTile + tok;
         const float* z = p.lse2 + ((int64_t)b * p.kv_heads + h) * p.rows + rt * RT;
         const int rows = min(RT, p.rows - rt * RT);
 #pragma unroll 4
         for (int r = 0; r < rows; ++r) w += exp2_diff(s[r * kPaTile], z[r]);
       }
-      off += p.kv_heads * nt;
+      off += p.kv_heads * (kItemCost + nt);
     }
     p.scores[((int64_t)b * p.kv_heads + h) * p.capacity + slot] += w;
   }
@@ -732,7 +755,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_weights_kernel(const __grid_
 // ---------------------------------------------------------------------------
 struct PaPlan {
   int hd, mt;
-  int64_t max_tiles, ml_off, o_off, lse_off, s_off, bytes;
+  int64_t max_tiles, positions, ml_off, o_off, lse_off, s_off, bytes;
 };
 
 // Sizes of the call's index space and workspace (no device work).
@@ -749,7 +772,8 @@ tp_status plan_attn(const tp_paged_cache* c, int tokens, int q_heads, int accumu
   const int64_t cap = (int64_t)c->max_pages * c->page_size;
   const int64_t items = (int64_t)c->batch * c->kv_heads * row_tiles;
   pl.max_tiles = items * std::max<int64_t>(1, (cap + kPaTile - 1) / kPaTile);
-  if (rows > (1 << 24) || items > (1 << 30) || pl.max_tiles > (int64_t(1) << 30))
+  pl.positions = pl.max_tiles + items * kItemCost;
+  if (rows > (1 << 24) || items > (1 << 30) || pl.positions > (int64_t(1) << 30))
     return fail(TP_ERR_UNSUPPORTED, "tp_paged_attn: too many rows, sequences or slots");
   int64_t at = kPaCounterBytes;
   auto take = [&](int64_t bytes) {
@@ -761,7 +785,7 @@ tp_status plan_attn(const tp_paged_cache* c, int tokens, int q_heads, int accumu
   pl.o_off = take((int64_t)kPaMaxCtas * 2 * rt * pl.hd * 4);
   if (accumulate) {
     pl.lse_off = take((int64_t)c->batch * c->kv_heads * rows * 4);
-    pl.s_off = take(pl.max_tiles * rt * kPaTile * 4);
+    pl.s_off = take(pl.positions * rt * kPaTile * 4);
   }
   pl.bytes = at;
   *out = pl;
@@ -828,7 +852,7 @@ tp_status launch_attn(const AttnParams& p, const PaPlan& pl, bool weights, cudaS
     if (occ < 1) return fail(TP_ERR_CUDA, "paged_attn: the kernel does not fit this device");
     __atomic_store_n(&ctas[weights][dev], occ, __ATOMIC_RELAXED);
   }
-  const int grid = static_cast<int>(std::min<int64_t>(std::min(kPaMaxCtas, sms * occ), pl.max_tiles));
+  const int grid = static_cast<int>(std::min<int64_t>(std::min(kPaMaxCtas, sms * occ), pl.positions));
   kern<<<grid, kPaThreads, S::kSmem, st>>>(p);
   s = check_launch("paged_attn launch");
   if (s != TP_OK || !weights) return s;
