@@ -32,6 +32,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "tp_decode.cuh"
 #include "tp_paged.cuh"
@@ -40,14 +41,12 @@ using namespace tp;
 
 namespace {
 
-constexpr int kPaThreads = 128;
-constexpr int kPaWarps = 4;
-constexpr int kPaTile = 64;
 // An item costs about two tiles beside its own (its queries, the join of the
 // warps), so the split counts it as that many tiles more: sequences of many
 // lengths 119 -> KRAG us (64 of 100 to 8000 tokens), against equal tile counts.
 constexpr int kItemCost = 2;
 constexpr int kPaMaxCtas = 512;
+constexpr int kWtThreads = 128;
 constexpr int kPaStatusOff = kPaMaxCtas * 4;      // status word after the counters
 constexpr int kPaCounterBytes = kPaStatusOff + 256;
 
@@ -64,6 +63,7 @@ struct AttnParams {
   int lg_box;       // log2 of the tokens per box: min(16, page_size)
   int batch, tokens, q_heads, kv_heads, group, head_dim;
   int lg_page, capacity;
+  uint64_t group_inv;  // ceil(2^64 / group), 0 for a group of 1
   int rows;      // tokens * group: query rows of a kv head
   int row_tiles;
   float scale_log2;
@@ -72,7 +72,7 @@ struct AttnParams {
   float* part_o;   // [ctas][2][16*MT][HD]
   float2* part_ml; // [ctas][2][16*MT]
   float* lse2;     // [batch][kv_heads][rows] log2 units (accumulate only)
-  float* sbuf;     // [index space][16*MT][64] scores in log2 units (accumulate only)
+  float* sbuf;     // [index space][16*MT][TILE] scores in log2 units (accumulate only)
 };
 
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
@@ -103,6 +103,11 @@ template <class T>
 struct Mma;
 template <>
 struct Mma<__half> {
+  // either half infinite or NaN: its exponent is all ones
+  static __device__ __forceinline__ bool not_finite(uint32_t v) {
+    constexpr uint32_t E = 0x7c007c00u;
+    return (v & E & 0xffffu) == (E & 0xffffu) || (v & E & 0xffff0000u) == (E & 0xffff0000u);
+  }
   static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -119,6 +124,11 @@ struct Mma<__half> {
 };
 template <>
 struct Mma<__nv_bfloat16> {
+  // either half infinite or NaN: its exponent is all ones
+  static __device__ __forceinline__ bool not_finite(uint32_t v) {
+    constexpr uint32_t E = 0x7f807f80u;
+    return (v & E & 0xffffu) == (E & 0xffffu) || (v & E & 0xffff0000u) == (E & 0xffff0000u);
+  }
   static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -140,21 +150,25 @@ __device__ __forceinline__ float exp2_diff(float a, float b) { return a == -INFI
 // ---------------------------------------------------------------------------
 // the index space of tiles
 // ---------------------------------------------------------------------------
+// Step token of query row `row`.
+__device__ __forceinline__ int token_of(const AttnParams& p, int row) {
+  return p.group_inv ? static_cast<int>(__umul64hi(static_cast<uint64_t>(row), p.group_inv)) : row;
+}
 // Slots that query row `row` of sequence length `len` (before the step) sees.
 __device__ __forceinline__ int visible(const AttnParams& p, int len, int row) {
-  return len < 0 ? 0 : static_cast<int>(min((int64_t)len + row / p.group + 1, (int64_t)p.capacity));
+  return len < 0 ? 0 : static_cast<int>(min((int64_t)len + token_of(p, row) + 1, (int64_t)p.capacity));
 }
 // Tiles of an item: one at least, so that every output row is written.
-template <int RT>
+template <class S>
 __device__ __forceinline__ int item_tiles(const AttnParams& p, int len, int rt) {
-  const int vis = visible(p, len, min(p.rows, (rt + 1) * RT) - 1);
-  return max(1, (vis + kPaTile - 1) / kPaTile);
+  const int vis = visible(p, len, min(p.rows, (rt + 1) * S::RT) - 1);
+  return max(1, (vis + S::TILE - 1) / S::TILE);
 }
 // Positions of a sequence's items.
-template <int RT>
+template <class S>
 __device__ __forceinline__ int seq_size(const AttnParams& p, int len) {
   int n = 0;
-  for (int rt = 0; rt < p.row_tiles; ++rt) n += kItemCost + item_tiles<RT>(p, len, rt);
+  for (int rt = 0; rt < p.row_tiles; ++rt) n += kItemCost + item_tiles<S>(p, len, rt);
   return n * p.kv_heads;
 }
 
@@ -162,13 +176,13 @@ struct Cursor {  // one tile: sequence, row tile, kv head, tile of the item, the
   int b, rt, h, tile, n, hi, len;
 };
 
-template <int RT>
+template <class S>
 __device__ __forceinline__ void set_item(const AttnParams& p, Cursor& c) {
-  c.hi = visible(p, c.len, min(p.rows, (c.rt + 1) * RT) - 1);
-  c.n = max(1, (c.hi + kPaTile - 1) / kPaTile);
+  c.hi = visible(p, c.len, min(p.rows, (c.rt + 1) * S::RT) - 1);
+  c.n = max(1, (c.hi + S::TILE - 1) / S::TILE);
 }
 
-template <int RT>
+template <class S>
 __device__ __forceinline__ void step_cursor(const AttnParams& p, Cursor& c) {
   if (++c.tile < c.n) return;
   c.tile = 0;
@@ -178,10 +192,11 @@ __device__ __forceinline__ void step_cursor(const AttnParams& p, Cursor& c) {
     c.rt = 0;
     c.len = p.lengths[++c.b];
   }
-  set_item<RT>(p, c);
+  set_item<S>(p, c);
 }
 
-// Sum over the block of one value per thread (all threads call it).
+// Sum over a block of W warps of one value per thread (all threads call it).
+template <int W>
 __device__ __forceinline__ int block_sum(int v, int* s_tmp) {
 #pragma unroll
   for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
@@ -190,7 +205,7 @@ __device__ __forceinline__ int block_sum(int v, int* s_tmp) {
   __syncthreads();
   int t = 0;
 #pragma unroll
-  for (int w = 0; w < kPaWarps; ++w) t += s_tmp[w];
+  for (int w = 0; w < W; ++w) t += s_tmp[w];
   return t;
 }
 
@@ -198,21 +213,21 @@ __device__ __forceinline__ int block_sum(int v, int* s_tmp) {
 // positions per sequence, `per` positions each; the sequence holding t0, its
 // length and the positions before it.  False (in every thread) where the share
 // is empty.
-template <class F>
+template <int W, class F>
 __device__ __forceinline__ bool find_share(const AttnParams& p, F count, int* s_tmp, int& per, int& t0, int& t1, int& b_out,
                                            int& len_out, int& before) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int len = threadIdx.x < p.batch ? p.lengths[threadIdx.x] : 0;
   int own = threadIdx.x < p.batch ? count(len) : 0;
   int sum = own;
-  for (int b = threadIdx.x + kPaThreads; b < p.batch; b += kPaThreads) sum += count(p.lengths[b]);
-  const int total = block_sum(sum, s_tmp);
+  for (int b = threadIdx.x + 32 * W; b < p.batch; b += 32 * W) sum += count(p.lengths[b]);
+  const int total = block_sum<W>(sum, s_tmp);
   per = (total + gridDim.x - 1) / gridDim.x;
   t0 = min((int)blockIdx.x * per, total);
   t1 = min(t0 + per, total);
   if (t0 >= t1) return false;
   int run = 0;
-  for (int base = 0;; base += kPaThreads) {
+  for (int base = 0;; base += 32 * W) {
     if (base) {
       const int b = base + threadIdx.x;
       len = b < p.batch ? p.lengths[b] : 0;
@@ -226,26 +241,26 @@ __device__ __forceinline__ bool find_share(const AttnParams& p, F count, int* s_
     }
     __syncthreads();
     if (lane == 31) s_tmp[warp] = inc;
-    if (threadIdx.x == 0) s_tmp[4] = -1;
+    if (threadIdx.x == 0) s_tmp[W] = -1;
     __syncthreads();
     int part = 0;
 #pragma unroll
-    for (int w = 0; w < kPaWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       if (w < warp) inc += s_tmp[w];
       part += s_tmp[w];
     }
     if (own > 0 && run + inc - own <= t0 && t0 < run + inc) {
-      s_tmp[4] = base + threadIdx.x;
-      s_tmp[5] = run + inc - own;
-      s_tmp[6] = len;
+      s_tmp[W] = base + threadIdx.x;
+      s_tmp[W + 1] = run + inc - own;
+      s_tmp[W + 2] = len;
     }
     __syncthreads();
-    if (s_tmp[4] >= 0 || base + kPaThreads >= p.batch) break;
+    if (s_tmp[W] >= 0 || base + 32 * W >= p.batch) break;
     run += part;
   }
-  b_out = s_tmp[4];
-  before = s_tmp[5];
-  len_out = s_tmp[6];
+  b_out = s_tmp[W];
+  before = s_tmp[W + 1];
+  len_out = s_tmp[W + 2];
   return true;
 }
 
@@ -254,37 +269,40 @@ __device__ __forceinline__ bool find_share(const AttnParams& p, F count, int* s_
 // ---------------------------------------------------------------------------
 template <int HD, int MT>
 struct PaShape {
+  static constexpr int W = HD == 256 ? 4 : 8;        // warps
+  static constexpr int THREADS = 32 * W;
+  static constexpr int TILE = 16 * W;                // tokens
   static constexpr int RT = 16 * MT;                 // rows of an item
-  static constexpr int WT = kPaWarps / MT;           // warps along the tokens
+  static constexpr int WT = W / MT;                  // warps along the tokens
   static constexpr int CH = HD / 8;                  // 16-byte chunks per token
-  static constexpr int kPanels = HD / 64;            // 128-byte columns of a 16-token block
+  static constexpr int kPanels = HD / 64;            // 128-byte columns of a block
   static constexpr int kBlock = 16 * HD * 2;         // K (or V) of a block: [panel][16][128 bytes], swizzled
-  static constexpr int kKV = (kPaTile / 16) * kBlock;
+  static constexpr int kKV = W * kBlock;
   static constexpr int kQ = RT * HD * 2;
   static constexpr int kStage = 2 * kKV;
-  // three tiles per CTA; two where three would leave one CTA per SM at
-  // head_dim 128, or none at 256
-  static constexpr int kStages = (HD == 128 && MT == 4) || (HD == 256 && MT > 1) ? 2 : 3;
-  static constexpr int kSmem = kStages * kStage + 2 * kQ;  // queries of the next two items
-  static_assert(kSmem <= 227 * 1024 - 1024, "shared memory");
+  // as many stages of 32 to 64 KB as fit beside the queries
+  static constexpr int kStages = HD == 64 ? 5 : HD == 256 && MT > 1 ? 2 : 3;
+  static constexpr int kItems = kStages - 1;  // that the fetches can be ahead: their queries
+  static constexpr int kSmem = kStages * kStage + kItems * kQ;
+  static_assert(kSmem <= 225 * 1024, "shared memory");
   static_assert(kStage % 1024 == 0, "the swizzle repeats every 1024 bytes");
-  static_assert(kPaWarps * 16 * HD * 4 == kStage, "the join buffer reuses a consumed stage");
+  static_assert(W * 16 * HD * 4 == kStage, "the join buffer reuses a consumed stage");
 };
 
 template <class T, int HD, int MT, bool WEIGHTS>
-__global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel(const __grid_constant__ AttnParams p) {
   using S = PaShape<HD, MT>;
-  constexpr int RT = S::RT, WT = S::WT, CH = S::CH, kStages = S::kStages;
+  constexpr int RT = S::RT, W = S::W, WT = S::WT, NB = MT == 1 || HD == 256 ? 1 : 2, CH = S::CH, kStages = S::kStages;
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ int s_tmp[8];
-  __shared__ __align__(8) uint64_t s_full[kStages][kPaWarps];  // one per block of 16 tokens
-  __shared__ uint32_t s_valid[kStages][kPaWarps];              // its tokens that have a page
-  __shared__ float s_m[kPaWarps][16], s_l[kPaWarps][16];
+  __shared__ int s_tmp[W + 4];
+  __shared__ __align__(8) uint64_t s_full[kStages][W];  // one per block of 16 tokens
+  __shared__ uint32_t s_valid[kStages][W];              // its tokens that have a page
+  __shared__ float s_m[W][16], s_l[W][16];
   __shared__ bool s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sbase = smem_u32(smem);
   if (tid == 0) {
-    for (int i = 0; i < kStages * kPaWarps; ++i) mbar_init(&s_full[0][0] + i, 1);
+    for (int i = 0; i < kStages * W; ++i) mbar_init(&s_full[0][0] + i, 1);
     fence_mbar_init();
   }
 
@@ -293,10 +311,10 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   Cursor c;
   if (WEIGHTS) pdl_trigger();
   // (its barriers also publish the mbarriers)
-  if (!find_share(p, [&](int len) { return seq_size<RT>(p, len); }, s_tmp, per, t0, t1, c.b, c.len, before)) return;
+  if (!find_share<W>(p, [&](int len) { return seq_size<S>(p, len); }, s_tmp, per, t0, t1, c.b, c.len, before)) return;
   int rem = t0 - before;
   for (c.rt = 0;; ++c.rt) {
-    set_item<RT>(p, c);
+    set_item<S>(p, c);
     if (rem < p.kv_heads * (kItemCost + c.n)) break;
     rem -= p.kv_heads * (kItemCost + c.n);
   }
@@ -313,7 +331,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   const int boxes = 16 >> p.lg_box;
   const int page_mask = (1 << p.lg_page) - 1;
   auto page_of = [&](const Cursor& u) {  // of this lane's box
-    const int tok = u.tile * kPaTile + warp * 16 + (lane << p.lg_box);
+    const int tok = u.tile * S::TILE + warp * 16 + (lane << p.lg_box);
     return lane < boxes && tok < p.capacity ? p.block_table[u.b * p.table_stride + (tok >> p.lg_page)] : -1;
   };
   int pid = page_of(ld);
@@ -321,7 +339,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
   auto issue = [&](bool first) {  // the tile at cursor ld (position t_ld), into stage ld_stage
     if (t_ld >= t1) return;
     const uint32_t st = sbase + ld_stage * S::kStage;
-    const int tok = ld.tile * kPaTile + warp * 16 + (lane << p.lg_box);
+    const int tok = ld.tile * S::TILE + warp * 16 + (lane << p.lg_box);
     const bool ok = lane < boxes && tok < ld.hi && pid >= 0 && pid < p.num_pages;
     const uint32_t got = __ballot_sync(0xffffffffu, ok);
     const uint32_t bar = smem_u32(&s_full[ld_stage][warp]);
@@ -345,21 +363,21 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     }
     if (ld.tile == 0 || first) {
       const T* q = static_cast<const T*>(p.q);
-      for (int i = tid; i < RT * CH; i += kPaThreads) {
+      for (int i = tid; i < RT * CH; i += S::THREADS) {
         const int r = i / CH, chunk = i % CH, row = ld.rt * RT + r;
         const bool on = row < p.rows && chunk * 8 < p.head_dim;
-        const int j = on ? row / p.group : 0;
+        const int j = on ? token_of(p, row) : 0;
         const int64_t o = on ? (((int64_t)ld.b * p.tokens + j) * p.q_heads + ld.h * p.group + row - j * p.group) *
                                        p.head_dim + chunk * 8
                              : 0;
         cp_async16_zfill(sbase + kStages * S::kStage + ld_item * S::kQ + r * (HD * 2) + ((chunk ^ (r & 7)) << 4), q + o, on);
       }
-      ld_item ^= 1;
+      ld_item = ld_item + 1 == S::kItems ? 0 : ld_item + 1;
     }
     ld_stage = ld_stage + 1 == kStages ? 0 : ld_stage + 1;
     t_ld += ld.tile + 1 == ld.n ? 1 + kItemCost : 1;
     if (t_ld < t1) {
-      step_cursor<RT>(p, ld);
+      step_cursor<S>(p, ld);
       pid = page_of(ld);
     }
   };
@@ -382,7 +400,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       const int r = mt * 16 + (lane & 15), chunk = ks * 2 + (lane >> 4);
       ldsm4(qf[ks], sbase + kStages * S::kStage + item * S::kQ + r * (HD * 2) + ((chunk ^ (r & 7)) << 4));
     }
-    item ^= 1;
+    item = item + 1 == S::kItems ? 0 : item + 1;
     float o[HD / 8][4];
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -392,10 +410,10 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int row = row0 + r0 + 8 * e;
-      jr[e] = row / p.group;
+      jr[e] = token_of(p, row);
       vis[e] = row < p.rows ? visible(p, c.len, row) : 0;
     }
-    const int j_lo = row0 / p.group, j_hi = last_row / p.group;  // j_hi < j_lo where these 16 rows are empty
+    const int j_lo = token_of(p, row0), j_hi = token_of(p, last_row);
     const int vis_lo = last_row >= row0 ? visible(p, c.len, row0) : 0;  // slots seen by every row,
     const int vis_hi = last_row >= row0 ? visible(p, c.len, last_row) : 0;  // and by any
     const int t_end = min(t1, t + c.n - c.tile);
@@ -406,7 +424,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
         if (row0 + r0 + 8 * e < p.rows)
 #pragma unroll
           for (int n = 0; n < 2; ++n)
-            *reinterpret_cast<float2*>(p.sbuf + ((size_t)t * RT + mt * 16 + r0 + 8 * e) * kPaTile + blk * 16 + n * 8 + cq * 2) =
+            *reinterpret_cast<float2*>(p.sbuf + ((size_t)t * RT + mt * 16 + r0 + 8 * e) * S::TILE + blk * 16 + n * 8 + cq * 2) =
                 s ? make_float2(s[n][2 * e], s[n][2 * e + 1]) : make_float2(-INFINITY, -INFINITY);
     };
 
@@ -418,53 +436,69 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       issue(false);
       const uint32_t st = sbase + stage * S::kStage;
 
-      // blocks of 16 tokens: one per warp at MT = 1, MT of them otherwise
+      // this warp's MT blocks of 16 tokens, NB at a time
 #pragma unroll 1
-      for (int blk = tw * MT; blk < (tw + 1) * MT; ++blk) {
-        const int tok0 = c.tile * kPaTile + blk * 16;
+      for (int blk = tw * MT; blk < (tw + 1) * MT; blk += NB) {
+        const int tok0 = c.tile * S::TILE + blk * 16;
         if (tok0 >= vis_hi) {  // nothing here for these rows (what was fetched is waited for by the rows that see it)
-          if (WEIGHTS) store_scores(blk, nullptr);
+          if (WEIGHTS)
+            for (int i = 0; i < NB; ++i) store_scores(blk + i, nullptr);
           continue;
         }
-        if (!dead && !mbar_wait(&s_full[stage][blk], phase)) {
-          dead = true;  // reported through the status word; the outputs become NaN
-          atomicOr(p.status, 1u);
+        uint32_t valid[NB];
+        bool whole = true;  // every slot seen by every row
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          if (!dead && !mbar_wait(&s_full[stage][blk + i], phase)) {
+            dead = true;  // reported through the status word; the outputs become NaN
+            atomicOr(p.status, 1u);
+          }
+          valid[i] = s_valid[stage][blk + i];
+          whole = whole && valid[i] == 0xffffu && tok0 + 16 * (i + 1) <= vis_lo;
         }
-        const uint32_t valid = s_valid[stage][blk];
         const uint32_t kb = st + blk * S::kBlock;
-        float s[2][4], s2[2][4];
+        float s[2 * NB][4], s2[2][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int e = 0; e < 4; ++e) {
+          s2[0][e] = s2[1][e] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {  // two chains of products per score
-          uint32_t kf[4];
-          const int r = (lane & 7) + ((lane >> 4) << 3), chunk = ks * 2 + ((lane >> 3) & 1);
-          ldsm4(kf, kb + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
-          Mma<T>::run(ks & 1 ? s2[0] : s[0], qf[ks], kf[0], kf[1]);
-          Mma<T>::run(ks & 1 ? s2[1] : s[1], qf[ks], kf[2], kf[3]);
+          for (int n = 0; n < 2 * NB; ++n) s[n][e] = 0.f;
         }
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int ks = 0; ks < HD / 16; ++ks) {  // four chains of products
+          const int r = (lane & 7) + ((lane >> 4) << 3), chunk = ks * 2 + ((lane >> 3) & 1);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = (s[n][e] + s2[n][e]) * p.scale_log2;
-        const bool whole = valid == 0xffffu && tok0 + 16 <= vis_lo;  // every slot seen by every row
+          for (int i = 0; i < NB; ++i) {
+            uint32_t kf[4];
+            ldsm4(kf, kb + i * S::kBlock + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
+            Mma<T>::run(NB == 1 && (ks & 1) ? s2[0] : s[2 * i], qf[ks], kf[0], kf[1]);
+            Mma<T>::run(NB == 1 && (ks & 1) ? s2[1] : s[2 * i + 1], qf[ks], kf[2], kf[3]);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < 2 * NB; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = (NB == 1 ? s[n][e] + s2[n % 2][e] : s[n][e]) * p.scale_log2;
         if (!whole) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < 2 * NB; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int col = n * 8 + cq * 2 + (e & 1);
-              if (!((valid >> col) & 1u) || tok0 + col >= vis[e >> 1]) s[n][e] = -INFINITY;
+              if (!((valid[n / 2] >> (col & 15)) & 1u) || tok0 + col >= vis[e >> 1]) s[n][e] = -INFINITY;
             }
         }
-        if (WEIGHTS) store_scores(blk, s);
+        if (WEIGHTS) {
+#pragma unroll
+          for (int i = 0; i < NB; ++i) store_scores(blk + i, s + 2 * i);
+        }
         // running maximum: the quad of four lanes shares a row
         float mn[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
+          float x = fmaxf(s[0][2 * e], s[0][2 * e + 1]);
+#pragma unroll
+          for (int n = 1; n < 2 * NB; ++n) x = fmaxf(x, fmaxf(s[n][2 * e], s[n][2 * e + 1]));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
           mn[e] = fmaxf(m[e], x);
@@ -484,58 +518,93 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
           }
         }
         const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
+        uint32_t ph[NB][4], pl[NB][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < 2 * NB; ++n) {
           s[n][0] = exp2f(s[n][0] - b0);
           s[n][1] = exp2f(s[n][1] - b0);
           s[n][2] = exp2f(s[n][2] - b1);
           s[n][3] = exp2f(s[n][3] - b1);
           l[0] += s[n][0] + s[n][1];
           l[1] += s[n][2] + s[n][3];
+          Mma<T>::split(s[n][0], s[n][1], ph[n / 2][n % 2 * 2], pl[n / 2][n % 2 * 2]);
+          Mma<T>::split(s[n][2], s[n][3], ph[n / 2][n % 2 * 2 + 1], pl[n / 2][n % 2 * 2 + 1]);
         }
-        uint32_t ph[4], pl[4];
-        Mma<T>::split(s[0][0], s[0][1], ph[0], pl[0]);
-        Mma<T>::split(s[0][2], s[0][3], ph[1], pl[1]);
-        Mma<T>::split(s[1][0], s[1][1], ph[2], pl[2]);
-        Mma<T>::split(s[1][2], s[1][3], ph[3], pl[3]);
-        const uint32_t vb = kb + S::kKV;
-        if (whole) {
+        // o += P V, 16-column pairs at a time (independent products in a row);
+        // `keep` masks the V fragments' two tokens of each 8 where MASKED
+        auto v_frag = [&](int i, int nn, uint32_t (&vf)[4]) {
+          const int r = lane & 15, chunk = nn * 2 + (lane >> 4);
+          ldsm4t(vf, kb + i * S::kBlock + S::kKV + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
+        };
+        auto keep_of = [&](int i, int see, uint32_t (&k)[2]) {  // tokens of block i below `see` that have a page
+          see -= tok0 + 16 * i;
+          const uint32_t seen = (see >= 16 ? valid[i] : see <= 0 ? 0u : valid[i] & ((1u << see) - 1u)) >> (cq * 2);
+          k[0] = (seen & 1u ? 0x0000ffffu : 0u) | (seen & 2u ? 0xffff0000u : 0u);
+          k[1] = (seen & 0x100u ? 0x0000ffffu : 0u) | (seen & 0x200u ? 0xffff0000u : 0u);
+        };
+        auto product = [&](int i, const uint32_t (&k)[2], auto masked) {
 #pragma unroll
-          for (int nn = 0; nn < HD / 16; ++nn) {
-            uint32_t vf[4];
-            const int r = lane & 15, chunk = nn * 2 + (lane >> 4);
-            ldsm4t(vf, vb + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
-            Mma<T>::run(o[2 * nn], ph, vf[0], vf[1]);
-            Mma<T>::run(o[2 * nn + 1], ph, vf[2], vf[3]);
-            Mma<T>::run(o[2 * nn], pl, vf[0], vf[1]);
-            Mma<T>::run(o[2 * nn + 1], pl, vf[2], vf[3]);
+          for (int nn = 0; nn < HD / 16; nn += 2) {
+            uint32_t vf[2][4];
+            v_frag(i, nn, vf[0]);
+            v_frag(i, nn + 1, vf[1]);
+            if constexpr (decltype(masked)::value) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) vf[e / 4][e % 4] &= k[e & 1];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) Mma<T>::run(o[2 * nn + e], ph[i], vf[e / 2][e % 2 * 2], vf[e / 2][e % 2 * 2 + 1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) Mma<T>::run(o[2 * nn + e], pl[i], vf[e / 2][e % 2 * 2], vf[e / 2][e % 2 * 2 + 1]);
           }
+        };
+        if (whole) {
+          const uint32_t all[2] = {~0u, ~0u};
+#pragma unroll
+          for (int i = 0; i < NB; ++i) product(i, all, std::false_type{});
         } else {
-          // Some slots are not seen by some rows, and 0 * (what they hold) may be
-          // NaN: each step token's product takes V with the slots it does not see
-          // zeroed, and only its own rows of the result.
+          // Slots that no row sees are zeroed (0 * what they hold may be NaN).
+          // Slots that some rows see and others do not are harmless while V is
+          // finite there; where it is not, each step token's product takes only
+          // what the token sees, and only its own rows of the result.
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            uint32_t k[2];
+            keep_of(i, vis_hi, k);
+            bool apart = false;
+            if (j_lo < j_hi) {
+#pragma unroll
+              for (int nn = 0; nn < HD / 16; ++nn) {
+                uint32_t vf[4];
+                v_frag(i, nn, vf);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) apart = apart || Mma<T>::not_finite(vf[e] & k[e & 1]);
+              }
+              apart = __any_sync(0xffffffffu, apart);
+            }
+            if (!apart) {
+              product(i, k, std::true_type{});
+              continue;
+            }
 #pragma unroll 1
-          for (int j = j_lo; j <= j_hi; ++j) {
-            const int see = visible(p, c.len, j * p.group) - tok0;  // slots of this block
-            const uint32_t seen = (see >= 16 ? valid : see <= 0 ? 0u : valid & ((1u << see) - 1u)) >> (cq * 2);
-            const uint32_t k0 = (seen & 1u ? 0x0000ffffu : 0u) | (seen & 2u ? 0xffff0000u : 0u);
-            const uint32_t k1 = (seen & 0x100u ? 0x0000ffffu : 0u) | (seen & 0x200u ? 0xffff0000u : 0u);
+            for (int j = j_lo; j <= j_hi; ++j) {
+              keep_of(i, visible(p, c.len, j * p.group), k);
 #pragma unroll
-            for (int nn = 0; nn < HD / 16; ++nn) {
-              uint32_t vf[4];
-              const int r = lane & 15, chunk = nn * 2 + (lane >> 4);
-              ldsm4t(vf, vb + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
-              float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-              Mma<T>::run(x, ph, vf[0] & k0, vf[1] & k1);
-              Mma<T>::run(y, ph, vf[2] & k0, vf[3] & k1);
-              Mma<T>::run(x, pl, vf[0] & k0, vf[1] & k1);
-              Mma<T>::run(y, pl, vf[2] & k0, vf[3] & k1);
+              for (int nn = 0; nn < HD / 16; ++nn) {
+                uint32_t vf[4];
+                v_frag(i, nn, vf);
+                float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+                Mma<T>::run(x, ph[i], vf[0] & k[0], vf[1] & k[1]);
+                Mma<T>::run(y, ph[i], vf[2] & k[0], vf[3] & k[1]);
+                Mma<T>::run(x, pl[i], vf[0] & k[0], vf[1] & k[1]);
+                Mma<T>::run(y, pl[i], vf[2] & k[0], vf[3] & k[1]);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (jr[e >> 1] == j) {
-                  o[2 * nn][e] += x[e];
-                  o[2 * nn + 1][e] += y[e];
-                }
+                for (int e = 0; e < 4; ++e)
+                  if (jr[e >> 1] == j) {
+                    o[2 * nn][e] += x[e];
+                    o[2 * nn + 1][e] += y[e];
+                  }
+              }
             }
           }
         }
@@ -550,38 +619,42 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     }
 
     // ---- the end of this CTA's part of the item ----
+    const int nrow = min(RT, p.rows - c.rt * RT);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       if (dead) l[e] = __int_as_float(0x7fc00000);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-      if (cq == 0) {
-        s_m[warp][r0 + 8 * e] = m[e];
-        s_l[warp][r0 + 8 * e] = l[e];
-      }
+      if (cq == 0) s_m[warp][r0 + 8 * e] = m[e];
     }
     __syncthreads();  // every warp is done with this tile: its stage becomes the join buffer
     float* buf = reinterpret_cast<float*>(smem + stage * S::kStage);  // [warp][16][HD], 32-byte groups swizzled
 #pragma unroll
-    for (int n = 0; n < HD / 8; ++n)
+    for (int e = 0; e < 2; ++e) {
+      const int r = r0 + 8 * e;
+      if (mt * 16 + r < nrow) {  // the warp's sums, to the row's maximum over its warps
+        float M = s_m[mt * WT][r];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = r0 + 8 * e;
-        *reinterpret_cast<float2*>(buf + (warp * 16 + r) * HD + ((n * 8 + cq * 2) ^ ((r & 7) << 3))) =
-            make_float2(o[n][2 * e], o[n][2 * e + 1]);
+        for (int w = 1; w < WT; ++w) M = fmaxf(M, s_m[mt * WT + w][r]);
+        const float f = exp2_diff(m[e], M);
+        if (cq == 0) s_l[warp][r] = l[e] == 0.f ? 0.f : l[e] * f;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n)
+          *reinterpret_cast<float2*>(buf + (warp * 16 + r) * HD + ((n * 8 + cq * 2) ^ ((r & 7) << 3))) =
+              make_float2(o[n][2 * e] * f, o[n][2 * e + 1] * f);
       }
+    }
     __syncthreads();
     const int begin = t - c.tile, end = begin + c.n;  // the item's tiles
     const int c0 = begin / per, c1 = (end - 1) / per; // CTAs that share it
     const bool alone = c0 == c1;
-    const int nrow = min(RT, p.rows - c.rt * RT);
     const int slot = blockIdx.x == c0 ? 1 : 0;  // an item that began in an earlier CTA: slot 0
     float* po = p.part_o + (size_t)(blockIdx.x * 2 + slot) * RT * HD;
     float2* pml = p.part_ml + (blockIdx.x * 2 + slot) * RT;
     const int64_t out0 = ((int64_t)c.b * p.tokens) * p.q_heads + c.h * p.group;
     auto finish = [&](int r, int d, const auto& v, float M, float L) {  // row r, elements d..
       constexpr int N = sizeof(v) / sizeof(float);
-      const int row = c.rt * RT + r, j = row / p.group;
+      const int row = c.rt * RT + r, j = token_of(p, row);
       const int64_t at = out0 + (int64_t)j * p.q_heads + row - j * p.group;
       const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
       if (d < p.head_dim) {
@@ -596,23 +669,20 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
         if (WEIGHTS) p.lse2[((int64_t)c.b * p.kv_heads + c.h) * p.rows + row] = lg;
       }
     };
-    for (int i = tid; i < nrow * (HD / 4); i += kPaThreads) {
+    for (int i = tid; i < nrow * (HD / 4); i += S::THREADS) {
       const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
       const int w0 = (r / 16) * WT, rr = r % 16;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WT; ++w) M = fmaxf(M, s_m[w0 + w][rr]);
+      float M = s_m[w0][rr], L = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      float L = 0.f;
 #pragma unroll
       for (int w = 0; w < WT; ++w) {
-        const float f = exp2_diff(s_m[w0 + w][rr], M);
         const float4 x = *reinterpret_cast<const float4*>(buf + ((w0 + w) * 16 + rr) * HD + (d ^ ((rr & 7) << 3)));
-        L = fmaf(s_l[w0 + w][rr], f, L);
-        v.x = fmaf(x.x, f, v.x);
-        v.y = fmaf(x.y, f, v.y);
-        v.z = fmaf(x.z, f, v.z);
-        v.w = fmaf(x.w, f, v.w);
+        M = fmaxf(M, s_m[w0 + w][rr]);
+        L += s_l[w0 + w][rr];
+        v.x += x.x;
+        v.y += x.y;
+        v.z += x.z;
+        v.w += x.w;
       }
       if (alone) {
         const float vv[4] = {v.x, v.y, v.z, v.w};
@@ -634,7 +704,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
       if (s_last) {
         // a warp per row, each lane HD / 32 neighbouring elements
         constexpr int E = HD / 32;
-        for (int r = warp; r < nrow; r += kPaWarps) {
+        for (int r = warp; r < nrow; r += W) {
           float M = -INFINITY, L = 0.f, v[E];
 #pragma unroll
           for (int e = 0; e < E; ++e) v[e] = 0.f;
@@ -696,7 +766,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();  // the join buffer's stage may be filled again
     t += c.tile + 1 == c.n ? 1 + kItemCost : 1;
-    if (t < t1) step_cursor<RT>(p, c);
+    if (t < t1) step_cursor<S>(p, c);
     if (++stage == kStages) {
       stage = 0;
       phase ^= 1u;
@@ -709,40 +779,41 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
 // from the scores that the attention kernel left in the workspace (16 bytes a
 // slot and four rows, against head_dim * 4 for reading K again)
 // ---------------------------------------------------------------------------
-template <int RT>
-__global__ void __launch_bounds__(kPaThreads) paged_weights_kernel(const __grid_constant__ AttnParams p) {
-  __shared__ int s_tmp[8];
+template <class S>
+__global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int W = kWtThreads / 32, RT = S::RT, TILE = S::TILE;
+  __shared__ int s_tmp[W + 4];
   pdl_wait();
   const int last = p.row_tiles - 1;
-  auto count = [&](int len) { return p.kv_heads * item_tiles<RT>(p, len, last); };
+  auto count = [&](int len) { return p.kv_heads * item_tiles<S>(p, len, last); };
   int per, t0, t1, b, len, before;
-  if (!find_share(p, count, s_tmp, per, t0, t1, b, len, before)) return;
+  if (!find_share<W>(p, count, s_tmp, per, t0, t1, b, len, before)) return;
   // positions of the attention kernel's index space before sequence b
   int c1 = 0;
-  for (int i = threadIdx.x; i < b; i += kPaThreads) c1 += seq_size<RT>(p, p.lengths[i]);
-  int base = block_sum(c1, s_tmp);
-  int n = item_tiles<RT>(p, len, last);
-  const int half = threadIdx.x >> 6, tok = threadIdx.x & 63;  // two tiles at a time
-  for (int t = t0 + half; t < t1; t += 2) {
+  for (int i = threadIdx.x; i < b; i += kWtThreads) c1 += seq_size<S>(p, p.lengths[i]);
+  int base = block_sum<W>(c1, s_tmp);
+  int n = item_tiles<S>(p, len, last);
+  const int sub = threadIdx.x / TILE, tok = threadIdx.x % TILE;
+  for (int t = t0 + sub; t < t1; t += kWtThreads / TILE) {
     while (t - before >= p.kv_heads * n) {
       before += p.kv_heads * n;
-      base += seq_size<RT>(p, len);
+      base += seq_size<S>(p, len);
       len = p.lengths[++b];
-      n = item_tiles<RT>(p, len, last);
+      n = item_tiles<S>(p, len, last);
     }
     const int h = (t - before) / n, tile = (t - before) - h * n;
-    const int slot = tile * kPaTile + tok;
+    const int slot = tile * TILE + tok;
     if (slot >= visible(p, len, p.rows - 1)) continue;
     float w = 0.f;
     int off = base;
     for (int rt = 0; rt <= last; ++rt) {
-      const int nt = item_tiles<RT>(p, len, rt);
+      const int nt = item_tiles<S>(p, len, rt);
       if (tile < nt) {
-        const float* s = p.sbuf + (size_t)(off + h * (kItemCost + nt) + kItemCost + tile) * RT * kPaTile + tok;
+        const float* s = p.sbuf + (size_t)(off + h * (kItemCost + nt) + kItemCost + tile) * RT * TILE + tok;
         const float* z = p.lse2 + ((int64_t)b * p.kv_heads + h) * p.rows + rt * RT;
         const int rows = min(RT, p.rows - rt * RT);
 #pragma unroll 4
-        for (int r = 0; r < rows; ++r) w += exp2_diff(s[r * kPaTile], z[r]);
+        for (int r = 0; r < rows; ++r) w += exp2_diff(s[r * TILE], z[r]);
       }
       off += p.kv_heads * (kItemCost + nt);
     }
@@ -754,7 +825,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_weights_kernel(const __grid_
 // host side
 // ---------------------------------------------------------------------------
 struct PaPlan {
-  int hd, mt;
+  int hd, mt, tile;
   int64_t max_tiles, positions, ml_off, o_off, lse_off, s_off, bytes;
 };
 
@@ -771,7 +842,8 @@ tp_status plan_attn(const tp_paged_cache* c, int tokens, int q_heads, int accumu
   const int64_t rt = 16 * pl.mt, row_tiles = (rows + rt - 1) / rt;
   const int64_t cap = (int64_t)c->max_pages * c->page_size;
   const int64_t items = (int64_t)c->batch * c->kv_heads * row_tiles;
-  pl.max_tiles = items * std::max<int64_t>(1, (cap + kPaTile - 1) / kPaTile);
+  pl.tile = pl.hd == 256 ? 64 : 128;
+  pl.max_tiles = items * std::max<int64_t>(1, (cap + pl.tile - 1) / pl.tile);
   pl.positions = pl.max_tiles + items * kItemCost;
   if (rows > (1 << 24) || items > (1 << 30) || pl.positions > (int64_t(1) << 30))
     return fail(TP_ERR_UNSUPPORTED, "tp_paged_attn: too many rows, sequences or slots");
@@ -785,7 +857,7 @@ tp_status plan_attn(const tp_paged_cache* c, int tokens, int q_heads, int accumu
   pl.o_off = take((int64_t)kPaMaxCtas * 2 * rt * pl.hd * 4);
   if (accumulate) {
     pl.lse_off = take((int64_t)c->batch * c->kv_heads * rows * 4);
-    pl.s_off = take(pl.positions * rt * kPaTile * 4);
+    pl.s_off = take(pl.positions * rt * pl.tile * 4);
   }
   pl.bytes = at;
   *out = pl;
@@ -837,6 +909,7 @@ tp_status page_map(const tp_paged_cache* c, void* base, bool token_major, int bo
 template <class T, int HD, int MT>
 tp_status launch_attn(const AttnParams& p, const PaPlan& pl, bool weights, cudaStream_t st) {
   using S = PaShape<HD, MT>;
+  static_assert(S::TILE == (HD == 256 ? 64 : 128), "as plan_attn");
   const auto kern = weights ? paged_attn_kernel<T, HD, MT, true> : paged_attn_kernel<T, HD, MT, false>;
   static int smem_set[2][64];
   static int ctas[2][64];  // resident CTAs per SM
@@ -848,24 +921,24 @@ tp_status launch_attn(const AttnParams& p, const PaPlan& pl, bool weights, cudaS
   TP_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
   int occ = __atomic_load_n(&ctas[weights][dev], __ATOMIC_RELAXED);
   if (!occ) {
-    TP_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, kPaThreads, S::kSmem), "paged_attn: occupancy");
+    TP_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, S::THREADS, S::kSmem), "paged_attn: occupancy");
     if (occ < 1) return fail(TP_ERR_CUDA, "paged_attn: the kernel does not fit this device");
     __atomic_store_n(&ctas[weights][dev], occ, __ATOMIC_RELAXED);
   }
   const int grid = static_cast<int>(std::min<int64_t>(std::min(kPaMaxCtas, sms * occ), pl.positions));
-  kern<<<grid, kPaThreads, S::kSmem, st>>>(p);
+  kern<<<grid, S::THREADS, S::kSmem, st>>>(p);
   s = check_launch("paged_attn launch");
   if (s != TP_OK || !weights) return s;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(8 * sms, pl.max_tiles)));
-  cfg.blockDim = dim3(kPaThreads);
+  cfg.blockDim = dim3(kWtThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_weights_kernel<S::RT>, p), "paged_weights launch");
+  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_weights_kernel<S>, p), "paged_weights launch");
   return clear_ok();
 }
 
@@ -932,6 +1005,7 @@ TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_ca
   p.head_dim = cache->head_dim;
   p.lg_page = log2_int(cache->page_size);
   p.capacity = cache->max_pages * cache->page_size;
+  p.group_inv = p.group == 1 ? 0 : ~uint64_t(0) / p.group + 1;
   p.rows = a.tokens * p.group;
   p.row_tiles = (p.rows + 16 * pl.mt - 1) / (16 * pl.mt);
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
