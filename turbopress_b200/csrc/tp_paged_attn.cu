@@ -21,12 +21,13 @@
 // arrive (a counter at the item's first CTA) joins them in run order, so the
 // result does not depend on timing.
 //
-// Tile: each of the four warps fetches its own 16 tokens of K and V as tensor
-// (TMA) boxes of up to 16 tokens x 128 bytes, one page id per box fetched one
-// tile ahead, two tiles in flight behind the one in use; the hardware's
-// 128-byte swizzle makes the fragment loads conflict-free.  Up to 16 rows a
-// warp consumes only what it fetched: no CTA barrier in the loop.  With more
-// rows the warps share the tile: MT row tiles of 16, 4/MT warps each.  Slots
+// Tile: four producer warps fetch tiles of 16 tokens per consumer warp as tensor
+// (TMA) boxes of up to 16 tokens x 128 bytes, page ids one tile ahead, through
+// a ring of stages; the hardware's 128-byte swizzle makes the fragment loads
+// conflict-free.  Up to 16 rows, each consumer warp takes its own 16 tokens;
+// with more, MT row tiles of 16 take W/MT warps each.  Consumers meet only
+// where an item ends.  An item's queries go from memory straight to the
+// registers of the products, fetched while the item before is joined.  Slots
 // that a row does not see may hold anything: their scores are replaced and
 // their V zeroed in registers, in the blocks where that can happen.
 #include <cuda.h>
@@ -51,7 +52,7 @@ constexpr int kPaStatusOff = kPaMaxCtas * 4;      // status word after the count
 constexpr int kPaCounterBytes = kPaStatusOff + 256;
 
 struct AttnParams {
-  CUtensorMap k_map, v_map;  // {head_dim, token | head, head | token, page}
+  CUtensorMap k_map, v_map;  // {64 elements, token, panel, head, page}, or without panels {head_dim, token, 1, head, page}
   const void* q;
   void* out;
   float* lse;
@@ -59,7 +60,7 @@ struct AttnParams {
   const int32_t* lengths;
   float* scores;
   int64_t num_pages, table_stride;
-  int token_major;  // the maps' second dimension is the head
+  int panels;       // boxes hold all panels of 64 elements
   int lg_box;       // log2 of the tokens per box: min(16, page_size)
   int batch, tokens, q_heads, kv_heads, group, head_dim;
   int lg_page, capacity;
@@ -75,23 +76,14 @@ struct AttnParams {
   float* sbuf;     // [index space][16*MT][TILE] scores in log2 units (accumulate only)
 };
 
-__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool on) {
-  const int bytes = on ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int token, int head, int page,
+                                        uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+      "[%7];" ::"r"(dst), "l"(map), "r"(x), "r"(token), "r"(0), "r"(head), "r"(page), "r"(bar)
       : "memory");
 }
 
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(a)
-               : "memory");
-}
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -143,6 +135,12 @@ struct Mma<__nv_bfloat16> {
     lo = *reinterpret_cast<const uint32_t*>(&r);
   }
 };
+
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
 
 // 2^(a - b) for a <= b, 0 where a is -inf (also where both are).
 __device__ __forceinline__ float exp2_diff(float a, float b) { return a == -INFINITY ? 0.f : exp2f(a - b); }
@@ -212,27 +210,21 @@ __device__ __forceinline__ int block_sum(int v, int* s_tmp) {
 // This CTA's equal share [t0, t1) of the concatenation of `count(len)`
 // positions per sequence, `per` positions each; the sequence holding t0, its
 // length and the positions before it.  False (in every thread) where the share
-// is empty.
+// is empty.  s_tmp: W + 3 words.
 template <int W, class F>
 __device__ __forceinline__ bool find_share(const AttnParams& p, F count, int* s_tmp, int& per, int& t0, int& t1, int& b_out,
                                            int& len_out, int& before) {
+  constexpr int N = 32 * W;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int len = threadIdx.x < p.batch ? p.lengths[threadIdx.x] : 0;
-  int own = threadIdx.x < p.batch ? count(len) : 0;
-  int sum = own;
-  for (int b = threadIdx.x + 32 * W; b < p.batch; b += 32 * W) sum += count(p.lengths[b]);
-  const int total = block_sum<W>(sum, s_tmp);
-  per = (total + gridDim.x - 1) / gridDim.x;
-  t0 = min((int)blockIdx.x * per, total);
-  t1 = min(t0 + per, total);
-  if (t0 >= t1) return false;
+  int rest = 0;  // sequences past the first block of the scan
+  if (p.batch > N) {
+    for (int b = threadIdx.x + N; b < p.batch; b += N) rest += count(p.lengths[b]);
+    rest = block_sum<W>(rest, s_tmp);
+  }
   int run = 0;
-  for (int base = 0;; base += 32 * W) {
-    if (base) {
-      const int b = base + threadIdx.x;
-      len = b < p.batch ? p.lengths[b] : 0;
-      own = b < p.batch ? count(len) : 0;
-    }
+  for (int base = 0; base < p.batch; base += N) {
+    const int b = base + threadIdx.x;
+    const int len = b < p.batch ? p.lengths[b] : 0, own = b < p.batch ? count(len) : 0;
     int inc = own;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -249,13 +241,20 @@ __device__ __forceinline__ bool find_share(const AttnParams& p, F count, int* s_
       if (w < warp) inc += s_tmp[w];
       part += s_tmp[w];
     }
+    if (base == 0) {
+      const int total = part + rest;
+      per = (total + gridDim.x - 1) / gridDim.x;
+      t0 = min((int)blockIdx.x * per, total);
+      t1 = min(t0 + per, total);
+      if (t0 >= t1) return false;
+    }
     if (own > 0 && run + inc - own <= t0 && t0 < run + inc) {
-      s_tmp[W] = base + threadIdx.x;
+      s_tmp[W] = b;
       s_tmp[W + 1] = run + inc - own;
       s_tmp[W + 2] = len;
     }
     __syncthreads();
-    if (s_tmp[W] >= 0 || base + 32 * W >= p.batch) break;
+    if (s_tmp[W] >= 0) break;
     run += part;
   }
   b_out = s_tmp[W];
@@ -269,40 +268,46 @@ __device__ __forceinline__ bool find_share(const AttnParams& p, F count, int* s_
 // ---------------------------------------------------------------------------
 template <int HD, int MT>
 struct PaShape {
-  static constexpr int W = HD == 256 ? 4 : 8;        // warps
-  static constexpr int THREADS = 32 * W;
+  static constexpr int W = HD == 256 ? 4 : 8;        // consumer warps
+  static constexpr int THREADS = 32 * (W + 4);       // and four producers
   static constexpr int TILE = 16 * W;                // tokens
   static constexpr int RT = 16 * MT;                 // rows of an item
   static constexpr int WT = W / MT;                  // warps along the tokens
-  static constexpr int CH = HD / 8;                  // 16-byte chunks per token
-  static constexpr int kPanels = HD / 64;            // 128-byte columns of a block
-  static constexpr int kBlock = 16 * HD * 2;         // K (or V) of a block: [panel][16][128 bytes], swizzled
+  static constexpr int kPanels = HD / 64;            // 128-byte columns of a block of 16 tokens
+  static constexpr int kBlock = 16 * HD * 2;         // its K (or V): [panel][16][128 bytes], swizzled
   static constexpr int kKV = W * kBlock;
-  static constexpr int kQ = RT * HD * 2;
-  static constexpr int kStage = 2 * kKV;
-  // as many stages of 32 to 64 KB as fit beside the queries
-  static constexpr int kStages = HD == 64 ? 5 : HD == 256 && MT > 1 ? 2 : 3;
-  static constexpr int kItems = kStages - 1;  // that the fetches can be ahead: their queries
-  static constexpr int kSmem = kStages * kStage + kItems * kQ;
+  static constexpr int kStage = 2 * kKV;             // 32 to 64 KB
+  static constexpr int kStages = HD == 64 ? 6 : 3;
+  static constexpr int kSmem = kStages * kStage;
   static_assert(kSmem <= 225 * 1024, "shared memory");
   static_assert(kStage % 1024 == 0, "the swizzle repeats every 1024 bytes");
   static_assert(W * 16 * HD * 4 == kStage, "the join buffer reuses a consumed stage");
 };
 
+template <int N>
+__device__ __forceinline__ void consumers_sync() {  // of N threads; the producers never join
+  asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
+}
+
 template <class T, int HD, int MT, bool WEIGHTS>
 __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel(const __grid_constant__ AttnParams p) {
   using S = PaShape<HD, MT>;
-  constexpr int RT = S::RT, W = S::W, WT = S::WT, NB = MT == 1 || HD == 256 ? 1 : 2, CH = S::CH, kStages = S::kStages;
+  constexpr int RT = S::RT, W = S::W, WT = S::WT, NB = MT == 1 || HD == 256 ? 1 : 2, kStages = S::kStages;
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ int s_tmp[W + 4];
-  __shared__ __align__(8) uint64_t s_full[kStages][W];  // one per block of 16 tokens
-  __shared__ uint32_t s_valid[kStages][W];              // its tokens that have a page
+  __shared__ int s_tmp[W + 8];
+  __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages];
+  __shared__ uint32_t s_valid[kStages][W];  // the tokens of a block of 16 that have a page
   __shared__ float s_m[W][16], s_l[W][16];
   __shared__ bool s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sbase = smem_u32(smem);
   if (tid == 0) {
-    for (int i = 0; i < kStages * W; ++i) mbar_init(&s_full[0][0] + i, 1);
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.v_map) : "memory");
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s_full[i], 4);
+      mbar_init(&s_empty[i], W);
+    }
     fence_mbar_init();
   }
 
@@ -311,7 +316,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
   Cursor c;
   if (WEIGHTS) pdl_trigger();
   // (its barriers also publish the mbarriers)
-  if (!find_share<W>(p, [&](int len) { return seq_size<S>(p, len); }, s_tmp, per, t0, t1, c.b, c.len, before)) return;
+  if (!find_share<W + 4>(p, [&](int len) { return seq_size<S>(p, len); }, s_tmp, per, t0, t1, c.b, c.len, before)) return;
   int rem = t0 - before;
   for (c.rt = 0;; ++c.rt) {
     set_item<S>(p, c);
@@ -325,82 +330,96 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
     c.tile = 0;
   }
   if (t0 >= t1) return;
-  Cursor ld = c;
-
-  // ---- loads: lane i < boxes of a warp fetches box i of the warp's block ----
-  const int boxes = 16 >> p.lg_box;
-  const int page_mask = (1 << p.lg_page) - 1;
-  auto page_of = [&](const Cursor& u) {  // of this lane's box
-    const int tok = u.tile * S::TILE + warp * 16 + (lane << p.lg_box);
-    return lane < boxes && tok < p.capacity ? p.block_table[u.b * p.table_stride + (tok >> p.lg_page)] : -1;
-  };
-  int pid = page_of(ld);
-  int ld_stage = 0, ld_item = 0, t_ld = t0;
-  auto issue = [&](bool first) {  // the tile at cursor ld (position t_ld), into stage ld_stage
-    if (t_ld >= t1) return;
-    const uint32_t st = sbase + ld_stage * S::kStage;
-    const int tok = ld.tile * S::TILE + warp * 16 + (lane << p.lg_box);
-    const bool ok = lane < boxes && tok < ld.hi && pid >= 0 && pid < p.num_pages;
-    const uint32_t got = __ballot_sync(0xffffffffu, ok);
-    const uint32_t bar = smem_u32(&s_full[ld_stage][warp]);
-    if (lane == 0) {
-      uint32_t valid = 0;
-      for (int i = 0; i < boxes; ++i)
-        if ((got >> i) & 1u) valid |= ((1u << (1 << p.lg_box)) - 1u) << (i << p.lg_box);
-      s_valid[ld_stage][warp] = valid;
-      const uint32_t bytes = __popc(got) * (S::kPanels * 2 * 128 << p.lg_box);
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-    }
-    __syncwarp();
-    if (ok) {
-      const int y = p.token_major ? ld.h : tok & page_mask, z = p.token_major ? tok & page_mask : ld.h;
-      const uint32_t d = st + warp * S::kBlock + ((lane << p.lg_box) << 7);
-#pragma unroll
-      for (int i = 0; i < S::kPanels; ++i) {
-        tma_box(d + i * 2048, &p.k_map, i * 64, y, z, pid, bar);
-        tma_box(d + S::kKV + i * 2048, &p.v_map, i * 64, y, z, pid, bar);
-      }
-    }
-    if (ld.tile == 0 || first) {
-      const T* q = static_cast<const T*>(p.q);
-      for (int i = tid; i < RT * CH; i += S::THREADS) {
-        const int r = i / CH, chunk = i % CH, row = ld.rt * RT + r;
-        const bool on = row < p.rows && chunk * 8 < p.head_dim;
-        const int j = on ? token_of(p, row) : 0;
-        const int64_t o = on ? (((int64_t)ld.b * p.tokens + j) * p.q_heads + ld.h * p.group + row - j * p.group) *
-                                       p.head_dim + chunk * 8
-                             : 0;
-        cp_async16_zfill(sbase + kStages * S::kStage + ld_item * S::kQ + r * (HD * 2) + ((chunk ^ (r & 7)) << 4), q + o, on);
-      }
-      ld_item = ld_item + 1 == S::kItems ? 0 : ld_item + 1;
-    }
-    ld_stage = ld_stage + 1 == kStages ? 0 : ld_stage + 1;
-    t_ld += ld.tile + 1 == ld.n ? 1 + kItemCost : 1;
-    if (t_ld < t1) {
-      step_cursor<S>(p, ld);
-      pid = page_of(ld);
+  int stage = 0, t = t0;
+  unsigned phase = 0;
+  auto next_stage = [&] {
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1u;
     }
   };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) issue(i == 0);
 
-  // ---- state of this warp's 16 rows ----
+  // Of the 168 registers that 384 threads get each, the producers' warpgroup
+  // gives up 112: 256 * 224 + 128 * 56 = 384 * 168.  (256 threads have 255.)
+  if (warp >= W) {
+    if (W == 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    // the producers: a quarter of a tile's boxes each, a box per lane (a warp
+    // issues its lanes' copies one after the other, some 90 cycles apart)
+    constexpr int B = W / 4;  // blocks of 16 tokens per producer
+    const int lg_boxes = 4 - p.lg_box, page_mask = (1 << p.lg_page) - 1;
+    const int at = (warp - W) * (16 * B) + (lane << p.lg_box);  // the lane's token of the tile
+    const bool mine = lane < (B << lg_boxes);
+    auto page_of = [&] {
+      const int tok = c.tile * S::TILE + at;
+      return mine && tok < p.capacity ? p.block_table[c.b * p.table_stride + (tok >> p.lg_page)] : -1;
+    };
+    int pid = page_of();
+    while (true) {
+      if (!mbar_wait(&s_empty[stage], phase ^ 1u)) {  // (the first round of the ring does not wait)
+        atomicOr(p.status, 1u);
+        return;
+      }
+      const uint32_t bar = smem_u32(&s_full[stage]);
+      const int tok = c.tile * S::TILE + at;
+      const bool ok = mine && tok < c.hi && pid >= 0 && pid < p.num_pages;
+      const uint32_t got = __ballot_sync(0xffffffffu, ok);
+      if (lane < B) {
+        uint32_t valid = 0;
+        for (int i = 0; i < 1 << lg_boxes; ++i)
+          if ((got >> ((lane << lg_boxes) + i)) & 1u) valid |= ((1u << (1 << p.lg_box)) - 1u) << (i << p.lg_box);
+        s_valid[stage][(warp - W) * B + lane] = valid;
+      }
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+                     "r"(__popc(got) * (S::kPanels * 2 * 128 << p.lg_box))
+                     : "memory");
+      __syncwarp();
+      if (ok) {
+        const uint32_t d = sbase + stage * S::kStage + (at >> 4) * S::kBlock + ((at & 15) << 7);
+        for (int i = 0; i < (p.panels ? 1 : S::kPanels); ++i) {
+          tma_box(d + i * 2048, &p.k_map, i * 64, tok & page_mask, c.h, pid, bar);
+          tma_box(d + S::kKV + i * 2048, &p.v_map, i * 64, tok & page_mask, c.h, pid, bar);
+        }
+      }
+      t += c.tile + 1 == c.n ? 1 + kItemCost : 1;
+      if (t >= t1) return;
+      step_cursor<S>(p, c);
+      pid = page_of();
+      next_stage();
+    }
+  }
+  if (W == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+
+  // ---- the consumers: this warp's 16 rows ----
   const int mt = warp / WT, tw = warp % WT;
   const int r0 = lane >> 2, cq = lane & 3;  // this thread: rows r0, r0 + 8, columns 2 cq + {0, 1} of each 8
   bool dead = false;
-  int stage = 0, item = 0, t = t0;
-  unsigned phase = 0;
-
-  while (t < t1) {  // an item, or this run's part of it
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();  // the queries are here
-    uint32_t qf[HD / 16][4];
+  // Fragments of the queries.  A product may take the columns in any order
+  // that both operands share: this thread holds the 16-byte chunks 2 cq and
+  // 2 cq + 1 of each 64 columns, so both operands load 16 bytes at a time.
+  uint32_t qf[HD / 16][4];
+  auto load_queries = [&] {
 #pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) {
-      const int r = mt * 16 + (lane & 15), chunk = ks * 2 + (lane >> 4);
-      ldsm4(qf[ks], sbase + kStages * S::kStage + item * S::kQ + r * (HD * 2) + ((chunk ^ (r & 7)) << 4));
+    for (int e = 0; e < 2; ++e) {
+      const int row = c.rt * RT + mt * 16 + r0 + 8 * e, j = token_of(p, row);
+      const T* q = static_cast<const T*>(p.q) +
+                   (((int64_t)c.b * p.tokens + j) * p.q_heads + c.h * p.group + row - j * p.group) * p.head_dim;
+#pragma unroll
+      for (int kk = 0; kk < HD / 32; ++kk) {
+        const int chunk = (kk >> 1) * 8 + 2 * cq + (kk & 1);
+        const uint4 x = row < p.rows && chunk * 8 < p.head_dim ? __ldg(reinterpret_cast<const uint4*>(q + chunk * 8))
+                                                                : make_uint4(0u, 0u, 0u, 0u);
+        qf[2 * kk][e] = x.x;
+        qf[2 * kk][2 + e] = x.y;
+        qf[2 * kk + 1][e] = x.z;
+        qf[2 * kk + 1][2 + e] = x.w;
+      }
     }
-    item = item + 1 == S::kItems ? 0 : item + 1;
+  };
+  load_queries();
+
+  while (true) {  // an item, or this run's part of it
     float o[HD / 8][4];
 #pragma unroll
     for (int n = 0; n < HD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -413,7 +432,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
       jr[e] = token_of(p, row);
       vis[e] = row < p.rows ? visible(p, c.len, row) : 0;
     }
-    const int j_lo = token_of(p, row0), j_hi = token_of(p, last_row);
+    const int j_lo = token_of(p, row0), j_hi = token_of(p, max(last_row, 0));
     const int vis_lo = last_row >= row0 ? visible(p, c.len, row0) : 0;  // slots seen by every row,
     const int vis_hi = last_row >= row0 ? visible(p, c.len, last_row) : 0;  // and by any
     const int t_end = min(t1, t + c.n - c.tile);
@@ -428,19 +447,17 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
                 s ? make_float2(s[n][2 * e], s[n][2 * e + 1]) : make_float2(-INFINITY, -INFINITY);
     };
 
-    for (bool head = true;; head = false) {
-      // Every warp has its queries, and is done with the stage that is filled
-      // next (last read in the round before; at MT = 1 by this warp alone).
-      if (MT > 1 || head) __syncthreads();
-      else __syncwarp();
-      issue(false);
+    while (true) {
       const uint32_t st = sbase + stage * S::kStage;
-
+      if (!dead && !mbar_wait(&s_full[stage], phase)) {
+        dead = true;  // reported through the status word; the outputs become NaN
+        atomicOr(p.status, 1u);
+      }
       // this warp's MT blocks of 16 tokens, NB at a time
 #pragma unroll 1
       for (int blk = tw * MT; blk < (tw + 1) * MT; blk += NB) {
         const int tok0 = c.tile * S::TILE + blk * 16;
-        if (tok0 >= vis_hi) {  // nothing here for these rows (what was fetched is waited for by the rows that see it)
+        if (tok0 >= vis_hi) {  // nothing here for these rows
           if (WEIGHTS)
             for (int i = 0; i < NB; ++i) store_scores(blk + i, nullptr);
           continue;
@@ -449,10 +466,6 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
         bool whole = true;  // every slot seen by every row
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          if (!dead && !mbar_wait(&s_full[stage][blk + i], phase)) {
-            dead = true;  // reported through the status word; the outputs become NaN
-            atomicOr(p.status, 1u);
-          }
           valid[i] = s_valid[stage][blk + i];
           whole = whole && valid[i] == 0xffffu && tok0 + 16 * (i + 1) <= vis_lo;
         }
@@ -465,14 +478,18 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
           for (int n = 0; n < 2 * NB; ++n) s[n][e] = 0.f;
         }
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks) {  // four chains of products
-          const int r = (lane & 7) + ((lane >> 4) << 3), chunk = ks * 2 + ((lane >> 3) & 1);
+        for (int kk = 0; kk < HD / 32; ++kk) {  // four chains of products
+          const int chunk = 2 * cq + (kk & 1);
 #pragma unroll
           for (int i = 0; i < NB; ++i) {
-            uint32_t kf[4];
-            ldsm4(kf, kb + i * S::kBlock + (chunk >> 3) * 2048 + r * 128 + (((chunk ^ r) & 7) << 4));
-            Mma<T>::run(NB == 1 && (ks & 1) ? s2[0] : s[2 * i], qf[ks], kf[0], kf[1]);
-            Mma<T>::run(NB == 1 && (ks & 1) ? s2[1] : s[2 * i + 1], qf[ks], kf[2], kf[3]);
+            uint4 kf[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              kf[n] = lds16(kb + i * S::kBlock + (kk >> 1) * 2048 + (n * 8 + r0) * 128 + (((chunk ^ r0) & 7) << 4));
+            Mma<T>::run(s[2 * i], qf[2 * kk], kf[0].x, kf[0].y);
+            Mma<T>::run(s[2 * i + 1], qf[2 * kk], kf[1].x, kf[1].y);
+            Mma<T>::run(NB == 1 ? s2[0] : s[2 * i], qf[2 * kk + 1], kf[0].z, kf[0].w);
+            Mma<T>::run(NB == 1 ? s2[1] : s[2 * i + 1], qf[2 * kk + 1], kf[1].z, kf[1].w);
           }
         }
 #pragma unroll
@@ -610,16 +627,21 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
         }
       }
       if (t + 1 == t_end) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_empty[stage]);
       ++t;
       ++c.tile;
-      if (++stage == kStages) {
-        stage = 0;
-        phase ^= 1u;
-      }
+      next_stage();
     }
 
     // ---- the end of this CTA's part of the item ----
     const int nrow = min(RT, p.rows - c.rt * RT);
+    const Cursor done = c;
+    const int t_next = t + (c.tile + 1 == c.n ? 1 + kItemCost : 1);
+    if (t_next < t1) {  // the next item's queries, on their way while this one is joined
+      step_cursor<S>(p, c);
+      load_queries();
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       if (dead) l[e] = __int_as_float(0x7fc00000);
@@ -627,7 +649,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
       if (cq == 0) s_m[warp][r0 + 8 * e] = m[e];
     }
-    __syncthreads();  // every warp is done with this tile: its stage becomes the join buffer
+    consumers_sync<32 * W>();  // every warp is done with this tile: its stage becomes the join buffer
     float* buf = reinterpret_cast<float*>(smem + stage * S::kStage);  // [warp][16][HD], 32-byte groups swizzled
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -644,17 +666,17 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
               make_float2(o[n][2 * e] * f, o[n][2 * e + 1] * f);
       }
     }
-    __syncthreads();
-    const int begin = t - c.tile, end = begin + c.n;  // the item's tiles
+    consumers_sync<32 * W>();
+    const int begin = t - done.tile, end = begin + done.n;  // the item's tiles
     const int c0 = begin / per, c1 = (end - 1) / per; // CTAs that share it
     const bool alone = c0 == c1;
     const int slot = blockIdx.x == c0 ? 1 : 0;  // an item that began in an earlier CTA: slot 0
     float* po = p.part_o + (size_t)(blockIdx.x * 2 + slot) * RT * HD;
     float2* pml = p.part_ml + (blockIdx.x * 2 + slot) * RT;
-    const int64_t out0 = ((int64_t)c.b * p.tokens) * p.q_heads + c.h * p.group;
+    const int64_t out0 = ((int64_t)done.b * p.tokens) * p.q_heads + done.h * p.group;
     auto finish = [&](int r, int d, const auto& v, float M, float L) {  // row r, elements d..
       constexpr int N = sizeof(v) / sizeof(float);
-      const int row = c.rt * RT + r, j = token_of(p, row);
+      const int row = done.rt * RT + r, j = token_of(p, row);
       const int64_t at = out0 + (int64_t)j * p.q_heads + row - j * p.group;
       const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
       if (d < p.head_dim) {
@@ -666,10 +688,10 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
       if (d == 0) {
         const float lg = L > 0.f || L != L ? M + log2f(L) : -INFINITY;
         if (p.lse) p.lse[at] = lg * 0.6931471805599453f;
-        if (WEIGHTS) p.lse2[((int64_t)c.b * p.kv_heads + c.h) * p.rows + row] = lg;
+        if (WEIGHTS) p.lse2[((int64_t)done.b * p.kv_heads + done.h) * p.rows + row] = lg;
       }
     };
-    for (int i = tid; i < nrow * (HD / 4); i += S::THREADS) {
+    for (int i = tid; i < nrow * (HD / 4); i += 32 * W) {
       const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
       const int w0 = (r / 16) * WT, rr = r % 16;
       float M = s_m[w0][rr], L = 0.f;
@@ -693,14 +715,14 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
       }
     }
     if (!alone) {
-      __syncthreads();
+      consumers_sync<32 * W>();
       if (tid == 0) {  // one acq_rel add publishes this part and orders the last arriver's reads
         unsigned n;
         asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(p.counters + c0) : "memory");
         s_last = n == static_cast<unsigned>(c1 - c0);
         if (s_last) p.counters[c0] = 0u;
       }
-      __syncthreads();
+      consumers_sync<32 * W>();
       if (s_last) {
         // a warp per row, each lane HD / 32 neighbouring elements
         constexpr int E = HD / 32;
@@ -708,7 +730,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
           float M = -INFINITY, L = 0.f, v[E];
 #pragma unroll
           for (int e = 0; e < E; ++e) v[e] = 0.f;
-          constexpr int U = HD == 256 ? 16 : 40;  // parts whose loads are in flight together
+          constexpr int U = HD == 256 ? 10 : 24;  // parts whose loads are in flight together
           for (int k0 = c0; k0 <= c1; k0 += U) {
             auto part = [&](int k) { return static_cast<size_t>(min(k, c1) * 2 + (k == c0 ? 1 : 0)) * RT + r; };
             float2 ml[2];
@@ -763,14 +785,13 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
         }
       }
     }
+    // the join buffer goes back to the producers
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();  // the join buffer's stage may be filled again
-    t += c.tile + 1 == c.n ? 1 + kItemCost : 1;
-    if (t < t1) step_cursor<S>(p, c);
-    if (++stage == kStages) {
-      stage = 0;
-      phase ^= 1u;
-    }
+    consumers_sync<32 * W>();
+    if (lane == 0) mbar_arrive(&s_empty[stage]);
+    t = t_next;
+    if (t >= t1) return;
+    next_stage();
   }
 }
 
@@ -883,22 +904,22 @@ tp_status encoder(EncodeTiled* out) {
   return TP_OK;
 }
 
-// The pages as a 4-D tensor of boxes of 64 elements x min(16, page_size)
-// tokens; the smaller of the token and head strides comes first.
-tp_status page_map(const tp_paged_cache* c, void* base, bool token_major, int box, CUtensorMap* map) {
+// The pages as a tensor of boxes of min(16, page_size) tokens: all of a token's
+// 64-element panels where they are whole and a box has 16 tokens (it is then
+// the block's layout in shared memory), else one panel, zero-filled past
+// head_dim.
+tp_status page_map(const tp_paged_cache* c, void* base, bool panels, int box, CUtensorMap* map) {
   EncodeTiled encode;
   const tp_status s = encoder(&encode);
   if (s != TP_OK) return s;
   const auto u64 = [](int64_t v) { return static_cast<cuuint64_t>(v); };
-  const cuuint64_t tok_bytes = u64(c->token_stride * 2), head_bytes = u64(c->head_stride * 2);
-  const cuuint64_t dims[4] = {u64(c->head_dim), u64(token_major ? c->kv_heads : c->page_size),
-                              u64(token_major ? c->page_size : c->kv_heads), u64(std::max<int64_t>(1, c->num_pages))};
-  const cuuint64_t strides[3] = {token_major ? head_bytes : tok_bytes, token_major ? tok_bytes : head_bytes,
-                                 u64(c->page_stride * 2)};
-  const cuuint32_t boxes[4] = {64u, token_major ? 1u : static_cast<cuuint32_t>(box),
-                               token_major ? static_cast<cuuint32_t>(box) : 1u, 1u};
-  const cuuint32_t ones[4] = {1u, 1u, 1u, 1u};
-  const CUresult r = encode(map, c->dtype == TP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+  const cuuint32_t np = panels ? static_cast<cuuint32_t>(c->head_dim / 64) : 1u;
+  const cuuint64_t dims[5] = {panels ? u64(64) : u64(c->head_dim), u64(c->page_size), np, u64(c->kv_heads),
+                              u64(std::max<int64_t>(1, c->num_pages))};
+  const cuuint64_t strides[4] = {u64(c->token_stride * 2), 128, u64(c->head_stride * 2), u64(c->page_stride * 2)};
+  const cuuint32_t boxes[5] = {64u, static_cast<cuuint32_t>(box), np, 1u, 1u};
+  const cuuint32_t ones[5] = {1u, 1u, 1u, 1u, 1u};
+  const CUresult r = encode(map, c->dtype == TP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                             base, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
@@ -983,11 +1004,11 @@ TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_ca
     return fail(TP_ERR_WORKSPACE, "tp_paged_attn: workspace missing, not 256-byte aligned or smaller than %lld bytes",
                 (long long)pl.bytes);
   AttnParams p{};
-  p.token_major = cache->head_stride < cache->token_stride;
   const int box = std::min(16, cache->page_size);
   p.lg_box = log2_int(box);
-  s = page_map(cache, cache->k_pages, p.token_major, box, &p.k_map);
-  if (s == TP_OK) s = page_map(cache, cache->v_pages, p.token_major, box, &p.v_map);
+  p.panels = box == 16 && cache->head_dim == pl.hd;
+  s = page_map(cache, cache->k_pages, p.panels, box, &p.k_map);
+  if (s == TP_OK) s = page_map(cache, cache->v_pages, p.panels, box, &p.v_map);
   if (s != TP_OK) return s;
   p.q = a.q;
   p.out = a.out;
