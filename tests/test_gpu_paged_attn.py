@@ -188,6 +188,24 @@ def test_streams_and_graph():
         torch.cuda.synchronize()
 
 
+def test_lengths_changed_between_calls():
+    """Lengths written by the kernel just before the call count in both of its launches."""
+    cache, g = _cache([640, 640, 640], 1, 2, 128, 16, torch.float16, 9, track=True)
+    q = torch.randn(3, 1, 8, 128, generator=g, device=DEV).half()
+    lens = torch.randint(0, 640, (40, 3), generator=g, device=DEV, dtype=torch.int32)
+    cache.attend(q, accumulate=True)
+    torch.cuda.synchronize()
+    sums = []
+    for i in range(len(lens)):
+        cache.scores.zero_()
+        cache.lengths.copy_(lens[i])
+        cache.attend(q, accumulate=True)
+        sums.append((cache.scores[0].sum(-1), (cache.scores[0] > 0).sum(-1)))
+    for i, (weight, count) in enumerate(sums):
+        assert float((weight - 4).abs().max()) < 1e-3  # four rows of weight one on each kv head
+        assert (count <= lens[i][:, None] + 1).all()
+
+
 def test_refusals():
     from turbopress_b200 import _abi
     from turbopress_b200.paged import PagedKVCache

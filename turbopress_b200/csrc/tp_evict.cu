@@ -72,6 +72,7 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const __gri
   __shared__ uint32_t s_pick[2];
   __shared__ int s_tmp[kEvWarps];
   pdl_trigger();
+  pdl_wait();
   const int b = blockIdx.y, h = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t bh = (int64_t)b * p.kv_heads + h;
@@ -186,6 +187,7 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const __gri
 
 // One row (K and V of a slot) per group of head_dim / 8 lanes.
 __global__ void __launch_bounds__(kMvThreads) evict_move_kernel(const __grid_constant__ EvictParams p, int lg_lanes) {
+  pdl_trigger();
   pdl_wait();
   const int64_t bh = blockIdx.y;
   const int b = static_cast<int>(bh / p.kv_heads), h = static_cast<int>(bh - (int64_t)b * p.kv_heads);
@@ -277,8 +279,7 @@ TP_API tp_status tp_cache_evict(const tp_evict_args* args, const tp_paged_cache*
   static int smem_set[64];
   s = ensure_smem(evict_select_kernel, smem, smem_set, "evict: shared memory attribute");
   if (s != TP_OK) return s;
-  evict_select_kernel<<<dim3(cache->kv_heads, cache->batch), kEvThreads, smem, st>>>(p);
-  s = check_launch("evict_select launch");
+  s = launch_early(evict_select_kernel, dim3(cache->kv_heads, cache->batch), kEvThreads, smem, st, "evict_select launch", p);
   if (s != TP_OK || max_moves == 0) return s;
   int sms = 0;
   s = device_sms(&sms);
@@ -287,17 +288,8 @@ TP_API tp_status tp_cache_evict(const tp_evict_args* args, const tp_paged_cache*
   const int rows = kMvThreads >> lg_lanes;
   // about eight CTAs per SM in all, never more than the rows that may move
   const int64_t per_head = std::max<int64_t>(1, std::min<int64_t>((max_moves + rows - 1) / rows, (8 * sms + heads - 1) / heads));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(per_head), heads);
-  cfg.blockDim = dim3(kMvThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_move_kernel, p, lg_lanes), "evict_move launch");
-  return clear_ok();
+  return launch_early(evict_move_kernel, dim3(static_cast<unsigned>(per_head), heads), kMvThreads, 0, st, "evict_move launch",
+                      p, lg_lanes);
 }
 
 }  // extern "C"

@@ -50,6 +50,26 @@ inline tp_status device_sms(int* sms) {
   return TP_OK;
 }
 
+// Launch that may begin while the kernel before it in the stream ends: every
+// kernel launched this way waits (griddepcontrol.wait) for that kernel's
+// completion before its first access to memory that others write.
+template <class... Params, class... Args>
+inline tp_status launch_early(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+                              const char* what, const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+  return clear_ok();
+}
+
 // N neighbouring elements, accessed 16 bytes at a time at most.
 template <class T, int VEC>
 struct alignas(VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16) Pack {

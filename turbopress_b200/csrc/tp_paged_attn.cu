@@ -314,7 +314,8 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
   // ---- this CTA's run [t0, t1) of the index space ----
   int per, t0, t1, before;
   Cursor c;
-  if (WEIGHTS) pdl_trigger();
+  pdl_wait();
+  pdl_trigger();  // after the wait: the weights kernel reads the lengths at once
   // (its barriers also publish the mbarriers)
   if (!find_share<W + 4>(p, [&](int len) { return seq_size<S>(p, len); }, s_tmp, per, t0, t1, c.b, c.len, before)) return;
   int rem = t0 - before;
@@ -804,16 +805,22 @@ template <class S>
 __global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_constant__ AttnParams p) {
   constexpr int W = kWtThreads / 32, RT = S::RT, TILE = S::TILE;
   __shared__ int s_tmp[W + 4];
-  pdl_wait();
+  pdl_trigger();
+  // The lengths are as old as the attention kernel's own inputs, which it had
+  // waited for before it let this one begin.
   const int last = p.row_tiles - 1;
   auto count = [&](int len) { return p.kv_heads * item_tiles<S>(p, len, last); };
   int per, t0, t1, b, len, before;
   if (!find_share<W>(p, count, s_tmp, per, t0, t1, b, len, before)) return;
   // positions of the attention kernel's index space before sequence b
-  int c1 = 0;
-  for (int i = threadIdx.x; i < b; i += kWtThreads) c1 += seq_size<S>(p, p.lengths[i]);
-  int base = block_sum<W>(c1, s_tmp);
+  int base = before + b * p.kv_heads * kItemCost;
+  if (last > 0) {
+    int c1 = 0;
+    for (int i = threadIdx.x; i < b; i += kWtThreads) c1 += seq_size<S>(p, p.lengths[i]);
+    base = block_sum<W>(c1, s_tmp);
+  }
   int n = item_tiles<S>(p, len, last);
+  pdl_wait();
   const int sub = threadIdx.x / TILE, tok = threadIdx.x % TILE;
   for (int t = t0 + sub; t < t1; t += kWtThreads / TILE) {
     while (t - before >= p.kv_heads * n) {
@@ -825,6 +832,8 @@ __global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_
     const int h = (t - before) / n, tile = (t - before) - h * n;
     const int slot = tile * TILE + tok;
     if (slot >= visible(p, len, p.rows - 1)) continue;
+    float* score = p.scores + ((int64_t)b * p.kv_heads + h) * p.capacity + slot;
+    const float was = *score;
     float w = 0.f;
     int off = base;
     for (int rt = 0; rt <= last; ++rt) {
@@ -833,12 +842,12 @@ __global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_
         const float* s = p.sbuf + (size_t)(off + h * (kItemCost + nt) + kItemCost + tile) * RT * TILE + tok;
         const float* z = p.lse2 + ((int64_t)b * p.kv_heads + h) * p.rows + rt * RT;
         const int rows = min(RT, p.rows - rt * RT);
-#pragma unroll 4
+#pragma unroll 8
         for (int r = 0; r < rows; ++r) w += exp2_diff(s[r * TILE], z[r]);
       }
       off += p.kv_heads * (kItemCost + nt);
     }
-    p.scores[((int64_t)b * p.kv_heads + h) * p.capacity + slot] += w;
+    *score = was + w;
   }
 }
 
@@ -947,20 +956,10 @@ tp_status launch_attn(const AttnParams& p, const PaPlan& pl, bool weights, cudaS
     __atomic_store_n(&ctas[weights][dev], occ, __ATOMIC_RELAXED);
   }
   const int grid = static_cast<int>(std::min<int64_t>(std::min(kPaMaxCtas, sms * occ), pl.positions));
-  kern<<<grid, S::THREADS, S::kSmem, st>>>(p);
-  s = check_launch("paged_attn launch");
+  s = launch_early(kern, dim3(grid), S::THREADS, S::kSmem, st, "paged_attn launch", p);
   if (s != TP_OK || !weights) return s;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(8 * sms, pl.max_tiles)));
-  cfg.blockDim = dim3(kWtThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_weights_kernel<S>, p), "paged_weights launch");
-  return clear_ok();
+  return launch_early(paged_weights_kernel<S>, dim3(static_cast<unsigned>(std::min<int64_t>(8 * sms, pl.max_tiles))),
+                      kWtThreads, 0, st, "paged_weights launch", p);
 }
 
 template <class T, int HD>

@@ -18,6 +18,7 @@
 // reduction and q, k can be turned in place.
 #include <algorithm>
 
+#include "tp_decode.cuh"
 #include "tp_paged.cuh"
 
 using namespace tp;
@@ -62,6 +63,8 @@ template <class T, int VEC, int UPL>
 __global__ void __launch_bounds__(kRtThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
   extern __shared__ float2 cs[];  // [tpc][rot/2]
   __shared__ int64_t s_dst[kRtMaxTokens];
+  pdl_trigger();
+  pdl_wait();
   const int tid = threadIdx.x;
   const int64_t tok0 = (int64_t)blockIdx.x * p.tpc;
   const int nt = static_cast<int>(min((int64_t)p.tpc, p.a.tokens - tok0));
@@ -261,8 +264,8 @@ tp_status launch_rotary(RotaryParams& p, cudaStream_t st) {
   const int64_t grid = (p.a.tokens + p.tpc - 1) / p.tpc;
   if (grid > 0x7FFFFFFF) return fail(TP_ERR_UNSUPPORTED, "tp_rotary: too many tokens");
   const int smem = p.tpc * (p.a.rot_dim / 2) * static_cast<int>(sizeof(float2));
-  rotary_kernel<T, VEC, UPL><<<dim3(static_cast<unsigned>(grid), split), kRtThreads, smem, st>>>(p);
-  return check_launch("rotary launch");
+  return launch_early(rotary_kernel<T, VEC, UPL>, dim3(static_cast<unsigned>(grid), split), kRtThreads, smem, st,
+                      "rotary launch", p);
 }
 
 template <class T>

@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const __grid_co
   __shared__ float s_rm[kVfMaxRows], s_rl[kVfMaxRows];
   __shared__ unsigned s_arg[kVfMaxRows];
   pdl_trigger();
+  pdl_wait();
   const int rows = p.a.drafts + 1;
   const int b = blockIdx.y / rows, k = blockIdx.y - b * rows;
   const int used = p.a.counts ? max(0, min(p.a.counts[b], p.a.drafts)) : p.a.drafts;
@@ -259,6 +260,7 @@ template <class T>
 __global__ void __launch_bounds__(kVfThreads) verify_race_kernel(const __grid_constant__ VerifyParams p) {
   __shared__ unsigned long long s_k[2][kVfWarps];
   __shared__ bool s_last;
+  pdl_trigger();
   pdl_wait();
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Choice ch = p.choice[b];
@@ -348,20 +350,9 @@ tp_status launch_verify(VerifyParams& p, cudaStream_t st) {
   };
   p.splits = slices(rows);
   p.race_splits = slices(p.a.batch);
-  verify_rows_kernel<T><<<dim3(p.splits, rows), kVfThreads, 0, st>>>(p);
-  s = check_launch("verify_rows launch");
+  s = launch_early(verify_rows_kernel<T>, dim3(p.splits, rows), kVfThreads, 0, st, "verify_rows launch", p);
   if (s != TP_OK || !p.a.temperature) return s;  // all greedy: the tokens are written
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.race_splits, p.a.batch);
-  cfg.blockDim = dim3(kVfThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  TP_CUDA_TRY(cudaLaunchKernelEx(&cfg, verify_race_kernel<T>, p), "verify_race launch");
-  return clear_ok();
+  return launch_early(verify_race_kernel<T>, dim3(p.race_splits, p.a.batch), kVfThreads, 0, st, "verify_race launch", p);
 }
 
 }  // namespace

@@ -176,7 +176,7 @@ class PagedKVCache:
                 self._plans.clear()
             self._plans[key] = plan
         addr = self._layer(layer)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
         if plan.tokens:
             q = q.contiguous()

@@ -144,7 +144,7 @@ class Rotary:
             self._plans[key] = plan
         if positions is not None:
             positions = positions.to(torch.int64).contiguous()
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         a = _RotaryArgs.from_buffer_copy(plan)
         a.q, a.k, a.q_out, a.inverse, a.eps = q.data_ptr(), k.data_ptr(), out.data_ptr(), inverse, eps
         if v is not None:
@@ -200,7 +200,7 @@ class Rotary:
         if positions is None:
             raise ValueError("positions are needed")
         a, q_out, keep = self._args(q, k, None, positions, q_norm, k_norm, eps, inverse)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         a.k_out = k_out.data_ptr()
         _abi.launch(_abi.lib().tp_rotary, "rotary", self.device.index, ctypes.addressof(a), None)
         return q_out, k_out
