@@ -26,11 +26,13 @@ namespace {
 
 constexpr int kVfThreads = 256;
 constexpr int kVfWarps = kVfThreads / 32;
+constexpr int kVfResident = 6;    // CTAs per SM
 constexpr int kVfMaxRows = 64;    // drafts + 1
 constexpr int kVfMaxSplits = 128;
 
 struct Part {  // one slice of a row
-  float m, l;               // sampled: maximum and sum of 2^((x - m) c)
+  float m, l;               // sampled: maximum and sum of 2^((x - m) c),
+  float draft, need;        // in slice 0 the draft's logit and uniform * q (infinite for a draft that cannot stand)
   unsigned long long key;   // greedy: argmax key
 };
 
@@ -45,7 +47,7 @@ struct VerifyParams {
   int splits, race_splits;
   Part* part;                 // [batch][rows][splits]
   Choice* choice;             // [batch]
-  unsigned long long* key;    // [batch][2]: race over the residual, over p
+  unsigned long long* key;    // [batch]: the race's leader
   unsigned* done;             // [batch][2]: CTAs that have arrived
 };
 
@@ -71,10 +73,11 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
   return k;
 }
 
-// f(i, x_i) for the elements [lo, hi) of a row that fall to this thread, in
-// ascending order: 16-byte vectors of the aligned middle, single elements at
-// ragged ends.
-template <class T, class F, class G>
+// Elements [lo, hi) of a row that fall to this thread, in ascending order:
+// vec(i, w) for U 16-byte vectors of the aligned middle (vector u at
+// i + u * kVfThreads vectors) or one, each(i, x) for single elements at ragged
+// ends.
+template <int U, class T, class F, class G>
 __device__ __forceinline__ void for_slice(const T* row, int lo, int hi, F each, G vec) {
   constexpr int V = 16 / sizeof(T);
   const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
@@ -83,27 +86,99 @@ __device__ __forceinline__ void for_slice(const T* row, int lo, int hi, F each, 
   const int nvec = (hi - head) / V;
   const uint4* mid = reinterpret_cast<const uint4*>(row + head);
   int i = threadIdx.x;
-  for (; i + 3 * kVfThreads < nvec; i += 4 * kVfThreads) {
-    uint4 w[4];
+  if constexpr (U > 1) {
+    for (; i + (U - 1) * kVfThreads < nvec; i += U * kVfThreads) {
+      uint4 w[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) w[u] = __ldg(mid + i + u * kVfThreads);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      float x[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) x[e] = Elem<T>::to(reinterpret_cast<const T*>(&w[u])[e]);
-      vec(head + (i + u * kVfThreads) * V, x);
+      for (int u = 0; u < U; ++u) w[u] = __ldg(mid + i + u * kVfThreads);
+      vec(head + i * V, w);
     }
   }
   for (; i < nvec; i += kVfThreads) {
-    const uint4 w = __ldg(mid + i);
-    float x[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = Elem<T>::to(reinterpret_cast<const T*>(&w)[e]);
-    vec(head + i * V, x);
+    const uint4 w[1] = {__ldg(mid + i)};
+    vec(head + i * V, w);
   }
   const int tail = head + nvec * V + threadIdx.x;
   if (tail < hi) each(tail, Elem<T>::to(row[tail]));
+}
+
+// Two neighbouring elements of a vector's word pair w[e].
+template <class T>
+struct Two;
+template <>
+struct Two<__half> {
+  static __device__ __forceinline__ float2 at(const uint4& w, int e) {
+    return __half22float2(reinterpret_cast<const __half2*>(&w)[e]);
+  }
+  template <int N>
+  static __device__ __forceinline__ float largest(const uint4 (&w)[N]) {
+    const __half2* h = reinterpret_cast<const __half2*>(w);
+    __half2 x = h[0];
+#pragma unroll
+    for (int e = 1; e < 4 * N; ++e) x = __hmax2(x, h[e]);
+    const float2 f = __half22float2(x);
+    return fmaxf(f.x, f.y);
+  }
+};
+template <>
+struct Two<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 at(const uint4& w, int e) {
+    return __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&w)[e]);
+  }
+  template <int N>
+  static __device__ __forceinline__ float largest(const uint4 (&w)[N]) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+    __nv_bfloat162 x = h[0];
+#pragma unroll
+    for (int e = 1; e < 4 * N; ++e) x = __hmax2(x, h[e]);
+    const float2 f = __bfloat1622float2(x);
+    return fmaxf(f.x, f.y);
+  }
+};
+template <>
+struct Two<float> {
+  static __device__ __forceinline__ float2 at(const uint4& w, int e) { return reinterpret_cast<const float2*>(&w)[e]; }
+  template <int N>
+  static __device__ __forceinline__ float largest(const uint4 (&w)[N]) {
+    const float* f = reinterpret_cast<const float*>(w);
+    float x = f[0];
+#pragma unroll
+    for (int e = 1; e < 4 * N; ++e) x = fmaxf(x, f[e]);
+    return x;
+  }
+};
+
+// Packed fp32 pairs (one instruction for two elements).
+__device__ __forceinline__ uint64_t pack2(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// 2^x to 2 ulp; below 2^-126 it gives 0, which no sum or comparison here notices.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // Joins two (m, l) with 2^((x - m) c) terms.
@@ -115,7 +190,7 @@ __device__ __forceinline__ void join(float& m, float& l, float m2, float l2, flo
 }
 
 template <class T>
-__global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const __grid_constant__ VerifyParams p) {
+__global__ void __launch_bounds__(kVfThreads, kVfResident) verify_rows_kernel(const __grid_constant__ VerifyParams p) {
   __shared__ float s_m[kVfWarps], s_l[kVfWarps];
   __shared__ unsigned long long s_k[kVfWarps];
   __shared__ bool s_last;
@@ -136,6 +211,17 @@ __global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const __grid_co
   const int per = (p.a.vocab + p.splits - 1) / p.splits;
   const int lo = min((int)blockIdx.x * per, p.a.vocab), hi = min(lo + per, p.a.vocab);
 
+  // what decides on the row's draft, fetched while the row streams
+  float draft = 0.f, need = INFINITY;
+  if (blockIdx.x == 0 && tid == 0 && k < used && !greedy) {
+    const int64_t d = p.a.draft_tokens[(int64_t)b * p.a.drafts + k];
+    if (d >= 0 && d < p.a.vocab) {
+      const float qd = p.a.draft_probs ? p.a.draft_probs[((int64_t)b * p.a.drafts + k) * p.a.vocab + d] : 1.f;
+      draft = Elem<T>::to(row[d]);
+      need = p.a.uniforms[(int64_t)b * p.a.drafts + k] * qd;
+    }
+  }
+
   float m = -INFINITY, l = 0.f;
   unsigned long long best = 0ull;
   if (greedy) {
@@ -147,34 +233,51 @@ __global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const __grid_co
         at = i;
       }
     };
-    constexpr int V = 16 / sizeof(T);
-    for_slice<T>(row, lo, hi, one, [&](int i, const float (&x)[V]) {
+    for_slice<4>(row, lo, hi, one, [&](int i, const auto& w) {
+      constexpr int N = sizeof(w) / 16, V = 16 / sizeof(T);
 #pragma unroll
-      for (int e = 0; e < V; ++e) one(i + e, x[e]);
+      for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          const float2 x = Two<T>::at(w[u], e / 2);
+          one(i + u * kVfThreads * V + e, x.x);
+          one(i + u * kVfThreads * V + e + 1, x.y);
+        }
     });
     if (at >= 0) best = argmax_key(top, at);
   } else {
+    // Elements two at a time: 2^(x c - m c), the sum in four parts.  (Rounding
+    // m c scales a thread's sum by 2^-24 |m c| at most, 1e-6.)
+    uint64_t sum[2] = {0ull, 0ull}, mc2 = 0ull;
+    const uint64_t c2 = pack2(make_float2(c, c));
+    auto raise = [&](float t) {  // to a new maximum
+      const float f = m == -INFINITY ? 0.f : exp2f((m - t) * c);
+      l *= f;
+      const uint64_t f2 = pack2(make_float2(f, f));
+      sum[0] = mul2(sum[0], f2);
+      sum[1] = mul2(sum[1], f2);
+      m = t;
+      mc2 = pack2(make_float2(-t * c, -t * c));
+    };
     auto one = [&](int, float x) {
       if (x == -INFINITY) return;
-      if (x > m) {
-        l *= m == -INFINITY ? 0.f : exp2f((m - x) * c);
-        m = x;
-      }
+      if (x > m) raise(x);
       l += exp2f((x - m) * c);
     };
-    constexpr int V = 16 / sizeof(T);
-    for_slice<T>(row, lo, hi, one, [&](int, const float (&x)[V]) {
-      float t = x[0];
+    for_slice<4>(row, lo, hi, one, [&](int, const auto& w) {
+      constexpr int N = sizeof(w) / 16;
+      const float t = Two<T>::largest(w);
+      if (t > m) raise(t);
 #pragma unroll
-      for (int e = 1; e < V; ++e) t = fmaxf(t, x[e]);
-      if (t > m) {
-        l *= m == -INFINITY ? 0.f : exp2f((m - t) * c);
-        m = t;
-      }
-      const float base = m == -INFINITY ? 0.f : m;
+      for (int u = 0; u < N; ++u)
 #pragma unroll
-      for (int e = 0; e < V; ++e) l += exp2f((x[e] - base) * c);
+        for (int e = 0; e < 8 / (int)sizeof(T); ++e) {
+          const float2 y = unpack2(fma2(pack2(Two<T>::at(w[u], e)), c2, mc2));
+          sum[e & 1] = add2(sum[e & 1], pack2(make_float2(exp2_fast(y.x), exp2_fast(y.y))));
+        }
     });
+    const float2 s = unpack2(add2(sum[0], sum[1]));
+    l += s.x + s.y;
   }
   if (greedy) {
     best = warp_max(best);
@@ -192,7 +295,7 @@ __global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const __grid_co
   }
   __syncthreads();
   if (tid == 0) {
-    Part out{-INFINITY, 0.f, 0ull};
+    Part out{-INFINITY, 0.f, draft, need, 0ull};
     for (int w = 0; w < kVfWarps; ++w) {
       if (greedy) out.key = s_k[w] > out.key ? s_k[w] : out.key;
       else join(out.m, out.l, s_m[w], s_l[w], c);
@@ -212,6 +315,7 @@ __global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const __grid_co
     const Part* q = p.part + ((int64_t)b * rows + r) * p.splits;
     float rm = -INFINITY, rl = 0.f;
     unsigned long long rk = 0ull;
+    const float draft_r = __ldcg(&q[0].draft), need_r = __ldcg(&q[0].need);
     for (int i = lane; i < p.splits; i += 32) {
       const float qm = __ldcg(&q[i].m), ql = __ldcg(&q[i].l);
       const unsigned long long qk = __ldcg(&q[i].key);
@@ -228,18 +332,8 @@ __global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const __grid_co
       s_rm[r] = rm;
       s_rl[r] = rl;
       s_arg[r] = key_index(rk);
-      if (r < used) {
-        const int64_t d = drafts[r];
-        bool ok = d >= 0 && d < p.a.vocab;
-        if (ok && greedy) ok = d == (int64_t)key_index(rk);
-        if (ok && !greedy) {
-          const T* x = static_cast<const T*>(p.a.logits) + (int64_t)b * p.a.batch_stride + (int64_t)r * p.a.row_stride;
-          const float pd = exp2f((Elem<T>::to(x[d]) - rm) * c) / rl;
-          const float qd = p.a.draft_probs ? p.a.draft_probs[((int64_t)b * p.a.drafts + r) * p.a.vocab + d] : 1.f;
-          ok = p.a.uniforms[(int64_t)b * p.a.drafts + r] * qd < pd;
-        }
-        s_ok[r] = ok;
-      }
+      if (r < used)  // an infinite need (and NaN) never stands
+        s_ok[r] = greedy ? drafts[r] == (int64_t)key_index(rk) : need_r < exp2f((draft_r - rm) * c) / rl;
     }
   }
   __syncthreads();
@@ -256,13 +350,49 @@ __global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const __grid_co
   }
 }
 
+// Largest key of the block, in every thread.
+__device__ __forceinline__ unsigned long long block_max(unsigned long long k, unsigned long long* s_k) {
+  k = warp_max(k);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s_k[threadIdx.x >> 5] = k;
+  __syncthreads();
+  k = s_k[0];
+#pragma unroll
+  for (int w = 1; w < kVfWarps; ++w) k = s_k[w] > k ? s_k[w] : k;
+  return k;
+}
+// *at, in every thread of the block, and 0 in its place.
+__device__ __forceinline__ unsigned long long take_key(unsigned long long* at, unsigned long long* s_k) {
+  __syncthreads();
+  if (threadIdx.x == 0) s_k[0] = atomicExch(at, 0ull);
+  __syncthreads();
+  return s_k[0];
+}
+// N neighbouring floats, 16 bytes at a time where the address allows.
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float (&v)[N]) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(p + i));
+      v[i] = x.x;
+      v[i + 1] = x.y;
+      v[i + 2] = x.z;
+      v[i + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __ldg(p + i);
+  }
+}
+
 template <class T>
-__global__ void __launch_bounds__(kVfThreads) verify_race_kernel(const __grid_constant__ VerifyParams p) {
-  __shared__ unsigned long long s_k[2][kVfWarps];
+__global__ void __launch_bounds__(kVfThreads, kVfResident) verify_race_kernel(const __grid_constant__ VerifyParams p) {
+  __shared__ unsigned long long s_k[kVfWarps];
   __shared__ bool s_last;
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = blockIdx.y, tid = threadIdx.x;
   const Choice ch = p.choice[b];
   if (ch.row < 0) return;
   const T* row = static_cast<const T*>(p.a.logits) + (int64_t)b * p.a.batch_stride + (int64_t)ch.row * p.a.row_stride;
@@ -273,48 +403,78 @@ __global__ void __launch_bounds__(kVfThreads) verify_race_kernel(const __grid_co
   const int64_t hot = ch.residual && !q ? p.a.draft_tokens[(int64_t)b * p.a.drafts + ch.row] : -1;
   const int per = (p.a.vocab + p.race_splits - 1) / p.race_splits;
   const int lo = min((int)blockIdx.x * per, p.a.vocab), hi = min(lo + per, p.a.vocab);
-  float bt[2] = {0.f, 0.f};  // largest r / e and p / e, and where
-  int at[2] = {-1, -1};
-  auto one = [&](int i, float x) {
-    const float pi = exp2f((x - ch.m) * ch.c) * ch.inv_l, e = noise[i];
-    const float qi = q ? q[i] : i == hot ? 1.f : 0.f;
-    const float r = fmaxf(pi - qi, 0.f) / e, f = pi / e;
-    if (r > bt[0]) {
-      bt[0] = r;
-      at[0] = i;
-    }
-    if (f > bt[1]) {
-      bt[1] = f;
-      at[1] = i;
+  float top = 0.f;  // the largest r / e, and where
+  int at = -1;
+  auto chance = [&](float x) { return exp2f((x - ch.m) * ch.c) * ch.inv_l; };
+  auto enter = [&](int i, float r, float e) {  // the exact quotient
+    const float f = r / e;
+    if (f > top) {
+      top = f;
+      at = i;
     }
   };
+  auto one = [&](int i, float x) {
+    const float qi = q ? q[i] : i == hot ? 1.f : 0.f;
+    enter(i, fmaxf(chance(x) - qi, 0.f), noise[i]);
+  };
   constexpr int V = 16 / sizeof(T);
-  for_slice<T>(row, lo, hi, one, [&](int i, const float (&x)[V]) {
+  for_slice<1>(row, lo, hi, one, [&](int i, const uint4 (&w)[1]) {
+    float e[V], r[V];
+    if (q) {
+      load_floats<V>(q + i, r);
+    } else {
 #pragma unroll
-    for (int e = 0; e < V; ++e) one(i + e, x[e]);
-  });
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const unsigned long long k = warp_max(at[w] >= 0 ? argmax_key(bt[w], at[w]) : 0ull);
-    if (lane == 0) s_k[w][warp] = k;
-  }
-  __syncthreads();
-  if (tid < 2) {
-    unsigned long long k = 0ull;
-    for (int w = 0; w < kVfWarps; ++w) k = s_k[tid][w] > k ? s_k[tid][w] : k;
-    if (k) atomicMax(&p.key[2 * b + tid], k);
-    __threadfence();
-  }
-  __syncthreads();
-  if (tid == 0) {
-    s_last = atomicAdd(&p.done[2 * b + 1], 1u) == gridDim.x - 1;
-    if (s_last) {
-      __threadfence();
-      const unsigned long long r = atomicExch(&p.key[2 * b], 0ull), f = atomicExch(&p.key[2 * b + 1], 0ull);
-      const unsigned long long k = r ? r : f;
-      p.a.tokens[(int64_t)b * (p.a.drafts + 1) + ch.row] = k ? (int64_t)key_index(k) : -1;
-      p.done[2 * b + 1] = 0u;
+      for (int k = 0; k < V; ++k) r[k] = i + k == hot ? 1.f : 0.f;
     }
+    load_floats<V>(noise + i, e);
+    // The exact divisions are for quotients near the vector's largest, if that
+    // is near the best or above; where the largest is below 1e-30 (no
+    // approximation holds there), for all.
+    float near = 0.f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float2 x = Two<T>::at(w[0], k / 2);
+      r[k] = fmaxf(exp2_fast(((k & 1 ? x.y : x.x) - ch.m) * ch.c) * ch.inv_l - r[k], 0.f);
+      float inv;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(e[k]));
+      e[k] = r[k] * inv;
+      near = fmaxf(near, e[k]);
+    }
+    if (near >= top * 0.999f || top < 1e-30f) {
+      unsigned some = 0;
+#pragma unroll
+      for (int k = 0; k < V; ++k) some |= (near < 1e-30f ? r[k] > 0.f : e[k] >= near * 0.999f) ? 1u << k : 0u;
+      for (; some; some &= some - 1) {
+        const int k = __ffs(some) - 1;
+        one(i + k, Elem<T>::to(row[i + k]));
+      }
+    }
+  });
+  const unsigned long long key = block_max(at >= 0 ? argmax_key(top, at) : 0ull, s_k);
+  if (tid == 0) {
+    if (key) atomicMax(&p.key[b], key);
+    __threadfence();
+    s_last = atomicAdd(&p.done[2 * b + 1], 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  // The last CTA of the sequence.  Nothing left of p - q anywhere (q is not
+  // normalised): the draw is from p, by this CTA alone, since it hardly occurs.
+  unsigned long long won = take_key(&p.key[b], s_k);
+  if (!won && ch.residual) {
+    top = 0.f;
+    at = -1;
+    auto whole = [&](int i, float x) { enter(i, chance(x), noise[i]); };
+    for_slice<1>(row, 0, p.a.vocab, whole, [&](int i, const uint4 (&w)[1]) {
+#pragma unroll 1
+      for (int k = 0; k < V; ++k) whole(i + k, Elem<T>::to(row[i + k]));
+    });
+    won = block_max(at >= 0 ? argmax_key(top, at) : 0ull, s_k);
+  }
+  if (tid == 0) {
+    p.a.tokens[(int64_t)b * (p.a.drafts + 1) + ch.row] = won ? (int64_t)key_index(won) : -1;
+    p.done[2 * b + 1] = 0u;
   }
 }
 
@@ -331,7 +491,7 @@ tp_status plan_verify(int64_t batch, int64_t drafts, int64_t vocab, VfPlan* pl) 
   if (vocab > 0x7FFFFFF0) return fail(TP_ERR_UNSUPPORTED, "tp_verify_drafts: vocabulary too large");
   // counters and keys of up to 65535 sequences at a fixed place, so that calls
   // of other sizes find them zero
-  pl->choice_off = round256(65536 * (2 * 4 + 2 * 8));
+  pl->choice_off = round256(65536 * (8 + 2 * 4));
   pl->part_off = pl->choice_off + round256(batch * (int64_t)sizeof(Choice));
   pl->bytes = pl->part_off + round256(batch * (drafts + 1) * kVfMaxSplits * (int64_t)sizeof(Part));
   return TP_OK;
@@ -343,10 +503,11 @@ tp_status launch_verify(VerifyParams& p, cudaStream_t st) {
   tp_status s = device_sms(&sms);
   if (s != TP_OK) return s;
   const int rows = p.a.batch * (p.a.drafts + 1);
-  // slices: about eight CTAs per SM in all, at least 1024 elements each
+  // slices: all CTAs resident at once, 4096 elements each at
+  // least (16 a thread): more and smaller ones cost more in the joins
   auto slices = [&](int n) {
-    const int64_t most = (p.a.vocab + 1023) / 1024;
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({(8 * sms + n - 1) / n, most, kVfMaxSplits})));
+    const int64_t most = (p.a.vocab + 4095) / 4096;
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kVfResident * sms / n, most, kVfMaxSplits})));
   };
   p.splits = slices(rows);
   p.race_splits = slices(p.a.batch);
@@ -384,7 +545,7 @@ TP_API tp_status tp_verify_drafts(const tp_verify_args* args, void* workspace, i
   p.a = a;
   auto* ws = static_cast<unsigned char*>(workspace);
   p.key = reinterpret_cast<unsigned long long*>(ws);
-  p.done = reinterpret_cast<unsigned*>(ws + 65536 * 16);
+  p.done = reinterpret_cast<unsigned*>(ws + 65536 * 8);
   p.choice = reinterpret_cast<Choice*>(ws + pl.choice_off);
   p.part = reinterpret_cast<Part*>(ws + pl.part_off);
   cudaStream_t st = as_stream(stream);
