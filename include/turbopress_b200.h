@@ -526,7 +526,7 @@ typedef struct tp_evict_args {
 } tp_evict_args;
 
 /* Workspace (no zero-fill needed; one per stream); minus the status on bad
- * arguments, TP_ERR_UNSUPPORTED above 2^20 slots per sequence. */
+ * arguments, TP_ERR_UNSUPPORTED above 2^19 slots per sequence. */
 TP_API int64_t tp_cache_evict_workspace_bytes(const tp_paged_cache* cache, int budget);
 TP_API tp_status tp_cache_evict(const tp_evict_args* args, const tp_paged_cache* cache, void* workspace,
                                 int64_t workspace_bytes, void* stream);

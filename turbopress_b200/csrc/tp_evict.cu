@@ -3,8 +3,8 @@
 // Mathematics: the `budget` largest of n keys per (sequence, kv head), a key
 // being the score's order-preserving 32-bit image (guarded slots above all,
 // the lower slot first on equality).  A radix selection finds the budget-th
-// key in three counting passes over 11, 11 and 10 bits; one ordered pass marks
-// the kept slots.  With the kept slots above the budget s_0 < s_1 < ... and the
+// key in three counting passes over 11, 11 and 10 bits; one ordered pass over
+// bit words (a thread per 32 slots) marks the kept slots.  With the kept slots above the budget s_0 < s_1 < ... and the
 // freed ones below it h_0 < h_1 < ..., slot s_i moves to h_i: as many rows as
 // must move, every source at or above the budget and every destination below
 // it, so the moves are independent of each other.
@@ -23,12 +23,12 @@ using namespace tp;
 
 namespace {
 
-constexpr int kEvThreads = 1024;
-constexpr int kEvWarps = kEvThreads / 32;
-constexpr int kEvMaxSlots = 1 << 20;
+constexpr int kEvMaxSlots = 1 << 19;
 constexpr int kEvCached = 40960;   // slots whose keys fit in shared memory
 constexpr int kEvBins = 2048;
-constexpr int kEvCopies = 4;        // of the histogram: fewer collisions
+// Threads of the selection: few where few slots are (its barriers cost less).
+// EVTHREADS
+constexpr int kEvSmall = 2048;      // capacity up to which 256 threads do
 constexpr int kMvThreads = 256;
 constexpr int kMvRows = 4;          // rows in flight per group of lanes
 // Moves per head up to which the selecting CTA does them itself.  EVNOTE
@@ -60,17 +60,32 @@ __device__ __forceinline__ uint32_t slot_key(const EvictParams& p, float v, int 
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive prefix sum of one value per warp (call with the value in every
-// lane); returns this warp's prefix.
-__device__ __forceinline__ int warps_prefix(int v, int* s_tmp) {
+// Exclusive prefix sums over the block of N values per thread, and the sums.
+template <int N, int WARPS>
+__device__ __forceinline__ void block_prefix(const uint32_t (&v)[N], uint32_t (*s_tmp)[32], uint32_t (&before)[N],
+                                             uint32_t (&all)[N]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __syncthreads();
-  if (lane == 0) s_tmp[warp] = v;
-  __syncthreads();
-  int x = lane < warp ? s_tmp[lane] : 0;
+  uint32_t inc[N];
 #pragma unroll
-  for (int m = 16; m; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
-  return x;
+  for (int k = 0; k < N; ++k) inc[k] = v[k];
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, inc[k], m);
+      if (lane >= m) inc[k] += o;
+    }
+  __syncthreads();
+  if (lane == 31)
+#pragma unroll
+    for (int k = 0; k < N; ++k) s_tmp[k][warp] = inc[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const uint32_t x = lane < WARPS ? s_tmp[k][lane] : 0u;
+    all[k] = __reduce_add_sync(0xffffffffu, x);
+    before[k] = __reduce_add_sync(0xffffffffu, lane < warp ? x : 0u) + inc[k] - v[k];
+  }
 }
 
 // Moves rows [first, n) step by step: K and V of a slot by a group of lanes,
@@ -100,14 +115,17 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, const longlong2*
   }
 }
 
-__global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
+// COPIES: of the histogram, against collisions.
+template <int THREADS, int COPIES>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ EvictParams p) {
+  constexpr int WARPS = THREADS / 32, D = kEvBins / THREADS;  // D: digits per thread
   extern __shared__ uint32_t s_dyn[];
   uint32_t* hist = s_dyn;                              // [copies][bins]; then the (to, from) slots of fused moves
-  uint32_t* kept = s_dyn + kEvCopies * kEvBins;        // a bit per slot
-  uint32_t* keys = kept + (p.capacity + 31) / 32;      // [capacity] where cached
-  __shared__ uint32_t s_warp[kEvWarps];
+  uint32_t* kept = s_dyn + COPIES * kEvBins;           // a bit per slot: key above the threshold
+  uint32_t* level = kept + (p.capacity + 31) / 32;     // a bit per slot: key equal to it
+  uint32_t* keys = level + (p.capacity + 31) / 32;     // [capacity] where cached
+  __shared__ uint32_t s_sum[2][32];
   __shared__ uint32_t s_pick[2];
-  __shared__ int s_tmp[kEvWarps];
   pdl_trigger();
   pdl_wait();
   const int b = blockIdx.y, h = blockIdx.x;
@@ -120,28 +138,39 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const __gri
   const int len = p.lengths[b], next = p.a.next_pos[b], budget = p.a.budget;
   const int n = max(0, min(len, p.capacity)), live = min(n, budget);
   if (h == 0 && tid == 0) p.a.new_lengths[b] = min(len, min(budget, p.capacity));
-  for (int i0 = tid; i0 < p.capacity; i0 += 4 * kEvThreads) {  // (four slots' loads in flight)
-    float v[4];
-    int at[4];
+  constexpr int U = 8;  // slots whose loads are in flight together
+  // f(i, score, position) for this thread's slots below `end`
+  auto each_slot = [&](int end, auto f) {
+    for (int i0 = tid; i0 < end; i0 += U * THREADS) {
+      float v[U];
+      int at[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u * kEvThreads;
-      v[u] = i < n ? sc[i] : 0.f;
-      at[u] = i < n ? pos[i] : -1;
-    }
+      for (int u = 0; u < U; ++u) {
+        const int i = min(i0 + u * THREADS, end - 1);
+        v[u] = sc[i];
+        at[u] = pos[i];
+      }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u * kEvThreads;
-      if (i >= p.capacity) break;
-      if (p.cached) keys[i] = slot_key(p, v[u], at[u], next);
-      nsc[i] = i < live ? v[u] : 0.f;
-      npos[i] = i < live ? at[u] : -1;
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * THREADS < end) f(i0 + u * THREADS, v[u], at[u]);
     }
-  }
+  };
+  auto copy = [&] {  // the kept range as it was (freed slots are overwritten later), zeros past it
+    for (int i = live + tid; i < p.capacity; i += THREADS) {
+      nsc[i] = 0.f;
+      npos[i] = -1;
+    }
+    each_slot(live, [&](int i, float v, int at) {
+      nsc[i] = v;
+      npos[i] = at;
+    });
+  };
   if (n <= budget) {
+    copy();
     if (tid == 0) p.moved[bh] = 0;
     return;
   }
+  if (p.cached) each_slot(n, [&](int i, float v, int at) { keys[i] = slot_key(p, v, at, next); });
   auto key = [&](int i) { return p.cached ? keys[i] : slot_key(p, sc[i], pos[i], next); };
 
   // ---- the budget-th largest key: digits of 11, 11 and 10 bits ----
@@ -149,37 +178,39 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const __gri
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < kEvCopies * kEvBins; i += kEvThreads) hist[i] = 0;
+    for (int i = tid; i < COPIES * kEvBins; i += THREADS) hist[i] = 0;
     __syncthreads();
-    uint32_t* mine = hist + (warp % kEvCopies) * kEvBins;
-    for (int i = tid; i < n; i += kEvThreads) {
-      const uint32_t k = key(i);
+    uint32_t* mine = hist + (warp % COPIES) * kEvBins;
+    auto count = [&](uint32_t k) {
       if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&mine[(k >> shift) & ((1u << bits) - 1)], 1u);
+    };
+    if (p.cached) {
+#pragma unroll 4
+      for (int i = tid; i < n; i += THREADS) count(keys[i]);
+    } else {
+      each_slot(n, [&](int, float v, int at) { count(slot_key(p, v, at, next)); });
     }
     __syncthreads();
-    // thread t holds the digits kEvBins - 1 - 2 t and the one below, from the top
-    uint32_t own[2] = {0, 0};
+    // thread t holds D digits down from kEvBins - 1 - D t
+    uint32_t own[D], sum[1] = {0}, pre[1], all[1];
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int e = 0; e < D; ++e) {
+      own[e] = 0;
 #pragma unroll
-      for (int w = 0; w < kEvCopies; ++w) own[e] += hist[w * kEvBins + kEvBins - 1 - 2 * tid - e];
-    uint32_t inc = own[0] + own[1];
-#pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-      const uint32_t o = __shfl_up_sync(0xffffffffu, inc, m);
-      if (lane >= m) inc += o;
+      for (int w = 0; w < COPIES; ++w) own[e] += hist[w * kEvBins + kEvBins - 1 - D * tid - e];
+      sum[0] += own[e];
     }
-    if (lane == 31) s_warp[warp] = inc;
-    __syncthreads();
-    uint32_t above = lane < warp ? s_warp[lane] : 0;
-    above = __reduce_add_sync(0xffffffffu, above) + inc - own[0] - own[1];
+    block_prefix<1, WARPS>(sum, s_sum, pre, all);
+    uint32_t above = pre[0];
+    if (above < want && want <= above + sum[0]) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (above < want && want <= above + own[e]) {
-        s_pick[0] = kEvBins - 1 - 2 * tid - e;
-        s_pick[1] = want - above;
+      for (int e = 0; e < D; ++e) {
+        if (above < want && want <= above + own[e]) {
+          s_pick[0] = kEvBins - 1 - D * tid - e;
+          s_pick[1] = want - above;
+        }
+        above += own[e];
       }
-      above += own[e];
     }
     __syncthreads();
     prefix |= s_pick[0] << shift;
@@ -187,60 +218,57 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const __gri
   }
   // keys above `prefix` are kept, and of those equal to it the first `want`
 
-  // ---- kept bits, in slot order: each warp walks a run of whole words ----
-  const int words = (n + 31) / 32, run = (words + kEvWarps - 1) / kEvWarps;
-  const int w0 = min(warp * run, words), w1 = min(w0 + run, words);
-  int equal = 0;
-  for (int w = w0; w < w1; ++w) {
-    const int i = w * 32 + lane;
-    equal += __popc(__ballot_sync(0xffffffffu, i < n && key(min(i, n - 1)) == prefix));
-  }
-  int taken = warps_prefix(equal, s_tmp);
-  int holes = 0, late = 0;
-  for (int w = w0; w < w1; ++w) {
+  const int words = (n + 31) / 32;
+#pragma unroll 4
+  for (int w = warp; w < words; w += WARPS) {
     const int i = w * 32 + lane;
     const uint32_t k = key(min(i, n - 1));
-    const uint32_t eq = __ballot_sync(0xffffffffu, i < n && k == prefix);
-    const int rank = taken + __popc(eq & ((1u << lane) - 1));
-    const bool keep = i < n && (k > prefix || (k == prefix && rank < (int)want));
-    const uint32_t word = __ballot_sync(0xffffffffu, keep);
-    taken += __popc(eq);
-    if (lane == 0) kept[w] = word;
-    const int below = budget - w * 32;  // of the word's slots, those under the budget
-    const uint32_t low = below >= 32 ? 0xffffffffu : below <= 0 ? 0u : (1u << below) - 1;
-    holes += __popc(~word & low);  // (the budget is below n: every such slot exists)
-    late += __popc(word & ~low);
+    const uint32_t gt = __ballot_sync(0xffffffffu, i < n && k > prefix), eq = __ballot_sync(0xffffffffu, i < n && k == prefix);
+    if (lane == 0) {
+      kept[w] = gt;
+      level[w] = eq;
+    }
   }
-  int hole_at = warps_prefix(holes, s_tmp);
-  int late_at = warps_prefix(late, s_tmp);
+  __syncthreads();
   // the slots of move m: in the shared memory of the counts where few, else in
   // the words of its entry of the list
   longlong2* mv = p.moves + bh * p.max_moves;
   int2* pairs = reinterpret_cast<int2*>(hist);
-  for (int w = w0; w < w1; ++w) {
-    const int i = w * 32 + lane;
-    const uint32_t word = kept[w];
-    const int below = budget - w * 32;
+  uint32_t equal = 0, moves = 0, freed = 0;  // equal keys, late slots and holes in the words before
+  for (int c0 = 0; c0 < words; c0 += THREADS) {  // a word per thread
+    const int w = c0 + tid;
+    uint32_t word = w < words ? kept[w] : 0, eq = w < words ? level[w] : 0;
+    uint32_t c[1] = {static_cast<uint32_t>(__popc(eq))}, at[1], all[1];
+    block_prefix<1, WARPS>(c, s_sum, at, all);
+    at[0] += equal;
+    equal += all[0];
+    int take = at[0] >= want ? 0 : static_cast<int>(min(want - at[0], c[0]));
+    if (take == (int)c[0]) {
+      word |= eq;
+    } else {
+      for (; take > 0; --take, eq &= eq - 1) word |= eq & (0u - eq);
+    }
+    const int below = budget - w * 32;  // of the word's slots, those under the budget
     const uint32_t low = below >= 32 ? 0xffffffffu : below <= 0 ? 0u : (1u << below) - 1;
-    const uint32_t hb = ~word & low, lb = word & ~low, under = (1u << lane) - 1;
-    if ((hb >> lane) & 1u) {
-      const int m = hole_at + __popc(hb & under);
+    uint32_t holes = ~word & low, late = word & ~low;  // (the budget is below n: every hole is a slot)
+    uint32_t two[2] = {static_cast<uint32_t>(__popc(holes)), static_cast<uint32_t>(__popc(late))}, from[2], sum[2];
+    block_prefix<2, WARPS>(two, s_sum, from, sum);
+    for (uint32_t m = freed + from[0]; holes; holes &= holes - 1, ++m) {
+      const int i = w * 32 + __ffs(holes) - 1;
       if (p.fused) pairs[m].y = i;
       else mv[m].y = i;
     }
-    if ((lb >> lane) & 1u) {
-      const int m = late_at + __popc(lb & under);
+    for (uint32_t m = moves + from[1]; late; late &= late - 1, ++m) {
+      const int i = w * 32 + __ffs(late) - 1;
       if (p.fused) pairs[m].x = i;
       else mv[m].x = i;
     }
-    hole_at += __popc(hb);
-    late_at += __popc(lb);
+    freed += sum[0];
+    moves += sum[1];
   }
+  copy();
   __syncthreads();
-  if (warp == kEvWarps - 1 && lane == 0) s_tmp[0] = late_at;  // the number of moves
-  __syncthreads();
-  const int moves = s_tmp[0];
-  // ---- the slots' entries, and where their rows lie ----
+  // ---- the moved slots' entries, and where their rows lie ----
   const int32_t* table = p.block_table + b * p.table_stride;
   const int mask = (1 << p.lg_page) - 1;
   auto offset = [&](int slot) -> long long {
@@ -249,18 +277,30 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const __gri
     return page * p.page_stride + h * p.head_stride + (slot & mask) * p.token_stride;
   };
   longlong2* list = p.fused ? reinterpret_cast<longlong2*>(hist) + kMvFused : mv;  // (past the pairs)
-  for (int i = tid; i < moves; i += kEvThreads) {
+  for (int i = tid; i < (int)moves; i += THREADS) {
     const int2 m = p.fused ? pairs[i] : make_int2(static_cast<int>(mv[i].x), static_cast<int>(mv[i].y));
     nsc[m.y] = sc[m.x];
     npos[m.y] = pos[m.x];
     list[i] = make_longlong2(offset(m.x), offset(m.y));
   }
   if (!p.fused) {
-    if (tid == 0) p.moved[bh] = moves;
+    if (tid == 0) p.moved[bh] = static_cast<int>(moves);
     return;
   }
   __syncthreads();
-  move_rows(p, list, moves, tid >> p.lg_lanes, kEvThreads >> p.lg_lanes, tid & ((1 << p.lg_lanes) - 1));
+  move_rows(p, list, moves, tid >> p.lg_lanes, THREADS >> p.lg_lanes, tid & ((1 << p.lg_lanes) - 1));
+}
+
+template <int THREADS, int COPIES>
+tp_status launch_select(const EvictParams& p, cudaStream_t st) {
+  const int smem = (COPIES * kEvBins + 2 * ((p.capacity + 31) / 32) + (p.cached ? p.capacity : 0)) * 4;
+  static int smem_set[64];
+  // (the default dynamic limit is 48 KB less the static shared memory)
+  const tp_status s = ensure_smem(evict_select_kernel<THREADS, COPIES>, smem > 47 * 1024 ? smem + 1024 : smem, smem_set,
+                                  "evict: shared memory attribute");
+  if (s != TP_OK) return s;
+  return launch_early(evict_select_kernel<THREADS, COPIES>, dim3(p.kv_heads, p.batch), THREADS, smem, st,
+                      "evict_select launch", p);
 }
 
 __global__ void __launch_bounds__(kMvThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
@@ -341,11 +381,7 @@ TP_API tp_status tp_cache_evict(const tp_evict_args* args, const tp_paged_cache*
   p.lg_lanes = log2_int((cache->head_dim + 7) / 8);
   p.cached = p.capacity <= kEvCached;
   p.fused = max_moves <= kMvFused;
-  const int smem = (kEvCopies * kEvBins + (p.capacity + 31) / 32 + (p.cached ? p.capacity : 0)) * 4;
-  static int smem_set[64];
-  s = ensure_smem(evict_select_kernel, smem, smem_set, "evict: shared memory attribute");
-  if (s != TP_OK) return s;
-  s = launch_early(evict_select_kernel, dim3(cache->kv_heads, cache->batch), kEvThreads, smem, st, "evict_select launch", p);
+  s = p.capacity <= kEvSmall ? launch_select<256, 2>(p, st) : launch_select<1024, 4>(p, st);
   if (s != TP_OK || p.fused) return s;
   int sms = 0;
   s = device_sms(&sms);
