@@ -50,6 +50,7 @@ struct EvictParams {
   int lg_lanes;      // lanes per row
   int cached;        // keys in shared memory
   int fused;         // moves by the selecting CTA
+  int vectors;       // rows of scores and positions are 16-byte aligned
 };
 
 __device__ __forceinline__ uint32_t slot_key(const EvictParams& p, float v, int at, int next) {
@@ -138,27 +139,63 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
   const int len = p.lengths[b], next = p.a.next_pos[b], budget = p.a.budget;
   const int n = max(0, min(len, p.capacity)), live = min(n, budget);
   if (h == 0 && tid == 0) p.a.new_lengths[b] = min(len, min(budget, p.capacity));
-  constexpr int U = 8;  // slots whose loads are in flight together
-  // f(i, score, position) for this thread's slots below `end`
+  // f(i, score, position) for this thread's slots below `end`, four
+  // neighbouring ones at a time where rows of the arrays are 16-byte aligned
   auto each_slot = [&](int end, auto f) {
-    for (int i0 = tid; i0 < end; i0 += U * THREADS) {
-      float v[U];
-      int at[U];
+    constexpr int U = 2;  // groups of four whose loads are in flight together
+    if (p.vectors) {
+      for (int i0 = 4 * tid; i0 < end; i0 += 4 * U * THREADS) {
+        float4 v[U];
+        int4 at[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = min(i0 + u * THREADS, end - 1);
-        v[u] = sc[i];
-        at[u] = pos[i];
+        for (int u = 0; u < U; ++u) {
+          const int i = min(i0 + 4 * u * THREADS, (end - 1) & ~3);  // (within the capacity, a multiple of four)
+          v[u] = *reinterpret_cast<const float4*>(sc + i);
+          at[u] = *reinterpret_cast<const int4*>(pos + i);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + 4 * u * THREADS;
+          if (i < end) f(i, v[u].x, at[u].x);
+          if (i + 1 < end) f(i + 1, v[u].y, at[u].y);
+          if (i + 2 < end) f(i + 2, v[u].z, at[u].z);
+          if (i + 3 < end) f(i + 3, v[u].w, at[u].w);
+        }
       }
+    } else {
+      constexpr int S = 4 * U;
+      for (int i0 = tid; i0 < end; i0 += S * THREADS) {
+        float v[S];
+        int at[S];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (i0 + u * THREADS < end) f(i0 + u * THREADS, v[u], at[u]);
+        for (int u = 0; u < S; ++u) {
+          const int i = min(i0 + u * THREADS, end - 1);
+          v[u] = sc[i];
+          at[u] = pos[i];
+        }
+#pragma unroll
+        for (int u = 0; u < S; ++u)
+          if (i0 + u * THREADS < end) f(i0 + u * THREADS, v[u], at[u]);
+      }
     }
   };
   auto copy = [&] {  // the kept range as it was (freed slots are overwritten later), zeros past it
-    for (int i = live + tid; i < p.capacity; i += THREADS) {
-      nsc[i] = 0.f;
-      npos[i] = -1;
+    int first = live;  // of the zeros
+    if (p.vectors) {
+      first = (live + 3) & ~3;
+      for (int i = first + 4 * tid; i < p.capacity; i += 4 * THREADS) {
+        *reinterpret_cast<float4*>(nsc + i) = make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<int4*>(npos + i) = make_int4(-1, -1, -1, -1);
+      }
+      if (tid < first - live) {
+        nsc[live + tid] = 0.f;
+        npos[live + tid] = -1;
+      }
+    } else {
+      for (int i = first + tid; i < p.capacity; i += THREADS) {
+        nsc[i] = 0.f;
+        npos[i] = -1;
+      }
     }
     each_slot(live, [&](int i, float v, int at) {
       nsc[i] = v;
@@ -174,6 +211,8 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
   auto key = [&](int i) { return p.cached ? keys[i] : slot_key(p, sc[i], pos[i], next); };
 
   // ---- the budget-th largest key: digits of 11, 11 and 10 bits ----
+  // (a digit's count lies where the threads that sum D digits each meet no bank twice)
+  auto place = [](uint32_t digit) { return digit % D * THREADS + digit / D; };
   uint32_t prefix = 0, want = budget;  // keys that match `prefix` above the digit hold the want-th largest
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
@@ -182,7 +221,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     __syncthreads();
     uint32_t* mine = hist + (warp % COPIES) * kEvBins;
     auto count = [&](uint32_t k) {
-      if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&mine[(k >> shift) & ((1u << bits) - 1)], 1u);
+      if (pass == 0 || (k >> (shift + bits)) == (prefix >> (shift + bits))) atomicAdd(&mine[place((k >> shift) & ((1u << bits) - 1))], 1u);
     };
     if (p.cached) {
 #pragma unroll 4
@@ -197,7 +236,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     for (int e = 0; e < D; ++e) {
       own[e] = 0;
 #pragma unroll
-      for (int w = 0; w < COPIES; ++w) own[e] += hist[w * kEvBins + kEvBins - 1 - D * tid - e];
+      for (int w = 0; w < COPIES; ++w) own[e] += hist[w * kEvBins + place(kEvBins - 1 - D * tid - e)];
       sum[0] += own[e];
     }
     block_prefix<1, WARPS>(sum, s_sum, pre, all);
@@ -277,11 +316,32 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     return page * p.page_stride + h * p.head_stride + (slot & mask) * p.token_stride;
   };
   longlong2* list = p.fused ? reinterpret_cast<longlong2*>(hist) + kMvFused : mv;  // (past the pairs)
-  for (int i = tid; i < (int)moves; i += THREADS) {
-    const int2 m = p.fused ? pairs[i] : make_int2(static_cast<int>(mv[i].x), static_cast<int>(mv[i].y));
-    nsc[m.y] = sc[m.x];
-    npos[m.y] = pos[m.x];
-    list[i] = make_longlong2(offset(m.x), offset(m.y));
+  constexpr int M = 2;  // moves whose loads are in flight together
+  for (int i0 = tid; i0 < (int)moves; i0 += M * THREADS) {
+    int2 m[M];
+    float v[M];
+    int at[M];
+    longlong2 rows[M];
+#pragma unroll
+    for (int u = 0; u < M; ++u) {
+      const int i = i0 + u * THREADS;  // (an entry is read and replaced by one thread)
+      m[u] = i >= (int)moves ? make_int2(0, 0)
+             : p.fused       ? pairs[i]
+                             : make_int2(static_cast<int>(mv[i].x), static_cast<int>(mv[i].y));
+    }
+#pragma unroll
+    for (int u = 0; u < M; ++u) {
+      v[u] = sc[m[u].x];
+      at[u] = pos[m[u].x];
+      rows[u] = make_longlong2(offset(m[u].x), offset(m[u].y));
+    }
+#pragma unroll
+    for (int u = 0; u < M; ++u)
+      if (i0 + u * THREADS < (int)moves) {
+        nsc[m[u].y] = v[u];
+        npos[m[u].y] = at[u];
+        list[i0 + u * THREADS] = rows[u];
+      }
   }
   if (!p.fused) {
     if (tid == 0) p.moved[bh] = static_cast<int>(moves);
@@ -380,6 +440,8 @@ TP_API tp_status tp_cache_evict(const tp_evict_args* args, const tp_paged_cache*
   cudaStream_t st = as_stream(stream);
   p.lg_lanes = log2_int((cache->head_dim + 7) / 8);
   p.cached = p.capacity <= kEvCached;
+  p.vectors = p.capacity % 4 == 0 && aligned(p.scores, 16) && aligned(p.positions, 16) && aligned(a.new_scores, 16) &&
+              aligned(a.new_positions, 16);
   p.fused = max_moves <= kMvFused;
   s = p.capacity <= kEvSmall ? launch_select<256, 2>(p, st) : launch_select<1024, 4>(p, st);
   if (s != TP_OK || p.fused) return s;
