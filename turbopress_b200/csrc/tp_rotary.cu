@@ -15,8 +15,11 @@
 // vectors (16 bytes each where VEC = 8) at p and p + rot/2, or adjacent ones
 // in the interleaved layout and in the part that is not turned.  G lanes (a
 // power of two) hold one head, so the norm's sum of squares is a shuffle
-// reduction and q, k can be turned in place.
+// reduction and q, k can be turned in place.  A thread keeps its unit and head
+// through the CTA's tokens (addresses advance by one addition), with several
+// tokens' loads in flight.
 #include <algorithm>
+#include <type_traits>
 
 #include "tp_decode.cuh"
 #include "tp_paged.cuh"
@@ -58,52 +61,95 @@ __device__ __forceinline__ void unit_at(const RotaryParams& p, int u, int& lo, i
   }
 }
 
+// A vector's elements as floats, and back, two at a time.
+template <class T, int N>
+__device__ __forceinline__ void unpack(const Pack<T, N>& x, float (&v)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = Elem<T>::to(x.v[e]);
+}
+template <class T, int N>
+__device__ __forceinline__ void pack(const float (&v)[N], Pack<T, N>& x) {
+#pragma unroll
+  for (int e = 0; e < N; e += 2) {
+    if constexpr (N > 1 && sizeof(T) == 2) {
+      if constexpr (std::is_same<T, __half>::value)
+        *reinterpret_cast<__half2*>(&x.v[e]) = __floats2half2_rn(v[e], v[(e + 1) % N]);
+      else
+        *reinterpret_cast<__nv_bfloat162*>(&x.v[e]) = __floats2bfloat162_rn(v[e], v[(e + 1) % N]);
+    } else {
+      x.v[e] = Elem<T>::from(v[e]);
+      if (N > 1) x.v[(e + 1) % N] = Elem<T>::from(v[(e + 1) % N]);
+    }
+  }
+}
+
+// N floats of shared memory, 16 bytes at a time (a unit's are so aligned).
+template <int N>
+__device__ __forceinline__ void read_floats(const float* p, float (&v)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p + e);
+      v[e] = x.x;
+      v[e + 1] = x.y;
+      v[e + 2] = x.z;
+      v[e + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = p[e];
+  }
+}
+
 // UPL: units per lane (more than one only where a head has over 32 units).
 template <class T, int VEC, int UPL>
-__global__ void __launch_bounds__(kRtThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  extern __shared__ float2 cs[];  // [tpc][rot/2]
+__global__ void __launch_bounds__(kRtThreads, VEC == 1 ? 2 : 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  extern __shared__ __align__(16) float cs[];  // [tpc][cos, sin][rot/2]
   __shared__ int64_t s_dst[kRtMaxTokens];
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x;
   const int64_t tok0 = (int64_t)blockIdx.x * p.tpc;
   const int nt = static_cast<int>(min((int64_t)p.tpc, p.a.tokens - tok0));
-  const int h0 = blockIdx.y * p.heads_cta, nh = min(p.heads_cta, p.heads - h0);
+  const int h0 = blockIdx.y * p.heads_cta, h1 = min(h0 + p.heads_cta, p.heads);
   const int half = p.a.rot_dim / 2;
   const int G = 1 << p.lg_group;
   const int u0 = tid & (G - 1), slot0 = tid >> p.lg_group, nslots = kRtThreads >> p.lg_group;
-  const int total = nt * nh;
 
-  // a lane's units of one head
-  auto source = [&](int idx, const T*& src, int& t, int& head) {
-    t = idx / nh;
-    head = h0 + idx - t * nh;
-    const int64_t n = tok0 + t;
-    if (head < p.a.q_heads) src = static_cast<const T*>(p.a.q) + n * p.a.q_token_stride + head * p.a.q_head_stride;
-    else if (head < p.a.q_heads + p.a.kv_heads)
-      src = static_cast<const T*>(p.a.k) + n * p.a.k_token_stride + (head - p.a.q_heads) * p.a.k_head_stride;
-    else
-      src = static_cast<const T*>(p.a.v) + n * p.a.v_token_stride + (head - p.a.q_heads - p.a.kv_heads) * p.a.v_head_stride;
-  };
-  auto load = [&](int idx, Pack<T, VEC> (&x)[UPL][2]) {
-    if (idx >= total) return;
-    const T* src;
-    int t, head;
-    source(idx, src, t, head);
-#pragma unroll
-    for (int i = 0; i < UPL; ++i) {
-      const int u = u0 + i * G;
-      if (u < p.units) {
-        int lo, hi;
-        unit_at<VEC>(p, u, lo, hi);
-        x[i][0] = *reinterpret_cast<const Pack<T, VEC>*>(src + lo);
-        x[i][1] = *reinterpret_cast<const Pack<T, VEC>*>(src + hi);
-      }
+  // The source row of `head` at the CTA's first token, and its step per token.
+  auto source = [&](int head, int64_t& step) -> const T* {
+    const int k = head - p.a.q_heads, v = k - p.a.kv_heads;
+    if (k < 0) {
+      step = p.a.q_token_stride;
+      return static_cast<const T*>(p.a.q) + tok0 * step + head * p.a.q_head_stride;
     }
+    if (v < 0) {
+      step = p.a.k_token_stride;
+      return static_cast<const T*>(p.a.k) + tok0 * step + k * p.a.k_head_stride;
+    }
+    step = p.a.v_token_stride;
+    return static_cast<const T*>(p.a.v) + tok0 * step + v * p.a.v_head_stride;
   };
-
-  Pack<T, VEC> x[UPL][2], nx[UPL][2];
-  load(slot0, x);  // in flight while the angles are computed
+  constexpr int TB = UPL == 1 ? 2 : 1;  // tokens whose loads are in flight
+  Pack<T, VEC> x[TB][UPL][2];
+  auto load = [&](const T* src, int64_t step, int t0) {
+#pragma unroll
+    for (int t = 0; t < TB; ++t)
+      if (t0 + t < nt)
+#pragma unroll
+        for (int i = 0; i < UPL; ++i) {
+          const int u = u0 + i * G;
+          if (u < p.units) {
+            int lo, hi;
+            unit_at<VEC>(p, u, lo, hi);
+            x[t][i][0] = *reinterpret_cast<const Pack<T, VEC>*>(src + t * step + lo);
+            x[t][i][1] = *reinterpret_cast<const Pack<T, VEC>*>(src + t * step + hi);
+          }
+        }
+  };
+  int64_t step = 0;
+  const T* src = h0 + slot0 < h1 ? source(h0 + slot0, step) : nullptr;
+  if (src) load(src, step, 0);  // in flight while the angles are computed
 
   if (p.paged && tid < nt) {
     const int64_t n = tok0 + tid;
@@ -138,108 +184,101 @@ __global__ void __launch_bounds__(kRtThreads) rotary_kernel(const __grid_constan
     const int64_t turn = static_cast<int64_t>(static_cast<uint64_t>(pos) * p.a.freq[n]);  // [-1/2, 1/2) turns
     float s, c;
     sincospif(__ll2float_rn(turn) * 1.0842021724855044e-19f /* 2^-63 */, &s, &c);
-    cs[i] = make_float2(c * p.a.scale, (p.a.inverse ? -s : s) * p.a.scale);
+    cs[(2 * t) * half + n] = c * p.a.scale;
+    cs[(2 * t + 1) * half + n] = (p.a.inverse ? -s : s) * p.a.scale;
   }
   __syncthreads();
 
+  const bool norms = p.a.q_norm || p.a.k_norm;
   // every warp makes the same number of rounds: the norm's shuffles need all lanes
-  for (int base = 0; base < total; base += nslots) {
-    const int idx = base + slot0;
-    load(idx + nslots, nx);
-    const bool on = idx < total;
-    const T* src;
-    int t = 0, head = 0;
-    if (on) source(idx, src, t, head);
+  for (int base = h0; base < h1; base += nslots) {
+    const int head = base + slot0;
+    const bool on = head < h1;
     const int kind = head < p.a.q_heads ? 0 : head < p.a.q_heads + p.a.kv_heads ? 1 : 2;
+    const int h = kind == 0 ? head : kind == 1 ? head - p.a.q_heads : head - p.a.q_heads - p.a.kv_heads;
     const T* w = static_cast<const T*>(kind == 0 ? p.a.q_norm : kind == 1 ? p.a.k_norm : nullptr);
-    float rinv = 1.f;
-    if (p.a.q_norm || p.a.k_norm) {  // the same in every thread
-      float sq = 0.f;
+    if (base != h0) src = on ? source(head, step) : nullptr;
+    // contiguous outputs advance by a row of heads; pages are looked up
+    const int64_t out_step = (int64_t)(kind == 0 ? p.a.q_heads : p.a.kv_heads) * p.a.head_dim;
+    T* out = kind == 0 ? static_cast<T*>(p.a.q_out) : p.paged ? nullptr : static_cast<T*>(p.a.k_out);
+    if (out) out += tok0 * out_step + h * p.a.head_dim;
+    T* pages = static_cast<T*>(kind == 1 ? p.k_pages : p.v_pages) + (p.paged ? h * p.head_stride : 0);
+    for (int t0 = 0; t0 < nt; t0 += TB) {
+      if (src && (base != h0 || t0)) load(src, step, t0);
 #pragma unroll
-      for (int i = 0; i < UPL; ++i)
-        if (on && u0 + i * G < p.units)
+      for (int tt = 0; tt < TB; ++tt) {
+        const int t = t0 + tt;
+        if (t >= nt) break;
+        float rinv = 1.f;
+        if (norms) {
+          float sq = 0.f;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float a = Elem<T>::to(x[i][0].v[e]), b = Elem<T>::to(x[i][1].v[e]);
-            sq = fmaf(a, a, fmaf(b, b, sq));
-          }
-      for (int m = G >> 1; m; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m);
-      if (w) rinv = rsqrtf(sq / p.a.head_dim + p.a.eps);
-    }
-    T* dst = nullptr;
-    if (on) {
-      const int64_t n = tok0 + t;
-      if (kind == 0) {
-        dst = static_cast<T*>(p.a.q_out) + (n * p.a.q_heads + head) * p.a.head_dim;
-      } else {
-        const int h = kind == 1 ? head - p.a.q_heads : head - p.a.q_heads - p.a.kv_heads;
-        if (!p.paged) {
-          dst = static_cast<T*>(p.a.k_out) + (n * p.a.kv_heads + h) * p.a.head_dim;
-        } else if (s_dst[t] >= 0) {
-          dst = static_cast<T*>(kind == 1 ? p.k_pages : p.v_pages) + s_dst[t] + h * p.head_stride;
-        }
-      }
-    }
-    if (dst) {
-#pragma unroll
-      for (int i = 0; i < UPL; ++i) {
-        const int u = u0 + i * G;
-        if (u >= p.units) continue;
-        int lo, hi;
-        unit_at<VEC>(p, u, lo, hi);
-        if (kind < 2 && (w || u < p.rot_units)) {
-          float a[VEC], b[VEC];
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            a[e] = Elem<T>::to(x[i][0].v[e]);
-            b[e] = Elem<T>::to(x[i][1].v[e]);
-          }
-          if (w) {
-            const Pack<T, VEC> wa = *reinterpret_cast<const Pack<T, VEC>*>(w + lo);
-            const Pack<T, VEC> wb = *reinterpret_cast<const Pack<T, VEC>*>(w + hi);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              a[e] *= rinv * Elem<T>::to(wa.v[e]);
-              b[e] *= rinv * Elem<T>::to(wb.v[e]);
-            }
-          }
-          if (u < p.rot_units) {
-            const float2* c = cs + t * half + u * VEC;
-            if (!p.a.interleaved || VEC == 1) {  // VEC = 1: both layouts pair the unit's two elements
+          for (int i = 0; i < UPL; ++i)
+            if (on && u0 + i * G < p.units)
 #pragma unroll
               for (int e = 0; e < VEC; ++e) {
-                const float2 f = c[e];
-                const float y = a[e] * f.x - b[e] * f.y;
-                b[e] = b[e] * f.x + a[e] * f.y;
-                a[e] = y;
+                const float a = Elem<T>::to(x[tt][i][0].v[e]), b = Elem<T>::to(x[tt][i][1].v[e]);
+                sq = fmaf(a, a, fmaf(b, b, sq));
               }
-            } else {
+          for (int m = G >> 1; m; m >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, m);
+          if (w) rinv = rsqrtf(sq / p.a.head_dim + p.a.eps);
+        }
+        T* dst = out ? out + t * out_step : s_dst[t] >= 0 ? pages + s_dst[t] : nullptr;
+        if (!on || !dst) continue;
 #pragma unroll
-              for (int e = 0; e < VEC; e += 2) {
-                const float2 f = c[e / 2], g = c[VEC / 2 + e / 2];
-                const float y = a[e] * f.x - a[(e + 1) % VEC] * f.y;
-                a[(e + 1) % VEC] = a[(e + 1) % VEC] * f.x + a[e] * f.y;
-                a[e] = y;
-                const float z = b[e] * g.x - b[(e + 1) % VEC] * g.y;
-                b[(e + 1) % VEC] = b[(e + 1) % VEC] * g.x + b[e] * g.y;
-                b[e] = z;
+        for (int i = 0; i < UPL; ++i) {
+          const int u = u0 + i * G;
+          if (u >= p.units) continue;
+          int lo, hi;
+          unit_at<VEC>(p, u, lo, hi);
+          if (kind < 2 && (w || u < p.rot_units)) {
+            float a[VEC], b[VEC];
+            unpack(x[tt][i][0], a);
+            unpack(x[tt][i][1], b);
+            if (w) {
+              float wa[VEC], wb[VEC];
+              unpack(*reinterpret_cast<const Pack<T, VEC>*>(w + lo), wa);
+              unpack(*reinterpret_cast<const Pack<T, VEC>*>(w + hi), wb);
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) {
+                a[e] *= rinv * wa[e];
+                b[e] *= rinv * wb[e];
               }
             }
-          }
+            if (u < p.rot_units) {
+              const float* co = cs + (2 * t) * half + u * VEC;
+              float c[VEC], s[VEC];
+              read_floats(co, c);
+              read_floats(co + half, s);
+              if (!p.a.interleaved || VEC == 1) {  // VEC = 1: both layouts pair the unit's two elements
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            x[i][0].v[e] = Elem<T>::from(a[e]);
-            x[i][1].v[e] = Elem<T>::from(b[e]);
+                for (int e = 0; e < VEC; ++e) {
+                  const float y = a[e] * c[e] - b[e] * s[e];
+                  b[e] = b[e] * c[e] + a[e] * s[e];
+                  a[e] = y;
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2) {
+                  constexpr int O = VEC > 1 ? 1 : 0, H = VEC / 2;
+                  const float ca = c[e / 2], sa = s[e / 2], cb = c[H + e / 2], sb = s[H + e / 2];
+                  const float y = a[e] * ca - a[e + O] * sa;
+                  a[e + O] = a[e + O] * ca + a[e] * sa;
+                  a[e] = y;
+                  const float z = b[e] * cb - b[e + O] * sb;
+                  b[e + O] = b[e + O] * cb + b[e] * sb;
+                  b[e] = z;
+                }
+              }
+            }
+            pack(a, x[tt][i][0]);
+            pack(b, x[tt][i][1]);
           }
+          *reinterpret_cast<Pack<T, VEC>*>(dst + lo) = x[tt][i][0];
+          *reinterpret_cast<Pack<T, VEC>*>(dst + hi) = x[tt][i][1];
         }
-        *reinterpret_cast<Pack<T, VEC>*>(dst + lo) = x[i][0];
-        *reinterpret_cast<Pack<T, VEC>*>(dst + hi) = x[i][1];
       }
-    }
-#pragma unroll
-    for (int i = 0; i < UPL; ++i) {
-      x[i][0] = nx[i][0];
-      x[i][1] = nx[i][1];
+      if (src) src += TB * step;
     }
   }
 }
@@ -263,7 +302,7 @@ tp_status launch_rotary(RotaryParams& p, cudaStream_t st) {
   split = (p.heads + p.heads_cta - 1) / p.heads_cta;
   const int64_t grid = (p.a.tokens + p.tpc - 1) / p.tpc;
   if (grid > 0x7FFFFFFF) return fail(TP_ERR_UNSUPPORTED, "tp_rotary: too many tokens");
-  const int smem = p.tpc * (p.a.rot_dim / 2) * static_cast<int>(sizeof(float2));
+  const int smem = p.tpc * p.a.rot_dim * static_cast<int>(sizeof(float));
   return launch_early(rotary_kernel<T, VEC, UPL>, dim3(static_cast<unsigned>(grid), split), kRtThreads, smem, st,
                       "rotary launch", p);
 }
