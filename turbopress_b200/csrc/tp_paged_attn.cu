@@ -842,8 +842,17 @@ __global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_
         const float* s = p.sbuf + (size_t)(off + h * (kItemCost + nt) + kItemCost + tile) * RT * TILE + tok;
         const float* z = p.lse2 + ((int64_t)b * p.kv_heads + h) * p.rows + rt * RT;
         const int rows = min(RT, p.rows - rt * RT);
-#pragma unroll 8
-        for (int r = 0; r < rows; ++r) w += exp2_diff(s[r * TILE], z[r]);
+        for (int r = 0; r < rows; r += 8) {  // eight rows' loads together
+          float a[8], m[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int at = min(r + k, rows - 1);
+            a[k] = s[at * TILE];
+            m[k] = z[at];
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) w += r + k < rows ? exp2_diff(a[k], m[k]) : 0.f;
+        }
       }
       off += p.kv_heads * (kItemCost + nt);
     }
