@@ -500,8 +500,9 @@ TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_ca
                                int64_t workspace_bytes, void* stream);
 
 /* Reads (synchronizing `stream`) and clears the status word of a workspace of
- * tp_paged_attn: TP_OK, or TP_ERR_DEVICE when a wait for a copy gave up (the
- * outputs of that call are NaN; the workspace is fit for the next). */
+ * tp_paged_attn: TP_OK, or TP_ERR_DEVICE when a wait for a copy gave up (rows
+ * of that call are NaN, and what they added to the scores; the workspace is
+ * fit for the next). */
 TP_API tp_status tp_paged_attn_status(void* workspace, void* stream);
 
 /* Eviction: of each sequence's slots keep the `budget` that come first by

@@ -206,6 +206,21 @@ def test_lengths_changed_between_calls():
         assert (count <= lens[i][:, None] + 1).all()
 
 
+def test_status_word():
+    """A wait that gave up is reported once (from a host-written record: the
+    status word behind the 512 counters) and the workspace stays fit."""
+    cache, g = _cache([50], 1, 2, 64, 16, torch.float16, 10)
+    cache.status()  # before any call
+    q = torch.randn(1, 1, 4, 64, generator=g, device=DEV).half()
+    want = cache.attend(q)
+    cache.status()
+    cache._ws[2048] = 1
+    with pytest.raises(RuntimeError, match="wait"):
+        cache.status()
+    cache.status()
+    assert torch.equal(cache.attend(q), want)
+
+
 def test_refusals():
     from turbopress_b200 import _abi
     from turbopress_b200.paged import PagedKVCache

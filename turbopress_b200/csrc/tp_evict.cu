@@ -53,7 +53,7 @@ struct EvictParams {
   int vectors;       // rows of scores and positions are 16-byte aligned
 };
 
-__device__ __forceinline__ uint32_t slot_key(const EvictParams& p, float v, int at, int next) {
+__device__ __forceinline__ uint32_t slot_key(const EvictParams& p, float v, int at, int64_t next) {
   if (at < p.a.sinks || at >= next - p.a.recent) return 0xFFFFFFFFu;
   if (v != v) return 0xFFFFFFFEu;
   if (v == 0.f) v = 0.f;  // -0 equals 0
@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
   const int32_t* pos = p.positions + bh * p.capacity;
   float* nsc = p.a.new_scores + bh * p.capacity;
   int32_t* npos = p.a.new_positions + bh * p.capacity;
-  const int len = p.lengths[b], next = p.a.next_pos[b], budget = p.a.budget;
+  const int len = p.lengths[b], budget = p.a.budget;
+  const int64_t next = p.a.next_pos[b];
   const int n = max(0, min(len, p.capacity)), live = min(n, budget);
   if (h == 0 && tid == 0) p.a.new_lengths[b] = min(len, min(budget, p.capacity));
   // f(i, score, position) for this thread's slots below `end`, four
