@@ -153,6 +153,7 @@ def require_cuda(*tensors: torch.Tensor | None) -> torch.device:
 # devices, never addresses) instead of repeating them.
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def meta(t: torch.Tensor | None) -> tuple | None:
@@ -162,7 +163,7 @@ def meta(t: torch.Tensor | None) -> tuple | None:
 
 def launch(fn, what: str, index: int, *args) -> None:
     """``fn(*args, stream)`` on device ``index`` and its current stream."""
-    if torch.cuda.current_device() != index:
+    if _device() != index:
         with torch.cuda.device(index):
             return launch(fn, what, index, *args)
     st = _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream

@@ -121,6 +121,9 @@ class PagedKVCache:
         self._evict_ws: Tensor | None = None
         self._outgrown: list[Tensor] = []  # workspaces that a captured graph may still use
         self._plans: dict[tuple, _AttnArgs] = {}
+        self._append_plans: dict[Rotary, dict] = {}
+        self._evict_bytes: dict[int, int] = {}
+        self._slots = None if scores is None or positions is None else [(scores[i], positions[i]) for i in range(L)]
 
     def _layer(self, layer: int) -> int:
         """Address of the layer's ``tp_paged_cache``."""
@@ -138,19 +141,25 @@ class PagedKVCache:
         tokens], by default ``next_pos`` onwards.  ``lengths`` stays: call
         ``advance`` once all layers have the step's tokens.  Tokens of idle
         sequences, past the capacity or without a page are not stored."""
-        if q.dim() != 4 or q.shape[0] != self.batch or k.shape[-2] != self.kv_heads or q.dtype != self.dtype:
-            raise ValueError(f"expected q [{self.batch}, tokens, heads, {self.head_dim}] and k, v with {self.kv_heads} heads, "
-                             f"all {self.dtype}")
-        if rotary.device != self.device or rotary.head_dim != self.head_dim:
-            raise ValueError("the rotary's device and head_dim differ from the cache's")
-        a, out, keep = rotary._args(q, k, v, positions, q_norm, k_norm, eps, inverse)
-        a.seq = q.shape[1]
+        plans = self._append_plans.get(rotary)
+        if plans is None:
+            if rotary.device != self.device or rotary.head_dim != self.head_dim:
+                raise ValueError("the rotary's device and head_dim differ from the cache's")
+            plans = self._append_plans[rotary] = {}
+        a, out, keep = rotary._args(plans, self._appendable, q, k, v, positions, q_norm, k_norm, eps, inverse)
         if positions is None:
             a.base = self.next_pos.data_ptr()
         addr = self._layer(layer)
-        if a.seq:
+        if a.tokens:
             _abi.launch(_abi.lib().tp_rotary, "append", self.device.index, ctypes.addressof(a), addr)
         return out
+
+    def _appendable(self, plan, q: Tensor, k: Tensor, v: Tensor) -> None:
+        """The cache's part of an append's checks; the tokens per sequence."""
+        if q.dim() != 4 or q.shape[0] != self.batch or k.shape[-2] != self.kv_heads or q.dtype != self.dtype:
+            raise ValueError(f"expected q [{self.batch}, tokens, heads, {self.head_dim}] and k, v with {self.kv_heads} heads, "
+                             f"all {self.dtype}")
+        plan.seq = max(1, q.shape[1])
 
     def advance(self, tokens: int | Tensor) -> None:
         """Count ``tokens`` (a number, or int32 [batch]) as cached: after the
@@ -232,14 +241,18 @@ class PagedKVCache:
         place; returns the layer's new (lengths [batch], scores, positions
         [batch, kv_heads, capacity]).  The cache itself still has the old ones:
         ``evict`` does all layers and takes them over."""
-        if self.scores is None or self.positions is None:
+        if self._slots is None:
             raise ValueError("eviction needs a cache with scores and positions")
         addr, lib = self._layer(layer), _abi.lib()
-        new = (torch.empty_like(self.lengths), torch.empty_like(self.scores[layer]), torch.empty_like(self.positions[layer]))
-        need = lib.tp_cache_evict_workspace_bytes(addr, budget)
-        if need < 0:
-            _abi.check(-need, "evict")
-        self._evict_ws = self._grown(self._evict_ws, need)
+        need = self._evict_bytes.get(budget)
+        if need is None:
+            need = lib.tp_cache_evict_workspace_bytes(addr, budget)
+            if need < 0:
+                _abi.check(-need, "evict")
+            self._evict_ws = self._grown(self._evict_ws, need)
+            self._evict_bytes[budget] = need
+        scores, positions = self._slots[layer]
+        new = (torch.empty_like(self.lengths), torch.empty_like(scores), torch.empty_like(positions))
         a = _EvictArgs(self.next_pos.data_ptr(), new[0].data_ptr(), new[1].data_ptr(), new[2].data_ptr(), budget, recent, sinks)
         _abi.launch(lib.tp_cache_evict, "evict", self.device.index, ctypes.addressof(a), addr, self._evict_ws.data_ptr(),
                     self._evict_ws.numel())

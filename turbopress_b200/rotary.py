@@ -128,28 +128,31 @@ class Rotary:
         return cls(head_dim, theta=theta, scaling=p, rot_dim=int(head_dim * part), interleaved=interleaved, device=device)
 
     # -- arguments shared with PagedKVCache.append ------------------------------
-    def _args(self, q: Tensor, k: Tensor, v: Tensor | None, positions: Tensor | None, q_norm: Tensor | None,
-              k_norm: Tensor | None, eps: float, inverse: bool) -> tuple[_RotaryArgs, Tensor, tuple]:
+    def _args(self, plans: dict, adapt, q: Tensor, k: Tensor, v: Tensor | None, positions: Tensor | None,
+              q_norm: Tensor | None, k_norm: Tensor | None, eps: float, inverse: bool) -> tuple[_RotaryArgs, Tensor, tuple]:
         """The call's arguments without k's destination, the queries' output and
-        the tensors to keep until the launch."""
+        the tensors to keep until the launch.  ``plans`` holds the checked part
+        by what the checks depend on; ``adapt(plan, q, k, v)`` completes a new one."""
         key = (_abi.meta(q), _abi.meta(k), _abi.meta(v), _abi.meta(positions), _abi.meta(q_norm), _abi.meta(k_norm))
-        plan = self._plans.get(key)
+        plan = plans.get(key)
         if plan is None:
             plan = self._checked(q, k, v, positions, q_norm, k_norm)
             if plan is None:  # not views of [tokens, heads, head_dim]
-                return self._args(q.contiguous(), k.contiguous(), None if v is None else v.contiguous(), positions, q_norm,
-                                  k_norm, eps, inverse)
-            if len(self._plans) >= 256:
-                self._plans.clear()
-            self._plans[key] = plan
-        if positions is not None:
-            positions = positions.to(torch.int64).contiguous()
+                return self._args(plans, adapt, q.contiguous(), k.contiguous(), None if v is None else v.contiguous(), positions,
+                                  q_norm, k_norm, eps, inverse)
+            if adapt is not None:
+                adapt(plan, q, k, v)
+            if len(plans) >= 256:
+                plans.clear()
+            plans[key] = plan
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         a = _RotaryArgs.from_buffer_copy(plan)
         a.q, a.k, a.q_out, a.inverse, a.eps = q.data_ptr(), k.data_ptr(), out.data_ptr(), inverse, eps
         if v is not None:
             a.v = v.data_ptr()
         if positions is not None:
+            if positions.dtype is not torch.int64 or not positions.is_contiguous():
+                positions = positions.to(torch.int64).contiguous()
             a.positions = positions.data_ptr()
         if q_norm is not None:
             a.q_norm = q_norm.data_ptr()
@@ -199,7 +202,7 @@ class Rotary:
         the rotation."""
         if positions is None:
             raise ValueError("positions are needed")
-        a, q_out, keep = self._args(q, k, None, positions, q_norm, k_norm, eps, inverse)
+        a, q_out, keep = self._args(self._plans, None, q, k, None, positions, q_norm, k_norm, eps, inverse)
         k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         a.k_out = k_out.data_ptr()
         _abi.launch(_abi.lib().tp_rotary, "rotary", self.device.index, ctypes.addressof(a), None)

@@ -50,7 +50,7 @@ class DraftVerifier:
         self.workspace = torch.zeros(need, dtype=torch.uint8, device=device)
         self.device = self.workspace.device
         _abi.require_cuda(self.workspace)
-        self._plans: dict[tuple, _VerifyArgs] = {}
+        self._plans: dict[tuple, tuple[_VerifyArgs, Tensor, Tensor]] = {}
 
     def __call__(self, logits: Tensor, draft_tokens: Tensor, *, uniforms: Tensor | None = None, noise: Tensor | None = None,
                  draft_probs: Tensor | None = None, temperature: Tensor | None = None,
@@ -70,10 +70,9 @@ class DraftVerifier:
             if len(self._plans) >= 256:
                 self._plans.clear()
             self._plans[key] = plan
-        B, rows = plan.batch, plan.drafts + 1
-        accepted = torch.empty(B, dtype=torch.int32, device=self.device)
-        tokens = torch.empty(B, rows, dtype=torch.int64, device=self.device)
-        a = _VerifyArgs.from_buffer_copy(plan)
+        template, like_accepted, like_tokens = plan
+        accepted, tokens = torch.empty_like(like_accepted), torch.empty_like(like_tokens)
+        a = _VerifyArgs.from_buffer_copy(template)
         a.logits, a.draft_tokens, a.accepted, a.tokens = (logits.data_ptr(), draft_tokens.data_ptr(), accepted.data_ptr(),
                                                           tokens.data_ptr())
         if temperature is not None:
@@ -89,9 +88,9 @@ class DraftVerifier:
         return accepted, tokens
 
     def _checked(self, logits: Tensor, draft_tokens: Tensor, uniforms: Tensor | None, noise: Tensor | None,
-                 draft_probs: Tensor | None, temperature: Tensor | None, n_drafts: Tensor | None) -> _VerifyArgs:
+                 draft_probs: Tensor | None, temperature: Tensor | None, n_drafts: Tensor | None) -> tuple[_VerifyArgs, Tensor, Tensor]:
         """Checks a call by what its key holds; the sizes and strides of its
-        arguments."""
+        arguments, and tensors like its outputs."""
         if logits.dim() != 3:
             raise ValueError(f"logits must be [batch, drafts + 1, vocab], got {tuple(logits.shape)}")
         B, rows, V = logits.shape
@@ -110,5 +109,6 @@ class DraftVerifier:
                 raise ValueError(f"{nm} must be a contiguous {dt} tensor {shape} on {self.device}")
         if logits.device != self.device:
             raise ValueError(f"logits must be on {self.device}")
-        return _VerifyArgs(batch_stride=logits.stride(0), row_stride=logits.stride(1), batch=B, drafts=K, vocab=V,
-                           dtype=_abi.dtype_code(logits.dtype))
+        return (_VerifyArgs(batch_stride=logits.stride(0), row_stride=logits.stride(1), batch=B, drafts=K, vocab=V,
+                            dtype=_abi.dtype_code(logits.dtype)),
+                torch.empty(B, dtype=torch.int32, device=self.device), torch.empty(B, rows, dtype=torch.int64, device=self.device))
