@@ -14,6 +14,12 @@
 // slot's 8 bytes once and keeps the keys in shared memory (up to 40960 slots;
 // above, it forms them again in each pass).  Few rows are moved by the CTA
 // that selected them; many by a second launch over the whole GPU.
+//
+// Measured (B200, whole calls): 64 of 1088 slots in each of 64 heads 8.0 us;
+// 16 sequences of up to 16384 slots cut to 2048 37 us, of which the longest
+// heads' selection about 20 (four passes' barriers and collisions) and the
+// moves 16 (86 MB, 5.4 TB/s).  A cluster of CTAs per head that adds its counts
+// up through distributed shared memory was slower at every length (65 us).
 #include <algorithm>
 
 #include "tp_decode.cuh"
@@ -27,11 +33,14 @@ constexpr int kEvMaxSlots = 1 << 19;
 constexpr int kEvCached = 40960;   // slots whose keys fit in shared memory
 constexpr int kEvBins = 2048;
 // Threads of the selection: few where few slots are (its barriers cost less).
-// EVTHREADS
+// Eight sequences of 1088 slots take 7.9 us with 256, 8.8 us with 1024; of 2000
+// slots 9.7 against 10.1 us.
 constexpr int kEvSmall = 2048;      // capacity up to which 256 threads do
 constexpr int kMvThreads = 256;
 constexpr int kMvRows = 4;          // rows in flight per group of lanes
-// Moves per head up to which the selecting CTA does them itself.  EVNOTE
+// Moves per head up to which the selecting CTA does them itself: 64 moves in
+// each of 64 heads take 7.9 us in all so and 11.6 us with the second launch,
+// 256 moves 10.3 against 14.6 us, 512 the same in both.
 constexpr int kMvFused = 256;
 
 struct EvictParams {

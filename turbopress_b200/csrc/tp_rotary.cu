@@ -18,6 +18,11 @@
 // reduction and q, k can be turned in place.  A thread keeps its unit and head
 // through the CTA's tokens (addresses advance by one addition), with several
 // tokens' loads in flight.
+//
+// Measured (B200): 8192 tokens of 64 + 8 + 8 heads of 128 with the append, bf16,
+// 62 us = 5.4 TB/s (0.83 of the measured HBM rate; issue slots 58 % busy); one
+// token of 32 + 8 + 8 heads with head norms 3.3 us, the launch and two round
+// trips.
 #include <algorithm>
 #include <type_traits>
 
@@ -290,7 +295,8 @@ tp_status launch_rotary(RotaryParams& p, cudaStream_t st) {
   p.lg_group = std::min(5, log2_int(p.units));
   // One token per CTA, and its heads over several CTAs, while that keeps the
   // grid under four CTAs per SM (short calls: latency); else several tokens
-  // per CTA, which share the launch's fixed costs.
+  // per CTA, which share the fixed costs (8192 tokens: 62 us, 65 us at eight
+  // CTAs per SM, i.e. half the tokens each).
   int sms = 0;
   const tp_status s = device_sms(&sms);
   if (s != TP_OK) return s;
