@@ -25,8 +25,8 @@ from torch import Tensor
 
 from . import _abi
 
-# 2^64 / (2 pi), from 60 digits of pi
-_TURNS = 2 ** 63 / Fraction("3.14159265358979323846264338327950288419716939937510582097494")
+# 2^192 / (2 pi), from 60 digits of pi
+_TURNS = int(2 ** 191 / Fraction("3.14159265358979323846264338327950288419716939937510582097494"))
 SCALINGS = ("default", "linear", "llama3", "yarn")
 
 
@@ -92,6 +92,13 @@ def rope_frequencies(rot_dim: int, theta: float = 10000.0, scaling: dict | None 
     return inv * (1 - ramp) + inv / factor * ramp, float(attention)
 
 
+def _turn_word(f: float) -> int:
+    """round(f 2^64 / (2 pi)) mod 2^64 of an fp32 value, in whole numbers."""
+    mantissa, exponent = math.frexp(f)
+    shift = 152 - exponent  # f = n 2^(exponent - 24)
+    return ((int(mantissa * 2 ** 24) * _TURNS + (1 << (shift - 1))) >> shift) % 2 ** 64
+
+
 class Rotary:
     """Rotary positions of one model: its frequencies, laid out once."""
 
@@ -111,7 +118,7 @@ class Rotary:
         if not torch.isfinite(self.inv_freq).all():
             raise ValueError("inv_freq must be finite")
         # turns per position as 64-bit fractions of a turn; whole turns drop out
-        words = [round(Fraction(f) * _TURNS) % 2 ** 64 for f in self.inv_freq.tolist()]
+        words = [_turn_word(f) for f in self.inv_freq.tolist()]
         self.freq = torch.tensor([w - 2 ** 64 if w >= 2 ** 63 else w for w in words], dtype=torch.int64).to(device)
         self.device = self.freq.device
         self._plans: dict[tuple, _RotaryArgs] = {}
