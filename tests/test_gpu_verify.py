@@ -72,6 +72,22 @@ def test_mixed_temperatures():
         _check(x)
 
 
+def test_low_temperatures_keep_their_digits():
+    """Acceptance at the edge: at temperature 1e-3 two near logits share the
+    probability; uniforms 1e-3 relative below and above p decide (fp32 logits
+    near 20 make m / t about 2^15, so p depends on x - m being taken first)."""
+    from turbopress_b200.speculative import DraftVerifier
+    x = _inputs(2, 1, 4096, torch.float32, 60, False, 1e-3)
+    g = torch.Generator(device=DEV).manual_seed(60)
+    x["logits"] = torch.randn(2, 2, 4096, generator=g, device=DEV)
+    x["logits"][:, 0, 100], x["logits"][:, 0, 3000] = 20.0, 20.0 - 4.0e-4
+    x["draft_tokens"].fill_(100)
+    p = torch.softmax(x["logits"][:, 0].double() / 1e-3, -1)[:, 100]
+    x["uniforms"] = torch.stack((p[:1] * (1 - 1e-4), p[1:] * (1 + 1e-4))).float()
+    accepted, _ = DraftVerifier(2, 1, 4096)(**x)
+    assert accepted.tolist() == [1, 0]
+
+
 def test_all_greedy_without_random_numbers():
     x = _inputs(3, 4, 5003, torch.bfloat16, 1, False, 0.0)
     x["draft_tokens"][0] = x["logits"][0, :4].float().argmax(-1)

@@ -129,7 +129,7 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, const longlong2*
 template <int THREADS, int COPIES>
 __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ EvictParams p) {
   constexpr int WARPS = THREADS / 32, D = kEvBins / THREADS;  // D: digits per thread
-  extern __shared__ uint32_t s_dyn[];
+  extern __shared__ __align__(16) uint32_t s_dyn[];
   uint32_t* hist = s_dyn;                              // [copies][bins]; then the (to, from) slots of fused moves
   uint32_t* kept = s_dyn + COPIES * kEvBins;           // a bit per slot: key above the threshold
   uint32_t* level = kept + (p.capacity + 31) / 32;     // a bit per slot: key equal to it

@@ -178,11 +178,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 // 2^x to 2 ulp; below 2^-126 it gives 0, which no sum or comparison here notices.
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
@@ -361,9 +356,9 @@ __global__ void __launch_bounds__(kVfThreads, kVfResident) verify_rows_kernel(co
     });
     if (at >= 0) best = argmax_key(top, at);
   } else {
-    // Elements two at a time: 2^(x c - m c), the sum in four parts.  (Rounding
-    // m c scales a thread's sum by 2^-24 |m c| at most, 1e-6.)
-    uint64_t sum[2] = {0ull, 0ull}, mc2 = 0ull;
+    // Elements two at a time: 2^((x - m) c), the sum in four parts.  (x c - m c
+    // in one instruction would lose 2^-24 |m c|, much at low temperatures.)
+    uint64_t sum[2] = {0ull, 0ull}, less = 0ull;
     const uint64_t c2 = pack2(make_float2(c, c));
     auto raise = [&](float t) {  // to a new maximum
       const float f = m == -INFINITY ? 0.f : exp2f((m - t) * c);
@@ -372,7 +367,7 @@ __global__ void __launch_bounds__(kVfThreads, kVfResident) verify_rows_kernel(co
       sum[0] = mul2(sum[0], f2);
       sum[1] = mul2(sum[1], f2);
       m = t;
-      mc2 = pack2(make_float2(-t * c, -t * c));
+      less = pack2(make_float2(-t, -t));
     };
     auto one = [&](int, float x) {
       if (x == -INFINITY) return;
@@ -387,7 +382,7 @@ __global__ void __launch_bounds__(kVfThreads, kVfResident) verify_rows_kernel(co
       for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int e = 0; e < 8 / (int)sizeof(T); ++e) {
-          const float2 y = unpack2(fma2(pack2(Two<T>::at(w[u], e)), c2, mc2));
+          const float2 y = unpack2(mul2(add2(pack2(Two<T>::at(w[u], e)), less), c2));
           sum[e & 1] = add2(sum[e & 1], pack2(make_float2(exp2_fast(y.x), exp2_fast(y.y))));
         }
     });
