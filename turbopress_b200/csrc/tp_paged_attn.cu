@@ -806,7 +806,8 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
 // accumulated weights: scores[b][h][s] += sum over the rows of 2^(s - lse)
 // from the scores that the attention kernel left in the workspace (16 bytes a
 // slot and four rows, against head_dim * 2 for reading K again).  Five tokens of
-// eight sequences, 7900 slots: 9 us of 30, most of it the read of those scores.
+// eight sequences, 7900 slots: 4 us of 24, a chain of round trips (30 us with
+// eight rows' loads together, i.e. one round trip more).
 // ---------------------------------------------------------------------------
 template <class S>
 __global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_constant__ AttnParams p) {
@@ -849,16 +850,16 @@ __global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_
         const float* s = p.sbuf + (size_t)(off + h * (kItemCost + nt) + kItemCost + tile) * RT * TILE + tok;
         const float* z = p.lse2 + ((int64_t)b * p.kv_heads + h) * p.rows + rt * RT;
         const int rows = min(RT, p.rows - rt * RT);
-        for (int r = 0; r < rows; r += 8) {  // eight rows' loads together
-          float a[8], m[8];
+        for (int r = 0; r < rows; r += 16) {  // sixteen rows' loads together: one round trip for most calls
+          float a[16], m[16];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
+          for (int k = 0; k < 16; ++k) {
             const int at = min(r + k, rows - 1);
             a[k] = s[at * TILE];
             m[k] = z[at];
           }
 #pragma unroll
-          for (int k = 0; k < 8; ++k) w += r + k < rows ? exp2_diff(a[k], m[k]) : 0.f;
+          for (int k = 0; k < 16; ++k) w += r + k < rows ? exp2_diff(a[k], m[k]) : 0.f;
         }
       }
       off += p.kv_heads * (kItemCost + nt);
