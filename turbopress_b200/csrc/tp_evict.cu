@@ -37,7 +37,9 @@ constexpr int kEvBins = 2048;
 // slots 9.7 against 10.1 us.
 constexpr int kEvSmall = 2048;      // capacity up to which 256 threads do
 constexpr int kMvThreads = 256;
-constexpr int kMvRows = 4;          // rows in flight per group of lanes
+// Rows in flight per group of lanes: four where one CTA moves its own few (one
+// round for 64), two in the launch over the GPU (more CTAs instead).
+constexpr int kMvOwn = 4, kMvRows = 2;
 // Moves per head up to which the selecting CTA does them itself: 64 moves in
 // each of 64 heads take 7.9 us in all so and 11.6 us with the second launch,
 // 256 moves 10.3 against 14.6 us, 512 the same in both.
@@ -99,25 +101,26 @@ __device__ __forceinline__ void block_prefix(const uint32_t (&v)[N], uint32_t (*
 }
 
 // Moves rows [first, n) step by step: K and V of a slot by a group of lanes,
-// kMvRows rows in flight.
+// R rows in flight.
+template <int R>
 __device__ __forceinline__ void move_rows(const EvictParams& p, const longlong2* moves, int n, int first, int step, int chunk) {
   if (chunk * 8 >= p.head_dim) return;
-  for (int i0 = first; i0 < n; i0 += kMvRows * step) {
-    longlong2 m[kMvRows];
-    uint4 kv[kMvRows], vv[kMvRows];
+  for (int i0 = first; i0 < n; i0 += R * step) {
+    longlong2 m[R];
+    uint4 kv[R], vv[R];
 #pragma unroll
-    for (int u = 0; u < kMvRows; ++u) {
+    for (int u = 0; u < R; ++u) {
       const int i = i0 + u * step;
       m[u] = i < n ? moves[i] : make_longlong2(-1, -1);
     }
 #pragma unroll
-    for (int u = 0; u < kMvRows; ++u)
+    for (int u = 0; u < R; ++u)
       if (m[u].x >= 0 && m[u].y >= 0) {
         kv[u] = *reinterpret_cast<const uint4*>(p.k_pages + 2 * (m[u].x + chunk * 8));
         vv[u] = *reinterpret_cast<const uint4*>(p.v_pages + 2 * (m[u].x + chunk * 8));
       }
 #pragma unroll
-    for (int u = 0; u < kMvRows; ++u)
+    for (int u = 0; u < R; ++u)
       if (m[u].x >= 0 && m[u].y >= 0) {
         *reinterpret_cast<uint4*>(p.k_pages + 2 * (m[u].y + chunk * 8)) = kv[u];
         *reinterpret_cast<uint4*>(p.v_pages + 2 * (m[u].y + chunk * 8)) = vv[u];
@@ -358,7 +361,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     return;
   }
   __syncthreads();
-  move_rows(p, list, moves, tid >> p.lg_lanes, THREADS >> p.lg_lanes, tid & ((1 << p.lg_lanes) - 1));
+  move_rows<kMvOwn>(p, list, moves, tid >> p.lg_lanes, THREADS >> p.lg_lanes, tid & ((1 << p.lg_lanes) - 1));
 }
 
 template <int THREADS, int COPIES>
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(kMvThreads) evict_move_kernel(const __grid_con
   pdl_wait();
   const int64_t bh = blockIdx.y;
   const int rows = kMvThreads >> p.lg_lanes;
-  move_rows(p, p.moves + bh * p.max_moves, p.moved[bh], blockIdx.x * rows + (threadIdx.x >> p.lg_lanes), gridDim.x * rows,
+  move_rows<kMvRows>(p, p.moves + bh * p.max_moves, p.moved[bh], blockIdx.x * rows + (threadIdx.x >> p.lg_lanes), gridDim.x * rows,
             threadIdx.x & ((1 << p.lg_lanes) - 1));
 }
 
@@ -458,9 +461,10 @@ TP_API tp_status tp_cache_evict(const tp_evict_args* args, const tp_paged_cache*
   int sms = 0;
   s = device_sms(&sms);
   if (s != TP_OK) return s;
-  // about eight CTAs per SM in all, never more than the rows that may move
+  // about 32 CTAs per SM in all (many end at once: their heads move little), never
+  // more than the rows that may move; with 8 and four rows in flight 7 % slower
   const int rows = (kMvThreads >> p.lg_lanes) * kMvRows;
-  const int64_t per_head = std::max<int64_t>(1, std::min<int64_t>((max_moves + rows - 1) / rows, (8 * sms + heads - 1) / heads));
+  const int64_t per_head = std::max<int64_t>(1, std::min<int64_t>((max_moves + rows - 1) / rows, (32 * sms + heads - 1) / heads));
   return launch_early(evict_move_kernel, dim3(static_cast<unsigned>(per_head), heads), kMvThreads, 0, st, "evict_move launch", p);
 }
 
