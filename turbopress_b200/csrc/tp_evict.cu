@@ -16,10 +16,10 @@
 // that selected them; many by a second launch over the whole GPU.
 //
 // Measured (B200, whole calls): 64 of 1088 slots in each of 64 heads 8.0 us;
-// 16 sequences of up to 16384 slots cut to 2048 37 us, of which the longest
-// heads' selection about 20 (four passes' barriers and collisions) and the
-// moves 16 (86 MB, 5.4 TB/s).  A cluster of CTAs per head that adds its counts
-// up through distributed shared memory was slower at every length (65 us).
+// 16 sequences of up to 16384 slots cut to 2048 35 us, of which the longest
+// heads' selection about 20 (the passes' barriers and collisions) and the moves
+// 14 (86 MB, 6 TB/s).  A cluster of CTAs per head that adds its counts up
+// through distributed shared memory was slower (65 us).
 #include <algorithm>
 
 #include "tp_decode.cuh"
