@@ -214,6 +214,45 @@ def test_offsets_past_32_bits():
     assert torch.allclose(out[0, 1], (k[0, 0] + k[0, 1]) / 65, rtol=0, atol=2e-4)
 
 
+def test_calls_of_other_kinds_in_turn():
+    """One Rotary and one cache over dtypes, strides and position types in
+    turn: what was checked for one call is not taken for another."""
+    from turbopress_b200.paged import PagedKVCache
+    from turbopress_b200.rotary import Rotary
+    rotary = Rotary(64)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    base = torch.randn(2, 3, 4, 128, generator=g, device=DEV)
+    pos = torch.randint(0, 500, (2, 3), generator=g, device=DEV)
+    wide = torch.zeros(2, 6, dtype=torch.int64, device=DEV)
+    wide[:, ::2] = pos
+    for _ in range(2):
+        for dtype in (torch.float16, torch.bfloat16, torch.float32):
+            x = base.to(dtype)
+            for q, k in ((x[..., :64], x[:, :, :2, 64:]), (x[..., :64].contiguous(), x[:, :, :2, 64:].contiguous()),
+                         (x.transpose(0, 1)[..., :64].transpose(0, 1), x[:, :, 1:3, :64]), (x[..., ::2], x[:, :, ::2, 1::2])):
+                for p in (pos, pos.int(), wide[:, ::2]):
+                    yq, yk = rotary(q, k, p)
+                    _near(yq, R.rotate(q, pos, rotary.inv_freq), dtype)
+                    _near(yk, R.rotate(k, pos, rotary.inv_freq), dtype)
+        with pytest.raises(ValueError):
+            rotary(base[..., :64], base[..., 64:], pos.cpu())
+        with pytest.raises(ValueError):
+            rotary(base[..., :64], base[..., 64:].cpu(), pos)
+    cache = PagedKVCache(2, 2, 64, 8, 16, 2)
+    cache.block_table.copy_(torch.arange(4, device=DEV).view(2, 2))
+    for T in (1, 3, 2, 3):
+        q, kv = base[:, :T, :, :64].half(), base[:, :T, :2, 64:].half()
+        out = cache.append(rotary, q, kv, kv)
+        at = cache.next_pos.long()[:, None] + torch.arange(T, device=DEV)
+        _near(out, R.rotate(q, at, rotary.inv_freq), torch.float16)
+        cache.advance(T)
+    assert cache.lengths.tolist() == [9, 9] == cache.next_pos.tolist()
+    with pytest.raises(ValueError):
+        cache.append(rotary, base[:, :1, :, :64].bfloat16(), base[:, :1, :2, 64:].bfloat16(), base[:, :1, :2, 64:].bfloat16())
+    with pytest.raises(ValueError):
+        cache.append(rotary, base[:, :1, :, :64].half(), base[:, :1, :2, 64:].half(), base[:, :1, :2, 64:].half().cpu())
+
+
 def test_refusals():
     from turbopress_b200.paged import PagedKVCache
     from turbopress_b200.rotary import Rotary
