@@ -89,6 +89,23 @@ def test_long_caches():
     _check(cache, 2047)
 
 
+@pytest.mark.parametrize("slots,budget,tied", [(50_000, 3001, False), (50_000, 40_000, True), (40_960, 20_479, True)])
+def test_caches_past_the_shared_memory(slots, budget, tied):
+    """Keys formed anew in each pass (above 40960 slots), more words than threads, many equal scores."""
+    cache, g = _cache([slots, slots - 12_345], 1, 8, 32, -(-slots // 32), seed=12)
+    if tied:
+        cache.scores.copy_(torch.randint(0, 3, cache.scores.shape, generator=g, device=DEV).float())
+    _check(cache, budget, recent=64, sinks=4)
+
+
+@pytest.mark.parametrize("slots", [203, 2051, 4098])
+def test_capacities_of_odd_size(slots):
+    """Pages of one slot: rows of scores and positions that are not 16-byte aligned."""
+    cache, _ = _cache([slots, slots - 1, slots // 2], 2, 16, 1, slots, seed=slots)
+    for budget in (50, slots // 2 + 1, slots - 2):
+        _check(cache, budget, recent=7, sinks=2)
+
+
 def test_budget_past_the_capacity_or_the_lengths():
     cache, _ = _cache([64, 3], 2, 64, 16, 4, seed=6)
     for budget in (64, 65, 1000):

@@ -94,6 +94,19 @@ def test_attention(T, hq, hk, dim, page, lengths, dtype):
     assert torch.equal(out, cache.attend(q))  # the same bits again: the joins do not depend on timing
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lengths", ["short", "ragged", "idle"])
+@pytest.mark.parametrize("T,hq,hk,dim,page", [(3, 16, 2, 128, 16), (5, 10, 2, 64, 32), (6, 4, 1, 256, 16), (17, 2, 2, 72, 4),
+                                              (32, 1, 1, 128, 64), (2, 31, 1, 64, 16), (16, 3, 3, 256, 8), (7, 9, 1, 200, 2)])
+def test_seventeen_rows_and_more(T, hq, hk, dim, page, lengths, dtype):
+    """Two and four row tiles per item at each width, partly empty ones among them."""
+    cache, g = _cache(LENGTHS[lengths], T, hk, dim, page, dtype, T * hq + dim, track=True)
+    q = torch.randn(cache.batch, T, hq, dim, generator=g, device=DEV).to(dtype)
+    out = _check(cache, q)
+    _check(cache, q, accumulate=True)
+    assert torch.equal(out, cache.attend(q))
+
+
 def test_token_major_pages_and_scale():
     cache, g = _cache([100, 37], 2, 4, 64, 16, torch.float16, 1, token_major=True)
     _check(cache, torch.randn(2, 2, 8, 64, generator=g, device=DEV).half(), scale=0.05)
