@@ -5,8 +5,9 @@
 // join as m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m), o likewise, and
 // out = o / l.  m, l, o, s are fp32.  The products run on the tensor cores
 // with fp32 accumulation; q, k, v enter exactly (they are 16-bit) and the
-// probabilities as two 16-bit terms (p = hi + lo, 2^-16 relative or better),
-// so the output is rounded once.
+// probabilities as two 16-bit terms (bf16: 2^-16 relative or better; fp16, taken
+// times 2^15 for its short range: 2^-21 relative, and 2^-40 of the row's largest
+// at least), so the output is rounded once.
 //
 // Bound: memory.  A cached token costs 4 * head_dim bytes per kv head and
 // 4 * head_dim * rows flops; with few rows (query heads of a kv head times
@@ -101,6 +102,10 @@ template <class T>
 struct Mma;
 template <>
 struct Mma<__half> {
+  // What the probabilities are taken times: at most 2^15 then, so fp16 keeps
+  // them down to 2^-39 of the row's largest (1 in its place would lose all
+  // below 2^-25, a long flat tail under one large score).
+  static constexpr float kScale = 32768.f;
   // either half infinite or NaN: its exponent is all ones
   static __device__ __forceinline__ bool not_finite(uint32_t v) {
     constexpr uint32_t E = 0x7c007c00u;
@@ -122,6 +127,7 @@ struct Mma<__half> {
 };
 template <>
 struct Mma<__nv_bfloat16> {
+  static constexpr float kScale = 1.f;  // fp32's range
   // either half infinite or NaN: its exponent is all ones
   static __device__ __forceinline__ bool not_finite(uint32_t v) {
     constexpr uint32_t E = 0x7f807f80u;
@@ -543,17 +549,21 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
         }
         const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
         uint32_t ph[NB][4], pl[NB][4];
+        float add[2] = {0.f, 0.f};  // (the block's sum first: many small terms beside a large l then lose little)
 #pragma unroll
         for (int n = 0; n < 2 * NB; ++n) {
           s[n][0] = exp2f(s[n][0] - b0);
           s[n][1] = exp2f(s[n][1] - b0);
           s[n][2] = exp2f(s[n][2] - b1);
           s[n][3] = exp2f(s[n][3] - b1);
-          l[0] += s[n][0] + s[n][1];
-          l[1] += s[n][2] + s[n][3];
-          Mma<T>::split(s[n][0], s[n][1], ph[n / 2][n % 2 * 2], pl[n / 2][n % 2 * 2]);
-          Mma<T>::split(s[n][2], s[n][3], ph[n / 2][n % 2 * 2 + 1], pl[n / 2][n % 2 * 2 + 1]);
+          add[0] += s[n][0] + s[n][1];
+          add[1] += s[n][2] + s[n][3];
+          constexpr float C = Mma<T>::kScale;
+          Mma<T>::split(s[n][0] * C, s[n][1] * C, ph[n / 2][n % 2 * 2], pl[n / 2][n % 2 * 2]);
+          Mma<T>::split(s[n][2] * C, s[n][3] * C, ph[n / 2][n % 2 * 2 + 1], pl[n / 2][n % 2 * 2 + 1]);
         }
+        l[0] += add[0];
+        l[1] += add[1];
         // o += P V, 16-column pairs at a time (independent products in a row);
         // `keep` masks the V fragments' two tokens of each 8 where MASKED
         auto v_frag = [&](int i, int nn, uint32_t (&vf)[4]) {
@@ -685,7 +695,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
       constexpr int N = sizeof(v) / sizeof(float);
       const int row = done.rt * RT + r, j = token_of(p, row);
       const int64_t at = out0 + (int64_t)j * p.q_heads + row - j * p.group;
-      const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+      const float inv = L > 0.f || L != L ? 1.f / (L * Mma<T>::kScale) : 0.f;
       if (d < p.head_dim) {
         Pack<T, N> w;
 #pragma unroll
