@@ -56,3 +56,48 @@ def test_a_flat_tail_below_one_large_score(heads, nats, dtype):
     err = (out.double() - want).abs() / want
     assert float(err.max()) <= HALF_ULP[dtype] + 2 * 2.0 ** -15 + 2.0 ** -16 + 2.0 ** -14 + 2.0 ** -25 / float(want.min())
     assert float((lse.double() - (top + math.log(total))).abs().max()) <= 2.0 ** -15
+
+
+def _values(cache, n):
+    from tests import paged_reference as R
+    return R.slots_of(cache.v_pages[0], cache.block_table[0], n)[0].double()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,hq,hk,dim,page", [(1, 4, 2, 128, 16), (1, 24, 1, 64, 16), (1, 40, 1, 128, 32), (4, 8, 1, 64, 8), (3, 32, 2, 256, 16),
+                                              (5, 20, 2, 72, 4)])
+def test_infinite_values_in_seen_slots(T, hq, hk, dim, page, dtype):
+    """A value of +-inf gives +-inf to the rows that see its slot (whatever
+    the slot's weight: the row's largest, a usual one or a very small one), NaN
+    where both signs meet, and nothing to other rows and columns."""
+    from tests import paged_reference as R
+    from turbopress_b200.paged import PagedKVCache
+    g = torch.Generator(device=DEV).manual_seed(T * hq + dim)
+    n = 700
+    P = -(-(n + T) // page)
+    kp, vp = (torch.randn(P, hk, page, dim, generator=g, device=DEV).to(dtype) for _ in range(2))
+    table = torch.randperm(P, generator=g, device=DEV).int()[None].contiguous()
+    cache = PagedKVCache.from_tensors(kp, vp, table, torch.tensor([n], dtype=torch.int32, device=DEV))
+    q = torch.randn(1, T, hq, dim, generator=g, device=DEV).to(dtype)
+
+    def at(slot):  # where a slot lies
+        return int(table[0, slot // page]), slot % page
+
+    # one slot with the row's largest score, one 20 nats below the others
+    page_id, off = at(40)
+    kp[page_id, :, off] = q[0, 0, ::hq // hk][:hk] * 2
+    page_id, off = at(41)
+    kp[page_id, :, off] = q[0, 0, ::hq // hk][:hk] * -1
+    for i, (slot, col, val) in enumerate([(0, 0, math.inf), (40, 1, -math.inf), (41, 2, math.inf), (100, 3, -math.inf), (333, 4, math.inf),
+                                          (n - 1, 5, math.inf), (n, 6, -math.inf), (n + T - 1, 7, math.inf), (255, 3, math.inf)]):
+        page_id, off = at(slot)
+        vp[page_id, :, off, col] = val
+    out = cache.attend(q)
+    want, _, _ = R.attention(q, kp, vp, table, cache.lengths)
+    assert torch.isinf(want).any() and torch.isnan(want[..., 3]).all()
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    sign = torch.where(torch.isinf(want), want.sign(), 0.0)
+    assert torch.equal(torch.where(torch.isinf(out), out.sign(), 0.0).double(), sign)
+    fine = torch.isfinite(want)
+    tol = HALF_ULP[dtype] * want.abs() * (1 + 2.0 ** -6) + 4 * 2.0 ** -15 * 6
+    assert ((out.double() - want).abs() <= tol)[fine].all()

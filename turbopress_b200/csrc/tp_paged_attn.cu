@@ -5,9 +5,9 @@
 // join as m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m), o likewise, and
 // out = o / l.  m, l, o, s are fp32.  The products run on the tensor cores
 // with fp32 accumulation; q, k, v enter exactly (they are 16-bit) and the
-// probabilities as two 16-bit terms (bf16: 2^-16 relative or better; fp16, taken
-// times 2^15 for its short range: 2^-21 relative, and 2^-40 of the row's largest
-// at least), so the output is rounded once.
+// probabilities as two 16-bit terms, hi cut off and lo rounded (bf16: within 2^-16
+// relative; fp16, taken times 2^15 for its short range: 2^-21 relative, or 2^-38 of
+// the row's largest where that is more), so the output is rounded once.
 //
 // Bound: memory.  A cached token costs 4 * head_dim bytes per kv head and
 // 4 * head_dim * rows flops; with few rows (query heads of a kv head times
@@ -98,6 +98,9 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
                : "memory");
 }
 
+// Mma<T>::split: x = hi + lo for x, y >= 0.  hi is x cut off and lo the rest, both
+// raised to the type's least positive (bf16: normal) value: an infinite V times a
+// term of 0, or of the other sign, would make NaN of an infinite output.
 template <class T>
 struct Mma;
 template <>
@@ -118,11 +121,14 @@ struct Mma<__half> {
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   static __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x, y);
+    __half2 h;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(reinterpret_cast<uint32_t&>(h)) : "f"(y), "f"(x));
+    const __half2 least = __halves2half2(__ushort_as_half(1), __ushort_as_half(1));
     const float2 f = __half22float2(h);
-    const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&r);
+    const __half2 r = __hmax2(__floats2half2_rn(x - f.x, y - f.y), least);
+    h = __hmax2(h, least);
+    hi = reinterpret_cast<const uint32_t&>(h);
+    lo = reinterpret_cast<const uint32_t&>(r);
   }
 };
 template <>
@@ -140,11 +146,14 @@ struct Mma<__nv_bfloat16> {
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   static __device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    __nv_bfloat162 h;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(reinterpret_cast<uint32_t&>(h)) : "f"(y), "f"(x));
+    const __nv_bfloat162 least = __halves2bfloat162(__ushort_as_bfloat16(0x80), __ushort_as_bfloat16(0x80));
     const float2 f = __bfloat1622float2(h);
-    const __nv_bfloat162 r = __floats2bfloat162_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&r);
+    const __nv_bfloat162 r = __hmax2(__floats2bfloat162_rn(x - f.x, y - f.y), least);
+    h = __hmax2(h, least);
+    hi = reinterpret_cast<const uint32_t&>(h);
+    lo = reinterpret_cast<const uint32_t&>(r);
   }
 };
 
@@ -564,6 +573,16 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
         }
         l[0] += add[0];
         l[1] += add[1];
+        if (!whole) {  // slots that a row does not see have no weight at all
+#pragma unroll
+          for (int n = 0; n < 2 * NB; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t some = (s[n][2 * e] > 0.f ? 0x0000ffffu : 0u) | (s[n][2 * e + 1] > 0.f ? 0xffff0000u : 0u);
+              ph[n / 2][n % 2 * 2 + e] &= some;
+              pl[n / 2][n % 2 * 2 + e] &= some;
+            }
+        }
         // o += P V, 16-column pairs at a time (independent products in a row);
         // `keep` masks the V fragments' two tokens of each 8 where MASKED
         auto v_frag = [&](int i, int nn, uint32_t (&vf)[4]) {
