@@ -493,8 +493,9 @@ typedef struct tp_paged_attn_args {
 
 /* Workspace of tp_paged_attn for a cache's sizes (batch, kv_heads, head_dim,
  * page_size and max_pages of `cache` are read): zero-filled once, left fit
- * for the next call of any such size that it can hold; one per stream.  Minus
- * the status on bad arguments. */
+ * for the next call of any such size that it can hold; one per stream.  With
+ * `accumulate` four bytes per row more, and up to 1 GiB for the scores of calls
+ * of a few rows.  Minus the status on bad arguments. */
 TP_API int64_t tp_paged_attn_workspace_bytes(const tp_paged_cache* cache, int tokens, int q_heads, int accumulate);
 TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_cache* cache, void* workspace,
                                int64_t workspace_bytes, void* stream);

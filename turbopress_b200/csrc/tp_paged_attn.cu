@@ -54,7 +54,9 @@ namespace {
 // 8000 tokens 81 us, against 101 us with equal tile counts.
 constexpr int kItemCost = 2;
 constexpr int kPaMaxCtas = 512;
+constexpr int64_t kPaStoredMax = int64_t(1) << 30;  // bytes of stored scores
 constexpr int kWtThreads = 128;
+constexpr int kWtRound = 32;  // row tiles whose weights are summed before they join the slot's
 constexpr int kPaStatusOff = kPaMaxCtas * 4;      // status word after the counters
 constexpr int kPaCounterBytes = kPaStatusOff + 256;
 
@@ -79,8 +81,10 @@ struct AttnParams {
   unsigned* status;
   float* part_o;   // [ctas][2][16*MT][HD]
   float2* part_ml; // [ctas][2][16*MT]
-  float* lse2;     // [batch][kv_heads][rows] log2 units (accumulate only)
-  float* sbuf;     // [index space][16*MT][TILE] scores in log2 units (accumulate only)
+  float* lse2;     // log2 units (accumulate only): [batch][tokens][q_heads], with stored scores [batch][kv_heads][rows]
+  float* sbuf;     // [index space][16*MT][TILE] scores in log2 units (stored scores only)
+  const void* k_pages;  // and its strides, in elements (accumulate only)
+  int64_t page_stride, head_stride, token_stride;
 };
 
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int token, int head, int page,
@@ -310,7 +314,8 @@ __device__ __forceinline__ void consumers_sync() {  // of N threads; the produce
   asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
 }
 
-template <class T, int HD, int MT, bool WEIGHTS>
+// STORE: the scores go to the workspace.
+template <class T, int HD, int MT, bool STORE>
 __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel(const __grid_constant__ AttnParams p) {
   using S = PaShape<HD, MT>;
   constexpr int RT = S::RT, W = S::W, WT = S::WT, NB = MT == 1 || HD == 256 ? 1 : 2, kStages = S::kStages;
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
   int per, t0, t1, before;
   Cursor c;
   pdl_wait();
-  pdl_trigger();  // after the wait: the weights kernel reads the lengths at once
+  pdl_trigger();  // after the wait: the weights kernel of stored scores reads the lengths at once
   // (its barriers also publish the mbarriers)
   if (!find_share<W + 4>(p, [&](int len) { return seq_size<S>(p, len); }, s_tmp, per, t0, t1, c.b, c.len, before)) return;
   int rem = t0 - before;
@@ -480,7 +485,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
       for (int blk = tw * MT; blk < (tw + 1) * MT; blk += NB) {
         const int tok0 = c.tile * S::TILE + blk * 16;
         if (tok0 >= vis_hi) {  // nothing here for these rows
-          if (WEIGHTS)
+          if (STORE)
             for (int i = 0; i < NB; ++i) store_scores(blk + i, nullptr);
           continue;
         }
@@ -527,7 +532,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
               if (!((valid[n / 2] >> (col & 15)) & 1u) || tok0 + col >= vis[e >> 1]) s[n][e] = -INFINITY;
             }
         }
-        if (WEIGHTS) {
+        if (STORE) {
 #pragma unroll
           for (int i = 0; i < NB; ++i) store_scores(blk + i, s + 2 * i);
         }
@@ -724,7 +729,8 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
       if (d == 0) {
         const float lg = L > 0.f || L != L ? M + log2f(L) : -INFINITY;
         if (p.lse) p.lse[at] = lg * 0.6931471805599453f;
-        if (WEIGHTS) p.lse2[((int64_t)done.b * p.kv_heads + done.h) * p.rows + row] = lg;
+        if (STORE) p.lse2[((int64_t)done.b * p.kv_heads + done.h) * p.rows + row] = lg;
+        else if (p.lse2) p.lse2[at] = lg;
       }
     };
     for (int i = tid; i < nrow * (HD / 4); i += 32 * W) {
@@ -833,38 +839,169 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
 
 // ---------------------------------------------------------------------------
 // accumulated weights: scores[b][h][s] += sum over the rows of 2^(s - lse)
-// from the scores that the attention kernel left in the workspace (16 bytes a
+//
+// The normaliser is known only when a row has met all its slots, so every slot
+// is looked at twice.  Few rows leave their scores in the workspace (two
+// kernels below, plan_attn has the rule); else the scores are computed again,
+// from K and the rows' log-sum-exp: a warp holds the K of its slots in registers
+// as the products' second operand and walks the rows, 16 at a time, that see
+// any of them.  Either way a slot's sum is made by one warp or thread, so the
+// result does not depend on timing.
+//
+// Measured: 512 tokens of 32 / 8 heads over 8000 slots 777 us, of which 365 are
+// the attention; from stored scores 955 us and 580 MB of workspace, where the
+// sequence's K and V take 35 MB.
+// ---------------------------------------------------------------------------
+struct WtShape {
+  static constexpr int W = kWtThreads / 32;
+  static constexpr int NS = 2;  // blocks of 8 slots per warp (four: 902 us, fewer CTAs fit)
+  static constexpr int SLOTS = 8 * NS;
+  static constexpr int TILE = W * SLOTS;
+};
+
+template <class T, int HD>
+__global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_constant__ AttnParams p) {
+  using S = WtShape;
+  constexpr int W = S::W, NS = S::NS;
+  __shared__ int s_tmp[W + 4];
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r0 = lane >> 2, cq = lane & 3;  // as in the attention kernel
+  auto tiles = [&](int len) { return (visible(p, len, p.rows - 1) + S::TILE - 1) / S::TILE; };
+  int per, t0, t1, b, len, before;
+  if (!find_share<W>(p, [&](int n) { return p.kv_heads * tiles(n); }, s_tmp, per, t0, t1, b, len, before)) return;
+  int n = tiles(len);
+  for (int t = t0; t < t1; ++t) {
+    while (t - before >= p.kv_heads * n) {
+      before += p.kv_heads * n;
+      len = p.lengths[++b];
+      n = tiles(len);
+    }
+    const int h = (t - before) / n, slot0 = ((t - before) - h * n) * S::TILE + warp * S::SLOTS;
+    const int rows = p.rows, hi = visible(p, len, rows - 1);
+    if (slot0 >= hi) continue;
+    // the slots' K: this lane's row of each block, the chunks of 8 columns as in the attention kernel
+    uint4 kf[NS][HD / 32];
+    uint32_t got[NS];  // bit 4 i: slot i of the block is there
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int slot = slot0 + 8 * i + r0;
+      const int page = slot < hi ? p.block_table[b * p.table_stride + (slot >> p.lg_page)] : -1;
+      const bool ok = page >= 0 && page < p.num_pages;
+      got[i] = __ballot_sync(0xffffffffu, ok);
+      all = all && got[i] == 0xffffffffu;
+      const T* k = static_cast<const T*>(p.k_pages) + (ok ? page * p.page_stride + h * p.head_stride +
+                                                                (slot & ((1 << p.lg_page) - 1)) * p.token_stride : 0);
+#pragma unroll
+      for (int kk = 0; kk < HD / 32; ++kk) {
+        const int chunk = (kk >> 1) * 8 + 2 * cq + (kk & 1);
+        kf[i][kk] = ok && chunk * 8 < p.head_dim ? *reinterpret_cast<const uint4*>(k + chunk * 8) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+    float* score = p.scores + ((int64_t)b * p.kv_heads + h) * p.capacity + slot0;
+    float was[NS][2], sum[NS][2];
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int at = 8 * i + 2 * cq + e;
+        was[i][e] = r0 == 0 && slot0 + at < hi ? score[at] : 0.f;
+        sum[i][e] = 0.f;
+      }
+    // rows from the first step token that sees the first slot; sums in two levels
+    for (int base = max(0, slot0 - len) * p.group & ~15; base < rows; base += 16 * kWtRound) {
+      float part[NS][2];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) part[i][0] = part[i][1] = 0.f;
+      const int end = min(rows, base + 16 * kWtRound);
+#pragma unroll 1
+      for (int row0 = base; row0 < end; row0 += 16) {
+        uint32_t qf[HD / 16][4];
+        float z[2];
+        int see[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = row0 + r0 + 8 * e, j = token_of(p, row);
+          const int64_t at = ((int64_t)b * p.tokens + j) * p.q_heads + h * p.group + row - j * p.group;
+          const bool on = row < rows;
+          const T* q = static_cast<const T*>(p.q) + at * p.head_dim;
+          z[e] = on ? p.lse2[at] : 0.f;
+          see[e] = on ? visible(p, len, row) : 0;
+#pragma unroll
+          for (int kk = 0; kk < HD / 32; ++kk) {
+            const int chunk = (kk >> 1) * 8 + 2 * cq + (kk & 1);
+            const uint4 x = on && chunk * 8 < p.head_dim ? __ldg(reinterpret_cast<const uint4*>(q + chunk * 8))
+                                                         : make_uint4(0u, 0u, 0u, 0u);
+            qf[2 * kk][e] = x.x;
+            qf[2 * kk][2 + e] = x.y;
+            qf[2 * kk + 1][e] = x.z;
+            qf[2 * kk + 1][2 + e] = x.w;
+          }
+        }
+        float s[NS][4];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < HD / 32; ++kk) {
+#pragma unroll
+          for (int i = 0; i < NS; ++i) Mma<T>::run(s[i], qf[2 * kk], kf[i][kk].x, kf[i][kk].y);
+#pragma unroll
+          for (int i = 0; i < NS; ++i) Mma<T>::run(s[i], qf[2 * kk + 1], kf[i][kk].z, kf[i][kk].w);
+        }
+        const bool whole = all && row0 + 16 <= rows && slot0 + S::SLOTS <= visible(p, len, row0);
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int col = 2 * cq + (e & 1);
+            const bool seen = whole || (((got[i] >> (4 * col)) & 1u) && slot0 + 8 * i + col < see[e >> 1]);
+            if (seen) part[i][e & 1] += exp2_diff(s[i][e] * p.scale_log2, z[e >> 1]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        sum[i][0] += part[i][0];
+        sum[i][1] += part[i][1];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int m = 4; m < 32; m <<= 1) sum[i][e] += __shfl_xor_sync(0xffffffffu, sum[i][e], m);
+        const int at = 8 * i + 2 * cq + e;
+        if (r0 == 0 && slot0 + at < hi) score[at] = was[i][e] + sum[i][e];
+      }
+  }
+}
+
+// From the scores that the attention kernel left in the workspace (16 bytes a
 // slot and four rows, against head_dim * 2 for reading K again).  Five tokens of
 // eight sequences, 7900 slots: 4 us of 24, a chain of round trips (30 us with
-// eight rows' loads together, i.e. one round trip more).
-// ---------------------------------------------------------------------------
+// eight rows' loads together, i.e. one round trip more; 28 us in all from K).
 template <class S>
-__global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kWtThreads) paged_stored_weights_kernel(const __grid_constant__ AttnParams p) {
   constexpr int W = kWtThreads / 32, RT = S::RT, TILE = S::TILE;
   __shared__ int s_tmp[W + 4];
   pdl_trigger();
   // The lengths are as old as the attention kernel's own inputs, which it had
-  // waited for before it let this one begin.
-  const int last = p.row_tiles - 1;
-  auto count = [&](int len) { return p.kv_heads * item_tiles<S>(p, len, last); };
+  // waited for before it let this one begin.  (All rows are in one row tile.)
+  auto count = [&](int len) { return p.kv_heads * item_tiles<S>(p, len, 0); };
   int per, t0, t1, b, len, before;
   if (!find_share<W>(p, count, s_tmp, per, t0, t1, b, len, before)) return;
-  // positions of the attention kernel's index space before sequence b
-  int base = before + b * p.kv_heads * kItemCost;
-  if (last > 0) {
-    int c1 = 0;
-    for (int i = threadIdx.x; i < b; i += kWtThreads) c1 += seq_size<S>(p, p.lengths[i]);
-    base = block_sum<W>(c1, s_tmp);
-  }
-  int n = item_tiles<S>(p, len, last);
+  int base = before + b * p.kv_heads * kItemCost;  // positions of the attention kernel's index space before sequence b
+  int n = item_tiles<S>(p, len, 0);
   pdl_wait();
   const int sub = threadIdx.x / TILE, tok = threadIdx.x % TILE;
   for (int t = t0 + sub; t < t1; t += kWtThreads / TILE) {
     while (t - before >= p.kv_heads * n) {
       before += p.kv_heads * n;
-      base += seq_size<S>(p, len);
+      base += p.kv_heads * (kItemCost + n);
       len = p.lengths[++b];
-      n = item_tiles<S>(p, len, last);
+      n = item_tiles<S>(p, len, 0);
     }
     const int h = (t - before) / n, tile = (t - before) - h * n;
     const int slot = tile * TILE + tok;
@@ -872,26 +1009,18 @@ __global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_
     float* score = p.scores + ((int64_t)b * p.kv_heads + h) * p.capacity + slot;
     const float was = *score;
     float w = 0.f;
-    int off = base;
-    for (int rt = 0; rt <= last; ++rt) {
-      const int nt = item_tiles<S>(p, len, rt);
-      if (tile < nt) {
-        const float* s = p.sbuf + (size_t)(off + h * (kItemCost + nt) + kItemCost + tile) * RT * TILE + tok;
-        const float* z = p.lse2 + ((int64_t)b * p.kv_heads + h) * p.rows + rt * RT;
-        const int rows = min(RT, p.rows - rt * RT);
-        for (int r = 0; r < rows; r += 16) {  // sixteen rows' loads together: one round trip for most calls
-          float a[16], m[16];
+    const float* s = p.sbuf + (size_t)(base + h * (kItemCost + n) + kItemCost + tile) * RT * TILE + tok;
+    const float* z = p.lse2 + ((int64_t)b * p.kv_heads + h) * p.rows;
+    for (int r = 0; r < p.rows; r += 16) {  // sixteen rows' loads together: one round trip for most calls
+      float a[16], m[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const int at = min(r + k, rows - 1);
-            a[k] = s[at * TILE];
-            m[k] = z[at];
-          }
-#pragma unroll
-          for (int k = 0; k < 16; ++k) w += r + k < rows ? exp2_diff(a[k], m[k]) : 0.f;
-        }
+      for (int k = 0; k < 16; ++k) {
+        const int at = min(r + k, p.rows - 1);
+        a[k] = s[at * TILE];
+        m[k] = z[at];
       }
-      off += p.kv_heads * (kItemCost + nt);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) w += r + k < p.rows ? exp2_diff(a[k], m[k]) : 0.f;
     }
     *score = was + w;
   }
@@ -902,6 +1031,7 @@ __global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_
 // ---------------------------------------------------------------------------
 struct PaPlan {
   int hd, mt, tile;
+  bool store;  // scores for the accumulated weights go through the workspace
   int64_t max_tiles, positions, ml_off, o_off, lse_off, s_off, bytes;
 };
 
@@ -931,10 +1061,14 @@ tp_status plan_attn(const tp_paged_cache* c, int tokens, int q_heads, int accumu
   };
   pl.ml_off = take((int64_t)kPaMaxCtas * 2 * rt * 8);
   pl.o_off = take((int64_t)kPaMaxCtas * 2 * rt * pl.hd * 4);
-  if (accumulate) {
-    pl.lse_off = take((int64_t)c->batch * c->kv_heads * rows * 4);
-    pl.s_off = take(pl.positions * rt * pl.tile * 4);
-  }
+  // Stored scores take rt * 4 bytes per slot of the capacity: for up to 32 rows
+  // (8000 slots of one sequence 33.5 us with the attention, 35.4 us from K; 16
+  // sequences, four rows 115 against 171 us; with 64 rows 45 against 38 us), and
+  // not where that workspace would grow past 1 GiB.
+  const int64_t stored = pl.positions * rt * pl.tile * 4;
+  pl.store = accumulate && rows <= 32 && stored <= kPaStoredMax;
+  if (accumulate) pl.lse_off = take((int64_t)c->batch * c->kv_heads * rows * 4);
+  if (pl.store) pl.s_off = take(stored);
   pl.bytes = at;
   *out = pl;
   return TP_OK;
@@ -982,44 +1116,48 @@ tp_status page_map(const tp_paged_cache* c, void* base, bool panels, int box, CU
   return TP_OK;
 }
 
-template <class T, int HD, int MT>
-tp_status launch_attn(const AttnParams& p, const PaPlan& pl, bool weights, cudaStream_t st) {
+template <class T, int HD, int MT, bool STORE>
+tp_status launch_attn(const AttnParams& p, const PaPlan& pl, cudaStream_t st) {
   using S = PaShape<HD, MT>;
   static_assert(S::TILE == (HD == 256 ? 64 : 128), "as plan_attn");
-  const auto kern = weights ? paged_attn_kernel<T, HD, MT, true> : paged_attn_kernel<T, HD, MT, false>;
-  static int smem_set[2][64];
-  static int ctas[2][64];  // resident CTAs per SM
-  tp_status s = ensure_smem(kern, S::kSmem, smem_set[weights], "paged_attn: shared memory attribute");
+  const auto kern = paged_attn_kernel<T, HD, MT, STORE>;
+  static int smem_set[64];
+  static int ctas[64];  // resident CTAs per SM
+  tp_status s = ensure_smem(kern, S::kSmem, smem_set, "paged_attn: shared memory attribute");
   if (s != TP_OK) return s;
   int sms = 0, dev = 0;
   s = device_sms(&sms);
   if (s != TP_OK) return s;
   TP_CUDA_TRY(cudaGetDevice(&dev), "cudaGetDevice");
-  int occ = __atomic_load_n(&ctas[weights][dev], __ATOMIC_RELAXED);
+  int occ = __atomic_load_n(&ctas[dev], __ATOMIC_RELAXED);
   if (!occ) {
     TP_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, kern, S::THREADS, S::kSmem), "paged_attn: occupancy");
     if (occ < 1) return fail(TP_ERR_CUDA, "paged_attn: the kernel does not fit this device");
-    __atomic_store_n(&ctas[weights][dev], occ, __ATOMIC_RELAXED);
+    __atomic_store_n(&ctas[dev], occ, __ATOMIC_RELAXED);
   }
   const int grid = static_cast<int>(std::min<int64_t>(std::min(kPaMaxCtas, sms * occ), pl.positions));
   s = launch_early(kern, dim3(grid), S::THREADS, S::kSmem, st, "paged_attn launch", p);
-  if (s != TP_OK || !weights) return s;
-  return launch_early(paged_weights_kernel<S>, dim3(static_cast<unsigned>(std::min<int64_t>(8 * sms, pl.max_tiles))),
-                      kWtThreads, 0, st, "paged_weights launch", p);
+  if (s != TP_OK || !p.lse2) return s;
+  auto blocks = [&](int64_t tiles) { return dim3(static_cast<unsigned>(std::min<int64_t>(8 * sms, tiles))); };
+  if constexpr (STORE)
+    return launch_early(paged_stored_weights_kernel<S>, blocks(pl.max_tiles), kWtThreads, 0, st, "paged_stored_weights launch", p);
+  else
+    return launch_early(paged_weights_kernel<T, HD>, blocks(pl.max_tiles * (S::TILE / WtShape::TILE)), kWtThreads, 0, st,
+                        "paged_weights launch", p);
 }
 
 template <class T, int HD>
-tp_status dispatch_rows(const AttnParams& p, const PaPlan& pl, bool weights, cudaStream_t st) {
-  if (pl.mt == 1) return launch_attn<T, HD, 1>(p, pl, weights, st);
-  if (pl.mt == 2) return launch_attn<T, HD, 2>(p, pl, weights, st);
-  return launch_attn<T, HD, 4>(p, pl, weights, st);
+tp_status dispatch_rows(const AttnParams& p, const PaPlan& pl, cudaStream_t st) {
+  if (pl.mt == 1) return pl.store ? launch_attn<T, HD, 1, true>(p, pl, st) : launch_attn<T, HD, 1, false>(p, pl, st);
+  if (pl.mt == 2) return pl.store ? launch_attn<T, HD, 2, true>(p, pl, st) : launch_attn<T, HD, 2, false>(p, pl, st);
+  return launch_attn<T, HD, 4, false>(p, pl, st);
 }
 
 template <class T>
-tp_status dispatch_dim(const AttnParams& p, const PaPlan& pl, bool weights, cudaStream_t st) {
-  if (pl.hd == 64) return dispatch_rows<T, 64>(p, pl, weights, st);
-  if (pl.hd == 128) return dispatch_rows<T, 128>(p, pl, weights, st);
-  return dispatch_rows<T, 256>(p, pl, weights, st);
+tp_status dispatch_dim(const AttnParams& p, const PaPlan& pl, cudaStream_t st) {
+  if (pl.hd == 64) return dispatch_rows<T, 64>(p, pl, st);
+  if (pl.hd == 128) return dispatch_rows<T, 128>(p, pl, st);
+  return dispatch_rows<T, 256>(p, pl, st);
 }
 
 }  // namespace
@@ -1080,12 +1218,16 @@ TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_ca
   p.status = reinterpret_cast<unsigned*>(ws + kPaStatusOff);
   p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_off);
   p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
-  p.lse2 = reinterpret_cast<float*>(ws + pl.lse_off);
-  p.sbuf = reinterpret_cast<float*>(ws + pl.s_off);
+  if (a.accumulate) {
+    p.lse2 = reinterpret_cast<float*>(ws + pl.lse_off);
+    p.sbuf = pl.store ? reinterpret_cast<float*>(ws + pl.s_off) : nullptr;
+    p.k_pages = cache->k_pages;
+    p.page_stride = cache->page_stride;
+    p.head_stride = cache->head_stride;
+    p.token_stride = cache->token_stride;
+  }
   cudaStream_t st = as_stream(stream);
-  const bool weights = a.accumulate != 0;
-  return cache->dtype == TP_F16 ? dispatch_dim<__half>(p, pl, weights, st)
-                                : dispatch_dim<__nv_bfloat16>(p, pl, weights, st);
+  return cache->dtype == TP_F16 ? dispatch_dim<__half>(p, pl, st) : dispatch_dim<__nv_bfloat16>(p, pl, st);
 }
 
 TP_API tp_status tp_paged_attn_status(void* workspace, void* stream) {
