@@ -500,6 +500,22 @@ TP_API int64_t tp_paged_attn_workspace_bytes(const tp_paged_cache* cache, int to
 TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_cache* cache, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* The accumulated weights of a step whose tokens may yet be dropped (drafts):
+ * tp_paged_attn without `accumulate`, and once it is known how many tokens
+ * stand, this call adds to cache->scores what `accumulate` would have, for each
+ * sequence's first counts[b] tokens (NULL: all), from the same queries and the
+ * log-sum-exp that the call gave.  Before the lengths are advanced.
+ * Deterministic; no workspace. */
+typedef struct tp_paged_weights_args {
+  const void* q;          /* as tp_paged_attn had them                       */
+  const float* lse;       /* [batch][tokens][q_heads], as it gave them       */
+  const int32_t* counts;  /* [batch], cut to 0..tokens, or NULL              */
+  int32_t tokens, q_heads;
+  float softmax_scale;
+  int32_t reserved;
+} tp_paged_weights_args;
+TP_API tp_status tp_paged_weights(const tp_paged_weights_args* args, const tp_paged_cache* cache, void* stream);
+
 /* Reads (synchronizing `stream`) and clears the status word of a workspace of
  * tp_paged_attn: TP_OK, or TP_ERR_DEVICE when a wait for a copy gave up (rows
  * of that call are NaN, and what they added to the scores; the workspace is

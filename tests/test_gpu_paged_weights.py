@@ -143,3 +143,97 @@ def _weights_small(q, cache):
         k, _ = R.slots_of(cache.k_pages[0], cache.block_table[b], n)
         w[b, 0, :n] = torch.softmax(q[b, 0].double() @ k[:, 0].double().T * q.shape[3] ** -0.5, -1).sum(0)
     return w
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,hq,hk,dim,page", [(1, 8, 2, 64, 16), (5, 16, 8, 128, 32), (40, 4, 1, 256, 8), (300, 3, 3, 72, 16)])
+def test_weights_of_the_tokens_that_stand(T, hq, hk, dim, page, dtype):
+    """add_weights takes each sequence's first tokens, and with all of them is what accumulate adds."""
+    lengths = [150, 0, -1, 64, 7, 1000]
+    cache, g = _cache(lengths, T, hk, dim, page, dtype, T + dim)
+    q = torch.randn(len(lengths), T, hq, dim, generator=g, device=DEV).to(dtype)
+    before = cache.scores[0].clone()
+    out, lse = cache.attend(q, return_lse=True)
+    for counts in (None, torch.tensor([T, 0, T, 1, max(1, T // 2), T + 9], dtype=torch.int32, device=DEV),
+                   torch.tensor([-4, 1, 1, T, T, 0], dtype=torch.int32, device=DEV)):
+        cache.scores[0].copy_(before)
+        cache.add_weights(q, lse, counts)
+        _check(cache, before, _weights(q, cache, counts))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # views are taken as they are, on another stream
+        cache.scores[0].copy_(before)
+        wide = torch.stack((q, q), -2).flatten(2, 3)[:, :, ::2]
+        cache.add_weights(wide, torch.stack((lse, lse), -1)[..., 0], scale=0.03)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.isfinite(cache.scores[0]).all()
+
+
+def test_add_weights_refusals():
+    from turbopress_b200 import _abi
+    from turbopress_b200.paged import PagedKVCache
+    cache = PagedKVCache(2, 2, 64, 4, 16, 2, track_weights=True)
+    q, lse = torch.zeros(2, 3, 4, 64, device=DEV).half(), torch.zeros(2, 3, 4, device=DEV)
+    n = torch.zeros(2, dtype=torch.int32, device=DEV)
+    for bad in (lambda: cache.add_weights(q[:1], lse[:1]), lambda: cache.add_weights(q.float(), lse), lambda: cache.add_weights(q, lse[:, :2]),
+                lambda: cache.add_weights(q, lse.double()), lambda: cache.add_weights(q, lse, n.long()), lambda: cache.add_weights(q, lse, n[:1]),
+                lambda: cache.add_weights(q, lse, n.cpu()), lambda: cache.add_weights(q, lse, layer=1),
+                lambda: cache.add_weights(q[:, :, :3], lse[:, :, :3]),
+                lambda: PagedKVCache(2, 2, 64, 4, 16, 2).add_weights(q, lse)):
+        with pytest.raises(ValueError):
+            bad()
+    cache.add_weights(q[:, :0], lse[:, :0])
+    assert _abi.lib().tp_paged_weights(None, None, None) == _abi.TP_ERR_ARG
+    assert (cache.scores == 0).all()
+
+
+def _decoder(batch, seed=3):
+    import numpy as np
+
+    from tests.conftest import GOLDEN
+    from turbopress_b200.paged import PagedKVCache
+    from turbopress_b200.paged_decoder import PagedDecoder
+    from turbopress_b200.synthetic import step_config, synthetic_decoder
+    cfg = dict(name="test", layers=2, hidden=1024, inter=2048, q_heads=16, kv_heads=8, head_dim=128, rope_theta=1_000_000.0,
+               qk_norm=True)
+    with np.load(GOLDEN / "codebooks.npz") as f:
+        cbs = {3: torch.from_numpy(f["opt_b3_s64"])}
+    layers, fnorm = synthetic_decoder(cfg, [3, 3], cbs, DEV, seed=seed)
+    cache = PagedKVCache(batch, 8, 128, batch * 8, 16, 8, layers=2, track_weights=True)
+    cache.block_table.copy_(torch.arange(batch * 8, device=DEV).view(batch, 8))
+    return PagedDecoder(layers, step_config(cfg), fnorm, cache)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_rejected_drafts_leave_no_weights(ragged):
+    """A bounded cache's weights after rounds with wrong drafts are those of the
+    emitted tokens alone, taken one by one (1 % of a weight: the linears of one
+    and of five rows round apart; the drafts' rows would add several times
+    that)."""
+    from turbopress_b200.speculative import DraftVerifier
+    g = torch.Generator(device=DEV).manual_seed(5)
+    V, B = 500, 2
+    emb = torch.randn(V, 1024, generator=g, device=DEV).half()
+    head = (emb * 0.05).contiguous()
+    prompt = torch.randint(0, V, (B, 40), generator=g, device=DEV)
+    none = torch.zeros(B, 0, dtype=torch.int64, device=DEV)
+    alone, drafting = _decoder(B), _decoder(B)
+    for dec in (alone, drafting):
+        dec.step(torch.nn.functional.embedding(prompt, emb), accumulate=True)
+        dec.cache.advance(40)
+    last = torch.tensor([3, 4], device=DEV)
+    plain, ver = [last.tolist()], DraftVerifier(B, 0, V)
+    for _ in range(3):
+        _, out = alone.speculative_step(last, none, emb, head, ver, accumulate=True)
+        last = out[:, 0].contiguous()
+        plain.append(last.tolist())
+    # the same three tokens in one round: two drafts that stand and two that do not (or are not in use)
+    drafts = torch.tensor([[plain[1][b], plain[2][b], (plain[3][b] + 1) % V, 7] for b in range(B)], device=DEV)
+    counts = torch.tensor([2, 4], dtype=torch.int32, device=DEV) if ragged else None
+    accepted, out = drafting.speculative_step(torch.tensor(plain[0], device=DEV), drafts, emb, head, DraftVerifier(B, 4, V),
+                                              accumulate=True, n_drafts=counts)
+    assert accepted.tolist() == [2, 2] and out[:, 2].tolist() == plain[3]
+    assert torch.equal(alone.cache.lengths, drafting.cache.lengths)
+    a, d = alone.cache.scores, drafting.cache.scores
+    assert (a[..., 43:] == 0).all() and (d[..., 43:] == 0).all()
+    assert float(((a - d).abs() / a.clamp(min=0.05))[..., :43].max()) < 1e-2

@@ -72,6 +72,7 @@ SIGNATURES: dict[str, tuple] = {
     "tp_paged_attn_workspace_bytes": (_I64, [_P, _I, _I, _I]),
     "tp_paged_attn": (_I, [_P, _P, _P, _I64, _P]),
     "tp_paged_attn_status": (_I, [_P, _P]),
+    "tp_paged_weights": (_I, [_P, _P, _P]),
     "tp_cache_evict_workspace_bytes": (_I64, [_P, _I]),
     "tp_cache_evict": (_I, [_P, _P, _P, _I64, _P]),
     "tp_verify_workspace_bytes": (_I64, [_I, _I, _I]),

@@ -83,7 +83,10 @@ struct AttnParams {
   float2* part_ml; // [ctas][2][16*MT]
   float* lse2;     // log2 units (accumulate only): [batch][tokens][q_heads], with stored scores [batch][kv_heads][rows]
   float* sbuf;     // [index space][16*MT][TILE] scores in log2 units (stored scores only)
-  const void* k_pages;  // and its strides, in elements (accumulate only)
+  // the weights kernel's
+  float lse_unit;        // what lse2 is taken times
+  const int32_t* counts; // [batch] step tokens whose weights are added, or NULL: all
+  const void* k_pages;   // and its strides, in elements
   int64_t page_stride, head_stride, token_stride;
 };
 
@@ -879,7 +882,8 @@ __global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_
       n = tiles(len);
     }
     const int h = (t - before) / n, slot0 = ((t - before) - h * n) * S::TILE + warp * S::SLOTS;
-    const int rows = p.rows, hi = visible(p, len, rows - 1);
+    const int rows = p.counts ? max(0, min(p.counts[b], p.tokens)) * p.group : p.rows;
+    const int hi = rows ? visible(p, len, rows - 1) : 0;
     if (slot0 >= hi) continue;
     // the slots' K: this lane's row of each block, the chunks of 8 columns as in the attention kernel
     uint4 kf[NS][HD / 32];
@@ -927,7 +931,7 @@ __global__ void __launch_bounds__(kWtThreads) paged_weights_kernel(const __grid_
           const int64_t at = ((int64_t)b * p.tokens + j) * p.q_heads + h * p.group + row - j * p.group;
           const bool on = row < rows;
           const T* q = static_cast<const T*>(p.q) + at * p.head_dim;
-          z[e] = on ? p.lse2[at] : 0.f;
+          z[e] = on ? p.lse2[at] * p.lse_unit : 0.f;
           see[e] = on ? visible(p, len, row) : 0;
 #pragma unroll
           for (int kk = 0; kk < HD / 32; ++kk) {
@@ -1011,16 +1015,17 @@ __global__ void __launch_bounds__(kWtThreads) paged_stored_weights_kernel(const 
     float w = 0.f;
     const float* s = p.sbuf + (size_t)(base + h * (kItemCost + n) + kItemCost + tile) * RT * TILE + tok;
     const float* z = p.lse2 + ((int64_t)b * p.kv_heads + h) * p.rows;
-    for (int r = 0; r < p.rows; r += 16) {  // sixteen rows' loads together: one round trip for most calls
+    const int rows = min(RT, p.rows);  // (all of them; the bound lets the loop go where RT is 16)
+    for (int r = 0; r < rows; r += 16) {  // sixteen rows' loads together: one round trip for most calls
       float a[16], m[16];
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
-        const int at = min(r + k, p.rows - 1);
+        const int at = min(r + k, rows - 1);
         a[k] = s[at * TILE];
         m[k] = z[at];
       }
 #pragma unroll
-      for (int k = 0; k < 16; ++k) w += r + k < p.rows ? exp2_diff(a[k], m[k]) : 0.f;
+      for (int k = 0; k < 16; ++k) w += r + k < rows ? exp2_diff(a[k], m[k]) : 0.f;
     }
     *score = was + w;
   }
@@ -1116,6 +1121,16 @@ tp_status page_map(const tp_paged_cache* c, void* base, bool panels, int box, CU
   return TP_OK;
 }
 
+template <class T, int HD>
+tp_status launch_weights(const AttnParams& p, cudaStream_t st) {
+  int sms = 0;
+  const tp_status s = device_sms(&sms);
+  if (s != TP_OK) return s;
+  const int64_t tiles = (int64_t)p.batch * p.kv_heads * ((p.capacity + WtShape::TILE - 1) / WtShape::TILE);
+  return launch_early(paged_weights_kernel<T, HD>, dim3(static_cast<unsigned>(std::min<int64_t>(8 * sms, tiles))), kWtThreads, 0,
+                      st, "paged_weights launch", p);
+}
+
 template <class T, int HD, int MT, bool STORE>
 tp_status launch_attn(const AttnParams& p, const PaPlan& pl, cudaStream_t st) {
   using S = PaShape<HD, MT>;
@@ -1138,12 +1153,11 @@ tp_status launch_attn(const AttnParams& p, const PaPlan& pl, cudaStream_t st) {
   const int grid = static_cast<int>(std::min<int64_t>(std::min(kPaMaxCtas, sms * occ), pl.positions));
   s = launch_early(kern, dim3(grid), S::THREADS, S::kSmem, st, "paged_attn launch", p);
   if (s != TP_OK || !p.lse2) return s;
-  auto blocks = [&](int64_t tiles) { return dim3(static_cast<unsigned>(std::min<int64_t>(8 * sms, tiles))); };
   if constexpr (STORE)
-    return launch_early(paged_stored_weights_kernel<S>, blocks(pl.max_tiles), kWtThreads, 0, st, "paged_stored_weights launch", p);
+    return launch_early(paged_stored_weights_kernel<S>, dim3(static_cast<unsigned>(std::min<int64_t>(8 * sms, pl.max_tiles))),
+                        kWtThreads, 0, st, "paged_stored_weights launch", p);
   else
-    return launch_early(paged_weights_kernel<T, HD>, blocks(pl.max_tiles * (S::TILE / WtShape::TILE)), kWtThreads, 0, st,
-                        "paged_weights launch", p);
+    return launch_weights<T, HD>(p, st);
 }
 
 template <class T, int HD>
@@ -1158,6 +1172,31 @@ tp_status dispatch_dim(const AttnParams& p, const PaPlan& pl, cudaStream_t st) {
   if (pl.hd == 64) return dispatch_rows<T, 64>(p, pl, st);
   if (pl.hd == 128) return dispatch_rows<T, 128>(p, pl, st);
   return dispatch_rows<T, 256>(p, pl, st);
+}
+
+// What both launches need of a call.
+void fill_params(const tp_paged_cache* c, int tokens, int q_heads, float scale, AttnParams* p) {
+  p->block_table = c->block_table;
+  p->lengths = c->lengths;
+  p->scores = c->scores;
+  p->num_pages = c->num_pages;
+  p->table_stride = c->table_stride;
+  p->batch = c->batch;
+  p->tokens = tokens;
+  p->q_heads = q_heads;
+  p->kv_heads = c->kv_heads;
+  p->group = q_heads / c->kv_heads;
+  p->head_dim = c->head_dim;
+  p->lg_page = log2_int(c->page_size);
+  p->capacity = c->max_pages * c->page_size;
+  p->group_inv = p->group == 1 ? 0 : ~uint64_t(0) / p->group + 1;
+  p->rows = tokens * p->group;
+  p->scale_log2 = scale * 1.4426950408889634f;
+  p->lse_unit = 1.f;
+  p->k_pages = c->k_pages;
+  p->page_stride = c->page_stride;
+  p->head_stride = c->head_stride;
+  p->token_stride = c->token_stride;
 }
 
 }  // namespace
@@ -1193,41 +1232,44 @@ TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_ca
   s = page_map(cache, cache->k_pages, p.panels, box, &p.k_map);
   if (s == TP_OK) s = page_map(cache, cache->v_pages, p.panels, box, &p.v_map);
   if (s != TP_OK) return s;
+  fill_params(cache, a.tokens, a.q_heads, a.softmax_scale, &p);
   p.q = a.q;
   p.out = a.out;
   p.lse = a.lse;
-  p.block_table = cache->block_table;
-  p.lengths = cache->lengths;
-  p.scores = cache->scores;
-  p.num_pages = cache->num_pages;
-  p.table_stride = cache->table_stride;
-  p.batch = cache->batch;
-  p.tokens = a.tokens;
-  p.q_heads = a.q_heads;
-  p.kv_heads = cache->kv_heads;
-  p.group = a.q_heads / cache->kv_heads;
-  p.head_dim = cache->head_dim;
-  p.lg_page = log2_int(cache->page_size);
-  p.capacity = cache->max_pages * cache->page_size;
-  p.group_inv = p.group == 1 ? 0 : ~uint64_t(0) / p.group + 1;
-  p.rows = a.tokens * p.group;
   p.row_tiles = (p.rows + 16 * pl.mt - 1) / (16 * pl.mt);
-  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   auto* ws = static_cast<unsigned char*>(workspace);
   p.counters = reinterpret_cast<unsigned*>(ws);
   p.status = reinterpret_cast<unsigned*>(ws + kPaStatusOff);
   p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_off);
   p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
-  if (a.accumulate) {
-    p.lse2 = reinterpret_cast<float*>(ws + pl.lse_off);
-    p.sbuf = pl.store ? reinterpret_cast<float*>(ws + pl.s_off) : nullptr;
-    p.k_pages = cache->k_pages;
-    p.page_stride = cache->page_stride;
-    p.head_stride = cache->head_stride;
-    p.token_stride = cache->token_stride;
-  }
+  if (a.accumulate) p.lse2 = reinterpret_cast<float*>(ws + pl.lse_off);
+  if (pl.store) p.sbuf = reinterpret_cast<float*>(ws + pl.s_off);
   cudaStream_t st = as_stream(stream);
   return cache->dtype == TP_F16 ? dispatch_dim<__half>(p, pl, st) : dispatch_dim<__nv_bfloat16>(p, pl, st);
+}
+
+TP_API tp_status tp_paged_weights(const tp_paged_weights_args* args, const tp_paged_cache* cache, void* stream) {
+  if (!args || !args->q || !args->lse) return fail(TP_ERR_ARG, "tp_paged_weights: null pointer");
+  const tp_paged_weights_args& a = *args;
+  tp_status s = check_cache(cache, "tp_paged_weights");
+  if (s != TP_OK) return s;
+  PaPlan pl;
+  s = plan_attn(cache, a.tokens, a.q_heads, 1, &pl);
+  if (s != TP_OK) return s;
+  if (!cache->scores) return fail(TP_ERR_ARG, "tp_paged_weights: the cache has no scores to accumulate in");
+  if (!aligned(a.q, 16)) return fail(TP_ERR_ALIGN, "tp_paged_weights: q must be 16-byte aligned");
+  AttnParams p{};
+  fill_params(cache, a.tokens, a.q_heads, a.softmax_scale, &p);
+  p.q = a.q;
+  p.lse2 = const_cast<float*>(a.lse);  // (only read)
+  p.lse_unit = 1.4426950408889634f;
+  p.counts = a.counts;
+  cudaStream_t st = as_stream(stream);
+  const auto launch = [&](auto t) {
+    using T = decltype(t);
+    return pl.hd == 64 ? launch_weights<T, 64>(p, st) : pl.hd == 128 ? launch_weights<T, 128>(p, st) : launch_weights<T, 256>(p, st);
+  };
+  return cache->dtype == TP_F16 ? launch(__half{}) : launch(__nv_bfloat16{});
 }
 
 TP_API tp_status tp_paged_attn_status(void* workspace, void* stream) {

@@ -43,6 +43,13 @@ class _AttnArgs(ctypes.Structure):
                 ("q_heads", ctypes.c_int32), ("softmax_scale", ctypes.c_float), ("accumulate", ctypes.c_int32)]
 
 
+class _WeightsArgs(ctypes.Structure):
+    """Mirror of ``tp_paged_weights_args``."""
+
+    _fields_ = [("q", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("tokens", ctypes.c_int32),
+                ("q_heads", ctypes.c_int32), ("softmax_scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
 class _EvictArgs(ctypes.Structure):
     """Mirror of ``tp_evict_args``."""
 
@@ -164,7 +171,8 @@ class PagedKVCache:
     def advance(self, tokens: int | Tensor) -> None:
         """Count ``tokens`` (a number, or int32 [batch]) as cached: after the
         last layer's ``append``.  Idle sequences stay idle.  Fewer than were
-        appended drops the last ones (rejected drafts)."""
+        appended drops the last ones (rejected drafts; ``add_weights`` for
+        their part in the accumulated weights)."""
         live = (self.lengths >= 0).int() * tokens
         self.lengths.add_(live)
         self.next_pos.add_(live)
@@ -174,8 +182,8 @@ class PagedKVCache:
         """Attention of a step's q [batch, tokens, q_heads, head_dim], already
         appended: token j sees the slots below ``lengths`` and the step's own
         tokens up to itself.  ``scale`` defaults to head_dim ** -0.5.
-        ``accumulate`` adds each slot's attention weight to ``scores``.  A row
-        that sees nothing (an idle sequence) gives zeros.  Returns out in q's
+        ``accumulate`` adds each slot's attention weight to ``scores`` (for
+        tokens that may be dropped again: ``add_weights``).  A row that sees nothing (an idle sequence) gives zeros.  Returns out in q's
         shape, with the fp32 log-sum-exp [batch, tokens, q_heads] on request."""
         key = (_abi.meta(q), scale, accumulate)
         plan = self._plans.get(key)
@@ -216,6 +224,29 @@ class PagedKVCache:
             _abi.check(-need, "attend")
         self._ws = self._grown(self._ws, need)
         return template
+
+    def add_weights(self, q: Tensor, lse: Tensor, counts: Tensor | None = None, *, layer: int = 0, scale: float | None = None) -> None:
+        """What ``attend(q, accumulate=True)`` adds to ``scores``, for the first
+        ``counts`` int32 [batch] tokens of each sequence (None: all), from the
+        log-sum-exp that ``attend(q, return_lse=True)`` gave: for drafts, once
+        it is known how many stand and before ``advance``."""
+        if q.dim() != 4 or q.shape[0] != self.batch or q.shape[3] != self.head_dim or q.dtype != self.dtype or q.device != self.device:
+            raise ValueError(f"expected q [{self.batch}, tokens, heads, {self.head_dim}] {self.dtype} on {self.device}, got "
+                             f"{tuple(q.shape)} {q.dtype} on {q.device}")
+        if self.scores is None:
+            raise ValueError("the cache keeps no scores to accumulate in")
+        if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.device != self.device:
+            raise ValueError(f"lse must be float32 {tuple(q.shape[:3])} on {self.device}")
+        if counts is not None and (counts.shape != (self.batch,) or counts.dtype != torch.int32 or counts.device != self.device):
+            raise ValueError(f"counts must be int32 [{self.batch}] on {self.device}")
+        addr = self._layer(layer)
+        if not q.shape[1]:
+            return
+        q, lse = q.contiguous(), lse.contiguous()
+        counts = None if counts is None else counts.contiguous()
+        a = _WeightsArgs(q.data_ptr(), lse.data_ptr(), _abi.ptr(counts), q.shape[1], q.shape[2],
+                         self.head_dim ** -0.5 if scale is None else scale, 0)
+        _abi.launch(_abi.lib().tp_paged_weights, "add_weights", self.device.index, ctypes.addressof(a), addr)
 
     def _grown(self, ws: Tensor | None, need: int) -> Tensor:
         """``ws`` if it holds ``need`` bytes, else a zero-filled one that does."""

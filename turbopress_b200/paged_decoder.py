@@ -51,11 +51,13 @@ class PagedDecoder:
         self.final_norm = on_device(final_norm)
         self.norms = [tuple(on_device(w) for w in (lw.ln1, lw.ln2, lw.q_norm, lw.k_norm)) for lw in layers]
 
-    def step(self, embeddings: Tensor, accumulate: bool = False) -> Tensor:
+    def step(self, embeddings: Tensor, accumulate: bool = False, held: list[tuple[Tensor, Tensor]] | None = None) -> Tensor:
         """[batch, tokens, hidden] input embeddings of each sequence's next
         tokens -> the final norm's output for each.  The tokens are in the
         cache behind ``lengths`` afterwards; ``cache.advance`` counts them.
-        ``accumulate``: add to the cache's attention weights."""
+        ``accumulate``: add to the cache's attention weights.  ``held``: takes
+        each layer's queries and log-sum-exp, for ``cache.add_weights`` once it
+        is known which of the tokens stay."""
         cfg, cache = self.cfg, self.cache
         B, T, _ = embeddings.shape
         h = embeddings.to(torch.float16)
@@ -65,7 +67,12 @@ class PagedDecoder:
             k = lw.k(x).view(B, T, cfg.kv_heads, cfg.head_dim)
             v = lw.v(x).view(B, T, cfg.kv_heads, cfg.head_dim)
             q = cache.append(self.rotary, q, k, v, layer=i, q_norm=q_norm, k_norm=k_norm, eps=cfg.rms_eps)
-            h = h + lw.o(cache.attend(q, layer=i, accumulate=accumulate).view(B, T, -1))
+            if held is None:
+                out = cache.attend(q, layer=i, accumulate=accumulate)
+            else:
+                out, lse = cache.attend(q, layer=i, accumulate=accumulate, return_lse=True)
+                held.append((q, lse))
+            h = h + lw.o(out.view(B, T, -1))
             x = _rms_norm(h, ln2, cfg.rms_eps)
             h = h + lw.down(F.silu(lw.gate(x)) * lw.up(x))
         return _rms_norm(h, self.final_norm, cfg.rms_eps)
@@ -77,9 +84,14 @@ class PagedDecoder:
         the drafts verified against the logits (``random``: uniforms, noise,
         draft_probs, temperature, n_drafts as ``DraftVerifier`` takes them).
         Returns (accepted [batch], tokens [batch, drafts + 1]); the cache holds
-        the token and the accepted drafts."""
+        the token and the accepted drafts, and with ``accumulate`` their
+        attention weights."""
         ids = torch.cat((tokens[:, None], drafts), 1)
-        hidden = self.step(F.embedding(ids, embedding), accumulate)
+        held: list[tuple[Tensor, Tensor]] | None = [] if accumulate else None
+        hidden = self.step(F.embedding(ids, embedding), held=held)
         accepted, out = verifier(F.linear(hidden, lm_head), drafts, **random)
-        self.cache.advance(accepted + 1)
+        stay = accepted + 1
+        for i, (q, lse) in enumerate(held or ()):
+            self.cache.add_weights(q, lse, stay, layer=i)
+        self.cache.advance(stay)
         return accepted, out
