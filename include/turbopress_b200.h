@@ -489,6 +489,9 @@ typedef struct tp_paged_attn_args {
   float softmax_scale;
   int32_t accumulate;   /* add each seen slot's probability, summed over the step's rows
                            of its kv head, to cache->scores                               */
+  int32_t wait_polls;   /* limit of the waits for copies, 0: the default                  */
+  int32_t wait_hold;    /* 0; n > 0: in each block one of the fetching warps stops before
+                           its tile n - 1, a wait that nothing ends (tests of the limit)  */
 } tp_paged_attn_args;
 
 /* Workspace of tp_paged_attn for a cache's sizes (batch, kv_heads, head_dim,
@@ -517,9 +520,12 @@ typedef struct tp_paged_weights_args {
 TP_API tp_status tp_paged_weights(const tp_paged_weights_args* args, const tp_paged_cache* cache, void* stream);
 
 /* Reads (synchronizing `stream`) and clears the status word of a workspace of
- * tp_paged_attn: TP_OK, or TP_ERR_DEVICE when a wait for a copy gave up (rows
- * of that call are NaN, and what they added to the scores; the workspace is
- * fit for the next). */
+ * tp_paged_attn: TP_OK, or TP_ERR_DEVICE when a wait for a copy gave up.  The
+ * rows that it cut short are NaN then, and what they added to the scores; the
+ * block had stopped fetching and waited, again with a limit, for the copies it
+ * had begun, so the workspace and the context are fit for the next call.  Bit 1
+ * of the status in the message says that this second wait ran out too: a copy
+ * never came back, and nothing can be promised. */
 TP_API tp_status tp_paged_attn_status(void* workspace, void* stream);
 
 /* Eviction: of each sequence's slots keep the `budget` that come first by

@@ -105,3 +105,62 @@ def test_gemv_noalloc_status_ok_after_calls():
         lin.block, lin.bits, lin.n_states, st), "noalloc")
     _abi.check(lib.tp_gemv_noalloc_status(st), "noalloc status")
     assert torch.isfinite(y.float()).all()
+
+
+def _held_cache(dim, hq, hk, T, page=16, track=False):
+    from turbopress_b200.paged import PagedKVCache
+    g = torch.Generator(device=DEV).manual_seed(dim + hq)
+    pages = 6000 // page + 2
+    cache = PagedKVCache(2, hk, dim, 2 * pages, page, pages, track_weights=track)
+    cache.block_table.copy_(torch.randperm(2 * pages, generator=g, device=DEV).view(2, pages))
+    cache.k_pages.normal_(generator=g)
+    cache.v_pages.normal_(generator=g)
+    cache.lengths.copy_(torch.tensor([6000, 60], dtype=torch.int32))
+    return cache, torch.randn(2, T, hq, dim, device=DEV, generator=g).half()
+
+
+@pytest.mark.parametrize("dim,hq,hk,T", [(128, 8, 2, 1), (64, 8, 1, 1), (256, 4, 2, 1), (128, 8, 1, 4), (128, 8, 1, 12), (256, 8, 1, 3)])
+@pytest.mark.parametrize("hold", [1, 2, 3])
+def test_paged_attention_gives_up_its_wait(dim, hq, hk, T, hold):
+    """One fetching warp of each block stops before a tile (nothing else is
+    wrong: every other copy comes): the consumers' wait runs out, the block
+    stops fetching, waits for what is in flight and ends; the rows are NaN, the
+    status says so once, and the next call is right."""
+    from turbopress_b200.paged import PagedKVCache
+    cache, q = _held_cache(dim, hq, hk, T)
+    # 96 sequences over the same pages: every block has many more than three tiles
+    many = PagedKVCache.from_tensors(cache.k_pages[0], cache.v_pages[0], cache.block_table[:1].repeat(96, 1).contiguous(),
+                                     torch.full((96,), 6000, dtype=torch.int32, device=DEV))
+    qm = q[:1].expand(96, T, hq, dim).contiguous()
+    want = many.attend(qm)
+    many.status()
+    many.set_wait(polls=2000, hold=hold)
+    out = many.attend(qm)
+    with pytest.raises(RuntimeError, match=r"wait.*status 1\)"):
+        many.status()
+    many.status()  # cleared by reading it
+    # a sequence has at least 47 tiles: one of its parts comes after some block's third
+    assert torch.isnan(out).any(-1).any(-1).any(-1).all()
+    same = torch.isnan(out) | (out == want)
+    assert same.all()  # what is not NaN is what it was
+    many.set_wait()
+    assert torch.equal(many.attend(qm), want)
+    many.status()
+
+
+def test_paged_attention_gives_up_with_weights():
+    cache, q = _held_cache(128, 16, 8, 2, track=True)
+    want = cache.attend(q, accumulate=True)
+    first = cache.scores.clone()
+    cache.scores.zero_()
+    cache.set_wait(polls=2000, hold=1)
+    out = cache.attend(q, accumulate=True)
+    with pytest.raises(RuntimeError, match="wait"):
+        cache.status()
+    assert torch.isnan(out[0]).all() and torch.isnan(cache.scores[0, 0, :, :6002]).all()
+    cache.set_wait()
+    cache.scores.zero_()
+    assert torch.equal(cache.attend(q, accumulate=True), want) and torch.equal(cache.scores, first)
+    for bad in (dict(polls=-1), dict(polls=10, hold=-1), dict(hold=1)):
+        with pytest.raises(ValueError):
+            cache.set_wait(**bad)

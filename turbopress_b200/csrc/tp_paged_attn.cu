@@ -79,6 +79,8 @@ struct AttnParams {
   float scale_log2;
   unsigned* counters;
   unsigned* status;
+  unsigned polls;  // limit of a wait
+  int hold;        // a test's: one producer stops before tile hold - 1 of its block (0: none does)
   float* part_o;   // [ctas][2][16*MT][HD]
   float2* part_ml; // [ctas][2][16*MT]
   float* lse2;     // log2 units (accumulate only): [batch][tokens][q_heads], with stored scores [batch][kv_heads][rows]
@@ -312,6 +314,49 @@ struct PaShape {
   static_assert(W * 16 * HD * 4 == kStage, "the join buffer reuses a consumed stage");
 };
 
+// A stage's barrier; false when the wait runs out.
+//
+// What happens then: a consumer that gave up neither waits nor hands stages back
+// any more, so the producers run dry within the ring and give up too, and the
+// rows it has a part in become NaN.  Consumers still go through their items
+// (they meet at the ends, and other blocks may wait to be counted), and before
+// the block ends the producers make up the arrivals of the tiles that some of
+// them had begun and wait, with a limit, for what is in flight.
+__device__ __forceinline__ bool stage_wait(uint64_t* bar, unsigned parity, unsigned polls) {
+  const uint32_t a = smem_u32(bar);
+  for (unsigned i = 0; i < polls; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+
+template <int N>
+__device__ __forceinline__ void block_end_sync() {  // of all N threads, producers and consumers
+  asm volatile("bar.sync 2, %0;" ::"n"(N) : "memory");
+}
+
+// The producers' end of a block that gave up: the arrivals of the tiles [fetched,
+// most) that others began and this one did not (no stage is more than a round
+// ahead, and none of these was handed back), then a wait for what is in flight.
+__device__ __noinline__ void settle(uint64_t* full, int stages, int fetched, const int* all_fetched, unsigned* status) {
+  int most = 0;
+  for (int i = 0; i < 4; ++i) most = max(most, all_fetched[i]);
+  for (int i = fetched; i < most; ++i)
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&full[i % stages]);
+  for (int i = max(0, most - stages); i < most; ++i)
+    if (!mbar_wait(&full[i % stages], (i / stages) & 1)) atomicOr(status, 2u);
+}
+// A test's held wait: until another of the block's waits runs out.
+__device__ __noinline__ void hold_wait(unsigned polls, const volatile int& gone) {
+  for (unsigned i = 0; i < polls && !gone; ++i) __nanosleep(1000);
+}
+
 template <int N>
 __device__ __forceinline__ void consumers_sync() {  // of N threads; the producers never join
   asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
@@ -328,9 +373,12 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
   __shared__ uint32_t s_valid[kStages][W];  // the tokens of a block of 16 that have a page
   __shared__ float s_m[W][16], s_l[W][16];
   __shared__ bool s_last;
+  __shared__ volatile int s_gone;  // a wait ran out
+  __shared__ int s_fetched[4];     // tiles that each producer began
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sbase = smem_u32(smem);
   if (tid == 0) {
+    s_gone = 0;
     asm volatile("prefetch.tensormap [%0];" ::"l"(&p.k_map) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&p.v_map) : "memory");
     for (int i = 0; i < kStages; ++i) {
@@ -345,7 +393,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
   Cursor c;
   pdl_wait();
   pdl_trigger();  // after the wait: the weights kernel of stored scores reads the lengths at once
-  // (its barriers also publish the mbarriers)
+  // (its barriers also publish the mbarriers and s_gone)
   if (!find_share<W + 4>(p, [&](int len) { return seq_size<S>(p, len); }, s_tmp, per, t0, t1, c.b, c.len, before)) return;
   int rem = t0 - before;
   for (c.rt = 0;; ++c.rt) {
@@ -361,7 +409,8 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
   }
   if (t0 >= t1) return;
   int stage = 0, t = t0;
-  unsigned phase = 0;
+  unsigned phase = 0;  // parity of the stage's round; a consumer's has kGaveUp set once its wait ran out
+  constexpr unsigned kGaveUp = 2;
   auto next_stage = [&] {
     if (++stage == kStages) {
       stage = 0;
@@ -383,11 +432,17 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
       const int tok = c.tile * S::TILE + at;
       return mine && tok < p.capacity ? p.block_table[c.b * p.table_stride + (tok >> p.lg_page)] : -1;
     };
-    int pid = page_of();
+    int pid = page_of(), fetched = 0;
     while (true) {
-      if (!mbar_wait(&s_empty[stage], phase ^ 1u)) {  // (the first round of the ring does not wait)
-        atomicOr(p.status, 1u);
-        return;
+      bool go = stage_wait(&s_empty[stage], phase ^ 1u, p.polls);  // (the first round of the ring does not wait)
+      if (p.hold && p.hold == fetched + 1 && warp == W + 1) {
+        hold_wait(p.polls, s_gone);
+        go = false;
+      }
+      if (!__all_sync(0xffffffffu, go)) {
+        s_gone = 1;
+        if (lane == 0) atomicOr(p.status, 1u);
+        break;
       }
       const uint32_t bar = smem_u32(&s_full[stage]);
       const int tok = c.tile * S::TILE + at;
@@ -412,19 +467,23 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
           tma_box(d + S::kKV + i * 2048, &p.v_map, i * 64, tok & page_mask, c.h, pid, bar);
         }
       }
+      ++fetched;
       t += c.tile + 1 == c.n ? 1 + kItemCost : 1;
-      if (t >= t1) return;
+      if (t >= t1) break;
       step_cursor<S>(p, c);
       pid = page_of();
       next_stage();
     }
+    if (lane == 0) s_fetched[warp - W] = fetched;
+    block_end_sync<S::THREADS>();
+    if (s_gone) settle(s_full, kStages, fetched, s_fetched, p.status);
+    return;
   }
   if (W == 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
 
   // ---- the consumers: this warp's 16 rows ----
   const int mt = warp / WT, tw = warp % WT;
   const int r0 = lane >> 2, cq = lane & 3;  // this thread: rows r0, r0 + 8, columns 2 cq + {0, 1} of each 8
-  bool dead = false;
   // Fragments of the queries.  A product may take the columns in any order
   // that both operands share: this thread holds the 16-byte chunks 2 cq and
   // 2 cq + 1 of each 64 columns, so both operands load 16 bytes at a time.
@@ -479,8 +538,9 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
 
     while (true) {
       const uint32_t st = sbase + stage * S::kStage;
-      if (!dead && !mbar_wait(&s_full[stage], phase)) {
-        dead = true;  // reported through the status word; the outputs become NaN
+      if (phase < kGaveUp && !stage_wait(&s_full[stage], phase, p.polls)) {
+        phase |= kGaveUp;  // reported through the status word
+        s_gone = 1;
         atomicOr(p.status, 1u);
       }
       // this warp's MT blocks of 16 tokens, NB at a time
@@ -496,7 +556,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
         bool whole = true;  // every slot seen by every row
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          valid[i] = s_valid[stage][blk + i];
+          valid[i] = phase >= kGaveUp ? 0xffffu : s_valid[stage][blk + i];
           whole = whole && valid[i] == 0xffffu && tok0 + 16 * (i + 1) <= vis_lo;
         }
         const uint32_t kb = st + blk * S::kBlock;
@@ -536,6 +596,12 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
             }
         }
         if (STORE) {
+          if (phase >= kGaveUp) {  // (what the slots hold is anything: their weights become NaN)
+#pragma unroll
+            for (int n = 0; n < 2 * NB; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[n][e] = s[n][e] == -INFINITY ? s[n][e] : __int_as_float(0x7fc00000);
+          }
 #pragma unroll
           for (int i = 0; i < NB; ++i) store_scores(blk + i, s + 2 * i);
         }
@@ -672,7 +738,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
       }
       if (t + 1 == t_end) break;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[stage]);
+      if (lane == 0 && phase < kGaveUp) mbar_arrive(&s_empty[stage]);
       ++t;
       ++c.tile;
       next_stage();
@@ -688,7 +754,7 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      if (dead) l[e] = __int_as_float(0x7fc00000);
+      if (__any_sync(0xffffffffu, phase >= kGaveUp)) l[e] = __int_as_float(0x7fc00000);  // (the products are the warp's)
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
       if (cq == 0) s_m[warp][r0 + 8 * e] = m[e];
@@ -833,11 +899,12 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
     // the join buffer goes back to the producers
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     consumers_sync<32 * W>();
-    if (lane == 0) mbar_arrive(&s_empty[stage]);
+    if (lane == 0 && phase < kGaveUp) mbar_arrive(&s_empty[stage]);
     t = t_next;
-    if (t >= t1) return;
+    if (t >= t1) break;
     next_stage();
   }
+  block_end_sync<S::THREADS>();
 }
 
 // ---------------------------------------------------------------------------
@@ -1220,6 +1287,8 @@ TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_ca
   s = plan_attn(cache, a.tokens, a.q_heads, a.accumulate, &pl);
   if (s != TP_OK) return s;
   if (a.accumulate && !cache->scores) return fail(TP_ERR_ARG, "tp_paged_attn: the cache has no scores to accumulate in");
+  if (a.wait_polls < 0 || a.wait_hold < 0 || (a.wait_hold && !a.wait_polls))
+    return fail(TP_ERR_ARG, "tp_paged_attn: bad wait limit (a held wait needs one of its own)");
   if (!aligned(a.q, 16) || !aligned(a.out, 16))
     return fail(TP_ERR_ALIGN, "tp_paged_attn: q and out must be 16-byte aligned");
   if (!workspace || workspace_bytes < pl.bytes || !aligned(workspace, 256))
@@ -1240,6 +1309,8 @@ TP_API tp_status tp_paged_attn(const tp_paged_attn_args* args, const tp_paged_ca
   auto* ws = static_cast<unsigned char*>(workspace);
   p.counters = reinterpret_cast<unsigned*>(ws);
   p.status = reinterpret_cast<unsigned*>(ws + kPaStatusOff);
+  p.polls = a.wait_polls > 0 ? static_cast<unsigned>(a.wait_polls) : kMaxPolls;
+  p.hold = a.wait_hold;
   p.part_ml = reinterpret_cast<float2*>(ws + pl.ml_off);
   p.part_o = reinterpret_cast<float*>(ws + pl.o_off);
   if (a.accumulate) p.lse2 = reinterpret_cast<float*>(ws + pl.lse_off);

@@ -40,7 +40,8 @@ class _AttnArgs(ctypes.Structure):
     """Mirror of ``tp_paged_attn_args``."""
 
     _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("tokens", ctypes.c_int32),
-                ("q_heads", ctypes.c_int32), ("softmax_scale", ctypes.c_float), ("accumulate", ctypes.c_int32)]
+                ("q_heads", ctypes.c_int32), ("softmax_scale", ctypes.c_float), ("accumulate", ctypes.c_int32),
+                ("wait_polls", ctypes.c_int32), ("wait_hold", ctypes.c_int32)]
 
 
 class _WeightsArgs(ctypes.Structure):
@@ -128,6 +129,7 @@ class PagedKVCache:
         self._evict_ws: Tensor | None = None
         self._outgrown: list[Tensor] = []  # workspaces that a captured graph may still use
         self._plans: dict[tuple, _AttnArgs] = {}
+        self._wait = (0, 0)
         self._append_plans: dict[Rotary, dict] = {}
         self._evict_bytes: dict[int, int] = {}
         self._slots = None if scores is None or positions is None else [(scores[i], positions[i]) for i in range(L)]
@@ -216,7 +218,7 @@ class PagedKVCache:
             raise ValueError("the cache keeps no scores to accumulate in")
         tokens, heads = q.shape[1], q.shape[2]
         template = _AttnArgs(tokens=tokens, q_heads=heads, softmax_scale=self.head_dim ** -0.5 if scale is None else scale,
-                             accumulate=accumulate)
+                             accumulate=accumulate, wait_polls=self._wait[0], wait_hold=self._wait[1])
         if tokens == 0:
             return template
         need = _abi.lib().tp_paged_attn_workspace_bytes(ctypes.addressof(self._structs[0]), tokens, heads, accumulate)
@@ -262,6 +264,16 @@ class PagedKVCache:
         """Raise if a device-side wait of an ``attend`` gave up (synchronizes)."""
         if self._ws is not None:
             _abi.launch(_abi.lib().tp_paged_attn_status, "attend", self.device.index, self._ws.data_ptr())
+
+    def set_wait(self, polls: int = 0, hold: int = 0) -> None:
+        """Polls after which an ``attend`` gives up waiting for a copy (0: the
+        default), and (``hold`` > 0) a copy of tile ``hold - 1`` of each block
+        that is never begun, so that the wait runs out.  Used to test that
+        path; every other run keeps 0."""
+        if polls < 0 or hold < 0 or (hold and not polls):
+            raise ValueError("polls and hold must be >= 0, and a hold needs its own polls")
+        self._wait = (polls, hold)
+        self._plans.clear()
 
     # -- a bounded cache --------------------------------------------------------
     def evict_slots(self, budget: int, *, recent: int = 0, sinks: int = 0, layer: int = 0) -> tuple[Tensor, Tensor, Tensor]:
