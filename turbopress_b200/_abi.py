@@ -155,6 +155,7 @@ def require_cuda(*tensors: torch.Tensor | None) -> torch.device:
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
 def meta(t: torch.Tensor | None) -> tuple | None:
@@ -162,8 +163,17 @@ def meta(t: torch.Tensor | None) -> tuple | None:
     return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
 
 
-def launch(fn, what: str, index: int, *args) -> None:
-    """``fn(*args, stream)`` on device ``index`` and its current stream."""
+def capturing(index: int) -> bool:
+    """Is device ``index``'s current stream recording a graph?"""
+    if _device() != index:
+        with torch.cuda.device(index):
+            return _capturing()
+    return _capturing()
+
+
+def launch(fn, what: str, index: int, *args) -> int:
+    """``fn(*args, stream)`` on device ``index`` and its current stream, which
+    is returned (0, the default stream, is never recorded into a graph)."""
     if _device() != index:
         with torch.cuda.device(index):
             return launch(fn, what, index, *args)
@@ -171,3 +181,4 @@ def launch(fn, what: str, index: int, *args) -> None:
     status = fn(*args, st)
     if status != TP_OK:
         check(status, what)
+    return st

@@ -127,7 +127,8 @@ class PagedKVCache:
             self.kv_heads, self.head_dim, self.page_size, self.max_pages, _abi.dtype_code(self.dtype)) for i in range(L)]
         self._ws: Tensor | None = None
         self._evict_ws: Tensor | None = None
-        self._outgrown: list[Tensor] = []  # workspaces that a captured graph may still use
+        self._captured: list[Tensor] = []  # workspaces of attend and of eviction that graphs were recorded with
+        self._evict_captured: list[Tensor] = []
         self._plans: dict[tuple, _AttnArgs] = {}
         self._wait = (0, 0)
         self._append_plans: dict[Rotary, dict] = {}
@@ -203,8 +204,10 @@ class PagedKVCache:
             a.q, a.out = q.data_ptr(), out.data_ptr()
             if lse is not None:
                 a.lse = lse.data_ptr()
-            _abi.launch(_abi.lib().tp_paged_attn, "attend", self.device.index, ctypes.addressof(a), addr, self._ws.data_ptr(),
-                        self._ws.numel())
+            st = _abi.launch(_abi.lib().tp_paged_attn, "attend", self.device.index, ctypes.addressof(a), addr, self._ws.data_ptr(),
+                             self._ws.numel())
+            if st and _abi.capturing(self.device.index):
+                self._keep(self._captured, self._ws)
         return (out, lse) if return_lse else out
 
     def _checked(self, q: Tensor, scale: float | None, accumulate: bool) -> _AttnArgs:
@@ -254,16 +257,29 @@ class PagedKVCache:
         """``ws`` if it holds ``need`` bytes, else a zero-filled one that does."""
         if ws is not None and ws.numel() >= need:
             return ws
-        if torch.cuda.is_current_stream_capturing():
+        if _abi.capturing(self.device.index):
             raise RuntimeError("the workspace has to grow: run this call once before capturing it")
-        if ws is not None:
-            self._outgrown.append(ws)
+        if ws is not None:  # the calls so far are on this stream or before it
+            ws.record_stream(torch.cuda.current_stream(self.device))
         return torch.zeros(need, dtype=torch.uint8, device=self.device)
 
+    @staticmethod
+    def _keep(kept: list[Tensor], ws: Tensor) -> None:
+        """A graph that is being recorded uses ``ws``: it stays, also when it is outgrown."""
+        if not kept or kept[-1] is not ws:
+            kept.append(ws)
+
     def status(self) -> None:
-        """Raise if a device-side wait of an ``attend`` gave up (synchronizes)."""
-        if self._ws is not None:
-            _abi.launch(_abi.lib().tp_paged_attn_status, "attend", self.device.index, self._ws.data_ptr())
+        """Raise if a device-side wait of an ``attend`` gave up, in a graph's
+        replay too (synchronizes)."""
+        failed = None
+        for ws in {id(w): w for w in (*self._captured, self._ws) if w is not None}.values():
+            try:
+                _abi.launch(_abi.lib().tp_paged_attn_status, "attend", self.device.index, ws.data_ptr())
+            except RuntimeError as e:  # (the others' words are read and cleared as well)
+                failed = failed or e
+        if failed is not None:
+            raise failed
 
     def set_wait(self, polls: int = 0, hold: int = 0) -> None:
         """Polls after which an ``attend`` gives up waiting for a copy (0: the
@@ -297,8 +313,10 @@ class PagedKVCache:
         scores, positions = self._slots[layer]
         new = (torch.empty_like(self.lengths), torch.empty_like(scores), torch.empty_like(positions))
         a = _EvictArgs(self.next_pos.data_ptr(), new[0].data_ptr(), new[1].data_ptr(), new[2].data_ptr(), budget, recent, sinks)
-        _abi.launch(lib.tp_cache_evict, "evict", self.device.index, ctypes.addressof(a), addr, self._evict_ws.data_ptr(),
-                    self._evict_ws.numel())
+        st = _abi.launch(lib.tp_cache_evict, "evict", self.device.index, ctypes.addressof(a), addr, self._evict_ws.data_ptr(),
+                         self._evict_ws.numel())
+        if st and _abi.capturing(self.device.index):
+            self._keep(self._evict_captured, self._evict_ws)
         return new
 
     def evict(self, budget: int, *, recent: int = 0, sinks: int = 0) -> None:
