@@ -93,6 +93,8 @@ def main(argv: list[str] | None = None) -> dict:
             noise=torch.empty(a.batch, a.vocab, device=dev).exponential_(generator=g))
         last = out.gather(1, accepted.long()[:, None])[:, 0].contiguous()
         for s, row, n in zip(said, out.tolist(), accepted.tolist()):
+            if row[n] < 0:
+                raise RuntimeError("the logits leave no token to draw (not finite?)")
             s += row[:n + 1]
             accepted_total += n
         rounds += 1

@@ -85,8 +85,11 @@ class PagedDecoder:
         draft_probs, temperature, n_drafts as ``DraftVerifier`` takes them).
         Returns (accepted [batch], tokens [batch, drafts + 1]); the cache holds
         the token and the accepted drafts, and with ``accumulate`` their
-        attention weights."""
-        ids = torch.cat((tokens[:, None], drafts), 1)
+        attention weights.  Ids outside the vocabulary are looked up as its
+        nearest: such a draft (padding behind n_drafts, say) is rejected, and a
+        next token of -1, of a row without any probability, is for the caller
+        to end the sequence at."""
+        ids = torch.cat((tokens[:, None], drafts), 1).clamp_(0, embedding.shape[0] - 1)
         held: list[tuple[Tensor, Tensor]] | None = [] if accumulate else None
         hidden = self.step(F.embedding(ids, embedding), held=held)
         accepted, out = verifier(F.linear(hidden, lm_head), drafts, **random)
