@@ -105,3 +105,22 @@ def test_a_graph_keeps_its_workspaces():
     with pytest.raises(RuntimeError, match="capturing"):
         with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
             cache.attend(larger, accumulate=True)
+
+
+def test_rotaries_of_the_past_are_let_go():
+    """A cache that meets many Rotary objects holds a few of them, and still takes each as it is."""
+    import gc
+    import weakref
+
+    from turbopress_b200.rotary import Rotary
+    cache, g = _cache()
+    q, kv = _q(g, 1, 4), _q(g, 1, 2)
+    seen = []
+    for i in range(40):
+        rotary = Rotary(64, theta=10000.0 + i)
+        want, _ = rotary(q, kv, cache.next_pos.long()[:, None])
+        assert torch.equal(cache.append(rotary, q, kv, kv), want)
+        seen.append(weakref.ref(rotary))
+    del rotary
+    gc.collect()
+    assert sum(r() is not None for r in seen) <= 16

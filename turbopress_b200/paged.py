@@ -155,6 +155,8 @@ class PagedKVCache:
         if plans is None:
             if rotary.device != self.device or rotary.head_dim != self.head_dim:
                 raise ValueError("the rotary's device and head_dim differ from the cache's")
+            if len(self._append_plans) >= 16:  # (a program has one, or one per kind of layer)
+                self._append_plans.clear()
             plans = self._append_plans[rotary] = {}
         a, out, keep = rotary._args(plans, self._appendable, q, k, v, positions, q_norm, k_norm, eps, inverse)
         if positions is None:
