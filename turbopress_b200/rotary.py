@@ -125,9 +125,15 @@ class Rotary:
 
     @classmethod
     def from_config(cls, config, device="cuda", interleaved: bool = False) -> "Rotary":
-        """From a Hugging Face decoder config (its theta, scaling and partial factor)."""
+        """From a Hugging Face decoder config (its theta, scaling and partial
+        factor).  A config with parameters for each kind of layer has a Rotary
+        for each of them, and is refused here."""
         head_dim = getattr(config, "head_dim", None) or config.hidden_size // config.num_attention_heads
         p = getattr(config, "rope_parameters", None) or getattr(config, "rope_scaling", None) or {}
+        kinds = [k for k, v in p.items() if isinstance(v, dict)]
+        if kinds:
+            raise ValueError(f"the config has rope parameters for each kind of layer ({', '.join(kinds)}): make a Rotary of each, "
+                             "Rotary(head_dim, theta=..., scaling=...)")
         theta = float(p.get("rope_theta") or getattr(config, "rope_theta", None) or 10000.0)
         part = float(p.get("partial_rotary_factor") or getattr(config, "partial_rotary_factor", None) or 1.0)
         if p and "original_max_position_embeddings" not in p and getattr(config, "max_position_embeddings", None):
