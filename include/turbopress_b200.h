@@ -563,7 +563,8 @@ TP_API tp_status tp_cache_evict(const tp_evict_args* args, const tp_paged_cache*
  * draft).  At the first rejection the next token is drawn from
  * max(p_k - q_k, 0) (from p_k should that be zero everywhere), after
  * acceptance of all from p_K: the token i of largest r_i / noise[i] (noise:
- * independent exponentials), lower i on equality.  With t = 0, drafts are
+ * independent exponentials), lower i on equality.  With t = 0 (or below the
+ * smallest normal fp32 value: their limit), drafts are
  * accepted while they are the argmax of their row (lower index on equality, a
  * NaN above all), and the next token is the argmax.  A draft outside the
  * vocabulary is rejected; a next token of -1 says that the row had none with

@@ -34,6 +34,7 @@ constexpr int kVfWarps = kVfThreads / 32;
 constexpr int kVfResident = 6;    // CTAs per SM
 constexpr int kVfMaxRows = 64;    // drafts + 1
 constexpr int kVfMaxSplits = 128;
+constexpr float kVfLeast = 1.17549435e-38f;  // temperatures below count as 0 (1 / t would pass fp32's range)
 // Vocabulary up to which the CTA that decides on a sequence also draws, without
 // a second launch: five sequences of 5003 tokens 9.8 us of GPU time so, 11.8 us
 // with it; of 16000 tokens 12.8 against 11.3 us.
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kVfThreads, kVfResident) verify_rows_kernel(co
   if (k > used) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float heat = p.a.temperature ? p.a.temperature[b] : 0.f;
-  const bool greedy = !(heat > 0.f);
+  const bool greedy = !(heat >= kVfLeast);
   const float c = greedy ? 0.f : 1.4426950408889634f / heat;
   const T* row = static_cast<const T*>(p.a.logits) + (int64_t)b * p.a.batch_stride + (int64_t)k * p.a.row_stride;
   const int per = (p.a.vocab + p.splits - 1) / p.splits;
