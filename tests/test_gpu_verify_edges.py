@@ -44,3 +44,18 @@ def test_the_smallest_temperatures(least):
     x["logits"][:, 0].scatter_(1, x["draft_tokens"][:, :1], 50.0)  # a first draft that stands
     done, n = _compare(x)
     assert done == n
+
+
+def test_every_sequence_of_many_calls():
+    """All dtypes, vocabularies and kinds of drafts, one sequence at a time, and how many were compared."""
+    done = total = 0
+    for dtype in (torch.float16, torch.bfloat16, torch.float32):
+        for B, K, V in ((5, 3, 5003), (3, 8, 1000), (40, 1, 257), (2, 63, 130), (1, 0, 9), (4, 2, 1), (2, 5, 7), (70, 2, 2049), (9, 4, 4001),
+                        (3, 4, 40003)):
+            for seed, (probs, heat, ragged) in enumerate([(True, 1.0, False), (False, 0.7, False), (True, 0.8, True), (False, 0.0, True)]):
+                x = _inputs(B, K, V, dtype, 900 + seed + B + K + V, probs, heat, ragged)
+                if B == 9:
+                    x["temperature"] = torch.tensor([0, 1, 0.5, 0, 2, 0.1, 100, 0, 1e-3], device=DEV)
+                d, n = _compare(x)
+                done, total = done + d, total + n
+    assert done >= 0.98 * total, (done, total)
