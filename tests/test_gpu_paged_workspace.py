@@ -125,3 +125,24 @@ def test_rotaries_of_the_past_are_let_go():
     del rotary
     gc.collect()
     assert sum(r() is not None for r in seen) <= 16
+
+
+def test_a_cache_keeps_its_tensors():
+    """Another tensor in the place of lengths would not reach the kernels: refused; in-place writes count."""
+    cache, g = _cache()
+    q = _q(g, 1, 4)
+    for name in ("lengths", "block_table", "k_pages", "v_pages", "scores", "positions"):
+        with pytest.raises(AttributeError, match="write into it"):
+            setattr(cache, name, getattr(cache, name).clone())
+    long = cache.attend(q)
+    cache.lengths -= 400
+    short = cache.attend(q)
+    assert not torch.equal(long, short)
+    cache.lengths[:] = 500
+    assert torch.equal(cache.attend(q), long)
+    cache.next_pos = torch.full((4,), 77, dtype=torch.int32, device=DEV)  # (read anew by every call)
+    kv = _q(g, 1, 2)
+    from turbopress_b200.rotary import Rotary
+    rotary = Rotary(64)
+    want, _ = rotary(q, kv, torch.full((4, 1), 77, device=DEV))
+    assert torch.equal(cache.append(rotary, q, kv, kv), want)

@@ -60,7 +60,18 @@ class _EvictArgs(ctypes.Structure):
 
 
 class PagedKVCache:
-    """Pages, block table and lengths of a batch of sequences, layer by layer."""
+    """Pages, block table and lengths of a batch of sequences, layer by layer.
+
+    The kernels have the addresses of its tensors: write into them (``copy_``,
+    indexing); another tensor in the place of one is refused."""
+
+    _FIXED = frozenset(("k_pages", "v_pages", "block_table", "lengths", "scores", "positions"))
+
+    def __setattr__(self, name: str, value) -> None:
+        if name in self._FIXED and self.__dict__.get(name, value) is not value:  # (an in-place operator gives back the same)
+            raise AttributeError(f"{name} keeps its tensor: write into it (cache.{name}.copy_(...)), or make another cache "
+                                 "with from_tensors")
+        object.__setattr__(self, name, value)
 
     def __init__(self, batch: int, kv_heads: int, head_dim: int, num_pages: int, page_size: int, max_pages: int, *,
                  layers: int = 1, dtype: torch.dtype = torch.float16, track_weights: bool = False, device="cuda") -> None:
