@@ -32,10 +32,10 @@
 // their V zeroed in registers, in the blocks where that can happen.
 //
 // Measured (B200): one sequence of 131071 tokens, 64 query and 8 kv heads of
-// 128, 85 us = 6.3 TB/s (0.96 of the measured HBM rate); 64 sequences of 100 to
-// 8000 tokens, 32 / 8 heads, 82 us = 5.9 TB/s (0.90); one of 1024 tokens 7.7 us,
+// 128, 86 us = 6.2 TB/s (0.95 of the measured HBM rate); 64 sequences of 100 to
+// 8000 tokens, 32 / 8 heads, 84 us = 5.8 TB/s (0.88); one of 1024 tokens 7.9 us,
 // a chain of latencies (launch, lengths, page ids, tile, part, join); 64 rows
-// over 32000 tokens 67 us (the warps' products).  One producer warp instead of
+// over 32000 tokens 66 us (the warps' products).  One producer warp instead of
 // four held the ragged batch at 90 us: a warp issues a box every 90 cycles or so.
 #include <cuda.h>
 
@@ -918,13 +918,13 @@ __global__ void __launch_bounds__(PaShape<HD, MT>::THREADS, 1) paged_attn_kernel
 // any of them.  Either way a slot's sum is made by one warp or thread, so the
 // result does not depend on timing.
 //
-// Measured: 512 tokens of 32 / 8 heads over 8000 slots 777 us, of which 365 are
+// Measured: 512 tokens of 32 / 8 heads over 8000 slots 823 us, of which 366 are
 // the attention; from stored scores 955 us and 580 MB of workspace, where the
 // sequence's K and V take 35 MB.
 // ---------------------------------------------------------------------------
 struct WtShape {
   static constexpr int W = kWtThreads / 32;
-  static constexpr int NS = 2;  // blocks of 8 slots per warp (four: 902 us, fewer CTAs fit)
+  static constexpr int NS = 2;  // blocks of 8 slots per warp (four: 16 % slower, fewer CTAs fit)
   static constexpr int SLOTS = 8 * NS;
   static constexpr int TILE = W * SLOTS;
 };
@@ -1134,8 +1134,8 @@ tp_status plan_attn(const tp_paged_cache* c, int tokens, int q_heads, int accumu
   pl.ml_off = take((int64_t)kPaMaxCtas * 2 * rt * 8);
   pl.o_off = take((int64_t)kPaMaxCtas * 2 * rt * pl.hd * 4);
   // Stored scores take rt * 4 bytes per slot of the capacity: for up to 32 rows
-  // (8000 slots of one sequence 33.5 us with the attention, 35.4 us from K; 16
-  // sequences, four rows 115 against 171 us; with 64 rows 45 against 38 us), and
+  // (8000 slots of one sequence 32 us with the attention, 35 us from K; 16
+  // sequences, four rows 114 against 171 us; with 64 rows 45 against 38 us), and
   // not where that workspace would grow past 1 GiB.
   const int64_t stored = pl.positions * rt * pl.tile * 4;
   pl.store = accumulate && rows <= 32 && stored <= kPaStoredMax;

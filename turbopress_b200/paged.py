@@ -14,7 +14,8 @@ held to a budget of slots by the attention weight each slot has received.
 ``lengths`` (slots in use; negative for an idle sequence) and ``next_pos`` (the
 next token's position) live on the device, so a step needs no host round trip.
 Every call runs on the current stream of the cache's device; one cache serves
-one stream at a time (its workspace is shared by its calls).
+one stream at a time (its workspace is shared by its calls).  No gradients are
+recorded.
 """
 
 from __future__ import annotations

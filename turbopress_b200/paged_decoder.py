@@ -37,7 +37,8 @@ class PagedDecoder:
 
     def __init__(self, layers: list[LayerWeights], cfg: StepConfig, final_norm: Tensor, cache: PagedKVCache,
                  rotary: Rotary | None = None) -> None:
-        """``rotary`` defaults to the configuration's plain one."""
+        """``rotary`` defaults to the configuration's plain one (it holds no
+        scaling: ``Rotary.from_config(config)`` for a checkpoint that has one)."""
         if cache.layers != len(layers) or (cache.kv_heads, cache.head_dim) != (cfg.kv_heads, cfg.head_dim):
             raise ValueError("the cache's layers, kv_heads and head_dim must be the decoder's")
         if cache.dtype != torch.float16:

@@ -11,7 +11,8 @@ tokens, with the per-head RMS norm that Qwen3 applies before it.
     q = cache.append(rotary, q, k, v)                     # the same, k and v into a PagedKVCache
 
 Angles are exact modulo one turn for every position (a 64-bit phase, not a
-32-bit product); arithmetic is fp32 with one rounding to the tensors' dtype.
+32-bit product); arithmetic is fp32 with one rounding to the tensors' dtype.  No
+gradients are recorded; ``inverse`` is the rotation's.
 """
 
 from __future__ import annotations
